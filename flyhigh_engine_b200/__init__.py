@@ -220,6 +220,14 @@ EXPORTS = [
     ("fhk_gmhs_scratch_floats", c_size_t, [c_int, c_int]),
     ("fhk_gmhs_noalloc", c_int, [c_void_p, c_void_p]),
     ("fhk_gmhs_noalloc_max_floats", c_size_t, []),
+    ("fhk_gated_ffn", c_int, [c_void_p, c_void_p]),
+    ("fhk_gated_ffn_scratch_bytes", c_size_t, [c_void_p]),
+    ("fhk_gated_ffn_grad", c_int, [c_void_p, c_void_p]),
+    ("fhk_gated_ffn_grad_scratch_bytes", c_size_t, [c_void_p]),
+    ("fhk_gated_ffn_wait_timeouts", ctypes.c_longlong, [c_int]),
+    ("fhk_residual_norm", c_int, [c_void_p, c_void_p]),
+    ("fhk_residual_norm_grad", c_int, [c_void_p, c_void_p]),
+    ("fhk_residual_norm_grad_scratch_bytes", c_size_t, [c_void_p]),
 ]
 
 

@@ -1,10 +1,13 @@
-"""The kernel-level C ABI (include/flyhigh_kernels.h) from Python: ctypes mirrors of its parameter structs and a 3x3
+"""The kernel-level C ABI (include/flyhigh_kernels.h) from Python: ctypes mirrors of its parameter structs, a 3x3
 conv on NHWC f16 device tensors, for hosts that drive the conv kernels without the session layer (and for bench.py's
-per-conv sweep). Device memory is torch's; the kernels run on the caller's CUDA stream."""
+per-conv sweep), and the row operators beside it: the gated feed-forward block (GatedFFN) and the residual norm
+(ResidualNorm), forward and gradient, on the rows of f16 or bf16 tensors. Device memory is torch's; the kernels run on
+the caller's CUDA stream."""
 from __future__ import annotations
 
 import ctypes
-from ctypes import Structure, c_float, c_int, c_longlong, c_void_p
+from ctypes import Structure, c_float, c_int, c_longlong, c_size_t, c_void_p
+from typing import NamedTuple, Optional
 
 import numpy as np
 
@@ -97,3 +100,336 @@ class Conv3x3:
             out = torch.zeros(self.out_shape(n, h, w), dtype=torch.float16, device=x.device)
         self.launch(self.params(x, out, res), torch.cuda.current_stream().cuda_stream)
         return out
+
+
+# ---- row operators ----
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
+NORMS = {"none": 0, "rms": 1, "layer": 2}
+
+
+class GatedFfnParams(Structure):  # FhGatedFfnParams
+    _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down", "y", "a", "g", "u")] + \
+        [(n, c_longlong) for n in ("x_pitch", "wg_pitch", "wu_pitch", "wd_pitch", "y_pitch", "h_pitch", "m")] + \
+        [(n, c_int) for n in ("cin", "hidden", "cout", "act", "dtype")] + \
+        [("scratch", c_void_p), ("scratch_bytes", c_size_t), ("wait_cycles", c_longlong)]
+
+
+class GatedFfnGradParams(Structure):  # FhGatedFfnGradParams
+    _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "g", "u", "a", "dy", "dx", "dw_gate", "dw_up",
+                                        "dw_down", "db_gate", "db_up", "db_down")] + \
+        [(n, c_longlong) for n in ("x_pitch", "wg_pitch", "wu_pitch", "wd_pitch", "h_pitch", "dy_pitch", "dx_pitch",
+                                   "dwg_pitch", "dwu_pitch", "dwd_pitch", "m")] + \
+        [(n, c_int) for n in ("cin", "hidden", "cout", "act", "dtype")] + \
+        [("scratch", c_void_p), ("scratch_bytes", c_size_t), ("wait_cycles", c_longlong)]
+
+
+class ResidualNormParams(Structure):  # FhResidualNormParams
+    _fields_ = [(n, c_void_p) for n in ("x", "f", "gate", "scale", "w_post", "b_post", "w_pre", "b_pre", "y", "h")] + \
+        [(n, c_longlong) for n in ("x_pitch", "f_pitch", "y_pitch", "h_pitch", "gate_pitch", "m")] + \
+        [(n, c_int) for n in ("c", "gates", "pre", "post")] + [("eps", c_float), ("dtype", c_int)]
+
+
+class ResidualNormGradParams(Structure):  # FhResidualNormGradParams
+    _fields_ = [(n, c_void_p) for n in ("dy", "dh", "y", "f", "gate", "scale", "w_post", "b_post", "w_pre", "dx", "df",
+                                        "dgate", "dscale", "dw_post", "db_post", "dw_pre", "db_pre")] + \
+        [(n, c_longlong) for n in ("dy_pitch", "dh_pitch", "y_pitch", "f_pitch", "gate_pitch", "dx_pitch", "df_pitch",
+                                   "dgate_pitch", "m")] + \
+        [(n, c_int) for n in ("c", "gates", "pre", "post")] + [("eps", c_float), ("dtype", c_int)] + \
+        [("scratch", c_void_p), ("scratch_bytes", c_size_t)]
+
+
+def empty_rows(shape, dtype, device="cuda"):
+    """An uninitialised tensor of rows for the row operators: shape (..., channels), each row beginning on a 16-byte
+    boundary (a pitch of channels rounded up to 8, as the feature maps of the convs)."""
+    import torch
+    *lead, c = shape
+    return torch.empty((*lead, _up8(c)), dtype=dtype, device=device)[..., :c]
+
+
+def _dtype_code(dtype) -> int:
+    import torch
+    if dtype == torch.float16:
+        return 0
+    if dtype == torch.bfloat16:
+        return 1
+    raise FlyHighError(f"row operators take float16 or bfloat16 tensors, not {dtype}")
+
+
+def _rows(name: str, t, channels: int, dtype, device):
+    """(pointer, pitch, rows) of a tensor of rows (..., channels); refuses what the kernels cannot address."""
+    if t.dtype != dtype or t.device != device:
+        raise FlyHighError(f"{name}: a {dtype} tensor on {device} is expected, got {t.dtype} on {t.device}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) < 1 or shape[-1] != channels:
+        raise FlyHighError(f"{name}: rows of {channels} channels are expected, got shape {tuple(shape)}")
+    m, pitch = 1, 0
+    if len(shape) == 2:
+        m, pitch = shape[0], stride[0]
+    else:
+        for n, st in zip(reversed(shape[:-1]), reversed(stride[:-1])):  # the leading dimensions as one of constant pitch
+            if n == 1:
+                continue
+            if m == 1:
+                pitch = st
+            elif st != pitch * m:
+                raise FlyHighError(f"{name}: its leading dimensions are not rows of one pitch (strides {stride})")
+            m *= n
+    ptr = t.data_ptr()
+    if m <= 1:
+        pitch = _up8(channels)
+    if m and ((channels > 1 and stride[-1] != 1) or pitch < channels or pitch & 7 or ptr & 15):
+        raise FlyHighError(f"{name}: rows must be contiguous, begin on 16-byte boundaries and not overlap (strides "
+                           f"{stride}, pointer {ptr:#x}); empty_rows allocates such tensors")
+    return ptr, pitch, m
+
+
+def _vector(name: str, t, n: int, dtype, device) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or tuple(t.shape) != (n,) or not t.is_contiguous() or t.data_ptr() & 15:
+        raise FlyHighError(f"{name}: a contiguous, 16-byte aligned {dtype} vector of {n} on {device} is expected, got "
+                           f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _launch(what: str, fn, p, device) -> None:
+    import torch
+    if torch.cuda.current_device() == device.index:
+        rc = fn(ctypes.byref(p), torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.byref(p), torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        raise FlyHighError(f"{what} failed: CUDA error {rc}")
+
+
+def _scratch(nbytes: int, device):
+    import torch
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+class GatedFFNSaved(NamedTuple):
+    """What a training forward call keeps for the gradient: gate and up projections and their activated product."""
+    g: object
+    u: object
+    a: object
+
+
+class GatedFFN:
+    """Gated feed-forward block on rows (the pixels of an NHWC map, or tokens):
+    y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down.
+
+    w_gate, w_up: [hidden][cin], w_down: [cout][hidden], biases [hidden], [hidden], [cout] or None: CUDA tensors of one
+    type (float16 or bfloat16), used where they lie (no copy: an optimiser may update them in place). act: silu, gelu
+    (erf), gelu_tanh, relu or sigmoid. x: (..., cin); every tensor's rows begin on 16-byte boundaries (empty_rows).
+    No autograd: forward / backward are called by the training step."""
+
+    def __init__(self, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu"):
+        if act not in ACTIVATIONS:
+            raise FlyHighError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+        if w_gate.dim() != 2 or w_down.dim() != 2 or not w_gate.is_cuda:
+            raise FlyHighError("the weights are CUDA matrices")
+        self.dtype, self.device, self.act = w_gate.dtype, w_gate.device, act
+        self.hidden, self.cin = w_gate.shape
+        self.cout = w_down.shape[0]
+        self.weights = (w_gate, w_up, w_down)
+        self.biases = (b_gate, b_up, b_down)
+        code = _dtype_code(self.dtype)
+        wg, wgp, mg = _rows("w_gate", w_gate, self.cin, self.dtype, self.device)
+        wu, wup, mu = _rows("w_up", w_up, self.cin, self.dtype, self.device)
+        wd, wdp, _ = _rows("w_down", w_down, self.hidden, self.dtype, self.device)
+        if mg != mu or w_up.dim() != 2 or min(self.hidden, self.cin, self.cout) < 1:
+            raise FlyHighError(f"w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and w_down {tuple(w_down.shape)} do not match")
+        bias = [_vector(n, b, k, self.dtype, self.device) for n, b, k in
+                (("b_gate", b_gate, self.hidden), ("b_up", b_up, self.hidden), ("b_down", b_down, self.cout))]
+        self._common = dict(w_gate=wg, w_up=wu, w_down=wd, wg_pitch=wgp, wu_pitch=wup, wd_pitch=wdp, cin=self.cin,
+                            hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[act], dtype=code, h_pitch=_up8(self.hidden))
+        self._fixed = dict(self._common, b_gate=bias[0], b_up=bias[1], b_down=bias[2])
+
+    def _out(self, name, t, lead, channels, m):
+        if t is None:
+            t = empty_rows((*lead, channels), self.dtype, self.device)
+        ptr, pitch, rows = _rows(name, t, channels, self.dtype, self.device)
+        if rows != m:
+            raise FlyHighError(f"{name}: {m} rows are expected, got {rows}")
+        return t, ptr, pitch
+
+    def _forward(self, x, out, keep: bool):
+        import torch
+        xp, x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
+        y, yp, y_pitch = self._out("out", out, x.shape[:-1], self.cout, m)
+        hp = _up8(self.hidden)
+        hid = torch.empty((3 if keep else 1, m, hp), dtype=self.dtype, device=self.device)
+        p = GatedFfnParams(x=xp, x_pitch=x_pitch, y=yp, y_pitch=y_pitch, a=hid.data_ptr(), m=m, **self._fixed)
+        if keep:
+            p.g, p.u = hid.data_ptr() + 2 * m * hp, hid.data_ptr() + 4 * m * hp
+        scratch = _scratch(lib().fhk_gated_ffn_scratch_bytes(ctypes.byref(p)), self.device)
+        if scratch is not None:
+            p.scratch, p.scratch_bytes = scratch.data_ptr(), scratch.numel()
+        _launch("gated_ffn", lib().fhk_gated_ffn, p, self.device)
+        return y, hid
+
+    def __call__(self, x, out=None):
+        """y for x (inference: nothing is kept)."""
+        return self._forward(x, out, False)[0]
+
+    def forward(self, x, out=None):
+        """(y, saved): y, and what `backward` needs beside x."""
+        y, hid = self._forward(x, out, True)
+        a, g, u = (h[:, :self.hidden] for h in hid)
+        return y, GatedFFNSaved(g, u, a)
+
+    def backward(self, dy, x, saved: GatedFFNSaved, want=None) -> dict:
+        """The gradients for dy of the call that returned `saved`: "x", "w_gate", "w_up", "w_down" and the biases' there
+        are, or those of them that `want` lists. They are new tensors, each written whole."""
+        names = ["x", "w_gate", "w_up", "w_down"] + [n for n, b in zip(("b_gate", "b_up", "b_down"), self.biases) if b is not None]
+        if want is not None:
+            if not set(want) <= set(names):
+                raise FlyHighError(f"gradients of {sorted(set(want) - set(names))} are not among {names}")
+            names = [n for n in names if n in set(want)]
+        xp, x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
+        dyp, dy_pitch, mdy = _rows("dy", dy, self.cout, self.dtype, self.device)
+        hid = [_rows(n, t, self.hidden, self.dtype, self.device) for n, t in zip(("g", "u", "a"), saved)]
+        if mdy != m or any(h[2] != m or (m > 1 and h[1] != hid[0][1]) for h in hid):
+            raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({[h[2] for h in hid]}) are not of one call")
+        p = GatedFfnGradParams(x=xp, x_pitch=x_pitch, dy=dyp, dy_pitch=dy_pitch, g=hid[0][0], u=hid[1][0], a=hid[2][0], m=m,
+                               **self._common)
+        p.h_pitch = hid[0][1]
+        r = {}
+        for n in names:
+            if n == "x":
+                r[n], p.dx, p.dx_pitch = self._out("dx", None, x.shape[:-1], self.cin, m)
+            elif n == "w_gate":
+                r[n], p.dw_gate, p.dwg_pitch = self._out("dw_gate", None, (self.hidden,), self.cin, self.hidden)
+            elif n == "w_up":
+                r[n], p.dw_up, p.dwu_pitch = self._out("dw_up", None, (self.hidden,), self.cin, self.hidden)
+            elif n == "w_down":
+                r[n], p.dw_down, p.dwd_pitch = self._out("dw_down", None, (self.cout,), self.hidden, self.cout)
+            else:
+                r[n] = empty_rows((self.cout if n == "b_down" else self.hidden,), self.dtype, self.device)
+                setattr(p, "d" + n, r[n].data_ptr())
+        scratch = _scratch(lib().fhk_gated_ffn_grad_scratch_bytes(ctypes.byref(p)), self.device)
+        if scratch is not None:
+            p.scratch, p.scratch_bytes = scratch.data_ptr(), scratch.numel()
+        _launch("gated_ffn gradient", lib().fhk_gated_ffn_grad, p, self.device)
+        return r
+
+
+class ResidualNorm:
+    """The join of a block with its residual stream and the next block's norm, one pass over the rows:
+    y = x + scale * gate * norm_post(f), h = norm_pre(y).
+
+    pre, post: "rms", "layer" or "none"; w_pre, b_pre, w_post, b_post, scale: vectors of `channels` or None (a norm
+    without them is only normalised). x, f: (..., channels); gate: (gates, channels) of any alignment, each of its rows
+    for an equal run of rows (one per image of a batch, say), or None. f None: y is x (the norm before a first block). No autograd."""
+
+    def __init__(self, channels: int, dtype, pre: str = "rms", post: str = "none", w_pre=None, b_pre=None, w_post=None,
+                 b_post=None, scale=None, eps: float = 1e-6):
+        for kind in (pre, post):
+            if kind not in NORMS:
+                raise FlyHighError(f"unknown norm {kind!r}: one of {', '.join(NORMS)}")
+        if not 1 <= channels <= 8192:
+            raise FlyHighError(f"residual norms take 1 to 8192 channels, not {channels}")
+        if not 0 <= eps < float("inf"):
+            raise FlyHighError(f"eps {eps} is not a finite number >= 0")
+        if (pre == "none" and (w_pre is not None or b_pre is not None)) or \
+                (post == "none" and (w_post is not None or b_post is not None)):
+            raise FlyHighError("a weight or bias was given for a norm that is none")
+        self.channels, self.dtype, self.pre, self.post, self.eps = channels, dtype, pre, post, float(eps)
+        self.params = {"w_pre": w_pre, "b_pre": b_pre, "w_post": w_post, "b_post": b_post, "scale": scale}
+        self._code = _dtype_code(dtype)
+        given = [t for t in self.params.values() if t is not None]
+        self._ptrs = {}
+        if given:
+            if not given[0].is_cuda:
+                raise FlyHighError("the norms' vectors are CUDA tensors")
+            self._ptrs = {n: _vector(n, t, channels, dtype, given[0].device) for n, t in self.params.items() if t is not None}
+        self.device = given[0].device if given else None
+
+    def _device(self, t):
+        if not t.is_cuda or (self.device is not None and t.device != self.device):
+            raise FlyHighError(f"a CUDA tensor on {self.device or 'a GPU'} is expected, got one on {t.device}")
+        return t.device
+
+    def _gate(self, gate, m, device):
+        if gate is None:
+            return None, 0, 0
+        if gate.dim() != 2:
+            raise FlyHighError(f"gate: (gates, {self.channels}) is expected, got {tuple(gate.shape)}")
+        n, c = gate.shape
+        if gate.dtype != self.dtype or gate.device != device or c != self.channels or \
+                (n > 1 and gate.stride(0) < c) or (c > 1 and gate.stride(1) != 1):
+            raise FlyHighError(f"gate: rows of {self.channels} {self.dtype} values on {device} are expected, got {gate.dtype} "
+                               f"{tuple(gate.shape)} (strides {gate.stride()}) on {gate.device}")
+        if n < 1 or m % n:
+            raise FlyHighError(f"gate: {n} rows do not divide the {m} rows")
+        return gate.data_ptr(), gate.stride(0) if n > 1 else c, n
+
+    def _like(self, name, t, lead, m, device):
+        if t is None:
+            t = empty_rows((*lead, self.channels), self.dtype, device)
+        ptr, pitch, rows = _rows(name, t, self.channels, self.dtype, device)
+        if rows != m:
+            raise FlyHighError(f"{name}: {m} rows are expected, got {rows}")
+        return t, ptr, pitch
+
+    def __call__(self, x, f=None, gate=None):
+        """(y, h); h is None where pre is "none", and y is x itself where f is None."""
+        dev = self._device(x)
+        xp, x_pitch, m = _rows("x", x, self.channels, self.dtype, dev)
+        p = ResidualNormParams(x=xp, x_pitch=x_pitch, m=m, c=self.channels, pre=NORMS[self.pre], post=NORMS[self.post],
+                               eps=self.eps, dtype=self._code, **self._ptrs)
+        y, h, lead = x, None, x.shape[:-1]
+        if f is not None:
+            _, p.f, p.f_pitch = self._like("f", f, lead, m, dev)
+            p.gate, p.gate_pitch, p.gates = self._gate(gate, m, dev)
+            y, p.y, p.y_pitch = self._like("y", None, lead, m, dev)
+        else:
+            if gate is not None or self.pre == "none":
+                raise FlyHighError("without f there is no gate, and a norm before the block")
+            p.post, p.scale, p.w_post, p.b_post = 0, None, None, None
+        if self.pre != "none":
+            h, p.h, p.h_pitch = self._like("h", None, lead, m, dev)
+        _launch("residual_norm", lib().fhk_residual_norm, p, dev)
+        return y, h
+
+    def backward(self, dy, dh, y, f=None, gate=None) -> dict:
+        """The gradients for dy and dh (either may be None: zero) of the call that returned y: "x", and with f "f",
+        "gate" where there is one, and those of the vectors there are. They are new tensors, each written whole."""
+        first = next((t for t in (dy, dh) if t is not None), None)
+        if first is None or (dh is not None and self.pre == "none"):
+            raise FlyHighError("dy or dh is needed, and dh only with a norm before the next block")
+        dev = self._device(first)
+        lead = first.shape[:-1]
+        m = _rows("dy", first, self.channels, self.dtype, dev)[2]
+        names = {n for n, t in self.params.items() if t is not None and (f is not None or n in ("w_pre", "b_pre"))}
+        p = ResidualNormGradParams(m=m, c=self.channels, pre=NORMS[self.pre], post=NORMS[self.post], eps=self.eps,
+                                   dtype=self._code, **{n: v for n, v in self._ptrs.items() if n != "b_pre" and
+                                                        (f is not None or n == "w_pre")})
+        if dy is not None:
+            _, p.dy, p.dy_pitch = self._like("dy", dy, lead, m, dev)
+        if dh is not None:
+            _, p.dh, p.dh_pitch = self._like("dh", dh, lead, m, dev)
+            _, p.y, p.y_pitch = self._like("y", y, lead, m, dev)
+        r = {}
+        r["x"], p.dx, p.dx_pitch = self._like("dx", None, lead, m, dev)
+        if f is not None:
+            _, p.f, p.f_pitch = self._like("f", f, lead, m, dev)
+            r["f"], p.df, p.df_pitch = self._like("df", None, lead, m, dev)
+            p.gate, p.gate_pitch, p.gates = self._gate(gate, m, dev)
+            if gate is not None:
+                r["gate"] = gate.new_empty(gate.shape)
+                p.dgate, p.dgate_pitch = r["gate"].data_ptr(), self.channels
+        else:
+            if gate is not None:
+                raise FlyHighError("without f there is no gate")
+            p.post = 0
+        for n in sorted(names):
+            r[n] = empty_rows((self.channels,), self.dtype, dev)
+            setattr(p, "d" + n, r[n].data_ptr())
+        scratch = _scratch(lib().fhk_residual_norm_grad_scratch_bytes(ctypes.byref(p)), dev)
+        if scratch is not None:
+            p.scratch, p.scratch_bytes = scratch.data_ptr(), scratch.numel()
+        _launch("residual_norm gradient", lib().fhk_residual_norm_grad, p, dev)
+        return r

@@ -123,6 +123,128 @@ size_t fhk_gmhs_scratch_floats(int h, int w);
 int fhk_gmhs_noalloc(const FhGmhsParams* p, void* stream);
 size_t fhk_gmhs_noalloc_max_floats(void);
 
+/* ---- row operators: channel-mixing blocks over the rows of a feature map (its pixels) or of a sequence ----
+ *
+ * No counterpart in the reference: layers for a host's own networks beside the convs above. A tensor is `rows` rows of
+ * `channels` values with a row pitch in elements: an NHWC view of contiguous pixels is one, its pitch the pixel pitch
+ * cs. Element type FH_F16 or FH_BF16, the same for every tensor of a call (weights, biases and gradients too). Every
+ * tensor begins on a 16-byte boundary and pitches are multiples of 8 elements; vectors are contiguous. Elements
+ * between a row's channels and its pitch are never read and never written. All products, sums, statistics and activations are held in
+ * f32. A call runs on the current device and on the given stream, allocates nothing, and leaves nothing behind:
+ * scratch is the caller's (16-byte aligned, contents of no meaning before or after), and calls that may overlap need
+ * scratch of their own. Results do not depend on timing: every sum has a fixed order. Invalid arguments are refused with
+ * cudaErrorInvalidValue before anything is launched. */
+#define FH_F16 0
+#define FH_BF16 1
+
+/* activations of the gated block */
+#define FH_ACT_SILU 0      /* g * sigmoid(g) */
+#define FH_ACT_GELU 1      /* g * Phi(g), by erf */
+#define FH_ACT_GELU_TANH 2 /* the tanh form of gelu */
+#define FH_ACT_RELU 3
+#define FH_ACT_SIGMOID 4   /* the plain gated linear unit */
+
+/* Gated feed-forward block: g = x w_gate^T + b_gate, u = x w_up^T + b_up, a = act(g) * u, y = a w_down^T + b_down.
+ * a is rounded to the element type before the down projection; so are g and u where they are kept. */
+typedef struct FhGatedFfnParams {
+    const void* x;         /* [m][cin] */
+    const void* w_gate;    /* [hidden][cin] */
+    const void* w_up;      /* [hidden][cin] */
+    const void* w_down;    /* [cout][hidden] */
+    const void* b_gate;    /* [hidden], or NULL: no bias; each bias on its own */
+    const void* b_up;      /* [hidden] or NULL */
+    const void* b_down;    /* [cout] or NULL */
+    void* y;               /* [m][cout] */
+    void* a;               /* [m][hidden], pitch h_pitch: written, and read back by the down projection */
+    void* g;               /* [m][hidden], pitch h_pitch: kept for the gradient, or NULL (then u is NULL too) */
+    void* u;
+    long long x_pitch, wg_pitch, wu_pitch, wd_pitch, y_pitch, h_pitch;
+    long long m;           /* rows, 0 .. 2^31 - 256; 0 is a call that does nothing */
+    int cin, hidden, cout; /* 1 .. 2^20 each */
+    int act;
+    int dtype;
+    void* scratch;         /* fhk_gated_ffn_scratch_bytes; NULL where that is 0 */
+    size_t scratch_bytes;
+    long long wait_cycles; /* bound of each wait inside the kernels, SM clock cycles; 0 = 2e9 (about a second) */
+} FhGatedFfnParams;
+int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream);
+size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p); /* of the sizes alone; pointers are not looked at */
+
+/* The block's gradient for dy, from x, the weights and what the forward call kept (g, u, a).
+ * da = dy w_down; dg = da * u * act'(g), du = da * act(g), both rounded to the element type;
+ * dx = dg w_gate + du w_up; dw_gate = dg^T x; dw_up = du^T x; dw_down = dy^T a; db_* the column sums of dg, du, dy.
+ * Each output may be NULL (not wanted). Every output is written, not added to. With m = 0 the weights' and biases'
+ * gradients are set to zero. */
+typedef struct FhGatedFfnGradParams {
+    const void *x, *w_gate, *w_up, *w_down, *g, *u, *a; /* as in FhGatedFfnParams */
+    const void* dy;                                     /* [m][cout] */
+    void* dx;                                           /* [m][cin] */
+    void *dw_gate, *dw_up, *dw_down;                    /* the weights' shapes */
+    void *db_gate, *db_up, *db_down;
+    long long x_pitch, wg_pitch, wu_pitch, wd_pitch, h_pitch, dy_pitch, dx_pitch, dwg_pitch, dwu_pitch, dwd_pitch;
+    long long m;
+    int cin, hidden, cout;
+    int act;
+    int dtype;
+    void* scratch;
+    size_t scratch_bytes;
+    long long wait_cycles;
+} FhGatedFfnGradParams;
+int fhk_gated_ffn_grad(const FhGatedFfnGradParams* p, void* stream);
+size_t fhk_gated_ffn_grad_scratch_bytes(const FhGatedFfnGradParams* p);
+/* Waits inside the block's kernels that ran out (the call's outputs are then not to be used) since the last reset, on
+ * the current device; reset != 0 zeroes the count. Returns -1 when the count cannot be read. */
+long long fhk_gated_ffn_wait_timeouts(int reset);
+
+/* norm kinds */
+#define FH_NORM_NONE 0
+#define FH_NORM_RMS 1   /* v / sqrt(mean(v^2) + eps) */
+#define FH_NORM_LAYER 2 /* (v - mean(v)) / sqrt(var(v) + eps) */
+
+/* The join of a block with its residual, and the next block's norm, in one pass over the rows:
+ * y = x + scale * gate * norm_post(f), h = norm_pre(y), with norm(v) = n * w + b of the normalised row n.
+ * h is formed from y before y is rounded. */
+typedef struct FhResidualNormParams {
+    const void* x;      /* [m][c] the residual stream */
+    const void* f;      /* [m][c] the block's output, or NULL: y = x (the norm before a first block; y is then NULL too) */
+    const void* gate;   /* [gates][c], row r uses gate row r / (m / gates), or NULL: 1. Any pitch >= c, any alignment */
+    const void* scale;  /* [c] or NULL: 1 */
+    const void *w_post, *b_post, *w_pre, *b_pre; /* [c] or NULL: 1 and 0 */
+    void* y;            /* [m][c]; may be x (in place) */
+    void* h;            /* [m][c], or NULL (then pre is FH_NORM_NONE) */
+    long long x_pitch, f_pitch, y_pitch, h_pitch, gate_pitch;
+    long long m;        /* rows, 0 .. 2^31 - 256 */
+    int c;              /* 1 .. 8192 */
+    int gates;          /* rows of gate, a divisor of m; 0 without one */
+    int pre, post;      /* FH_NORM_* */
+    float eps;          /* >= 0 */
+    int dtype;
+} FhResidualNormParams;
+int fhk_residual_norm(const FhResidualNormParams* p, void* stream);
+
+/* Its gradient for dy (of y) and dh (of h): d = dy + norm_pre'(dh), dx = d, df = norm_post'(scale * gate * d), and the
+ * parameters' gradients, from y and f (the normalised rows are formed again). Each output may be NULL. */
+typedef struct FhResidualNormGradParams {
+    const void *dy, *dh; /* [m][c]; either may be NULL (zero), dh is NULL where pre is FH_NORM_NONE */
+    const void* y;       /* [m][c] the forward call's y (its x where it had no f); NULL where pre is FH_NORM_NONE */
+    const void* f;       /* [m][c], or NULL where the forward call had none */
+    const void *gate, *scale, *w_post, *b_post, *w_pre;
+    void *dx, *df;       /* [m][c] */
+    void *dgate;         /* [gates][c], any pitch >= c */
+    void *dscale, *dw_post, *db_post, *dw_pre, *db_pre; /* [c] */
+    long long dy_pitch, dh_pitch, y_pitch, f_pitch, gate_pitch, dx_pitch, df_pitch, dgate_pitch;
+    long long m;
+    int c;
+    int gates;
+    int pre, post;
+    float eps;
+    int dtype;
+    void* scratch;       /* fhk_residual_norm_grad_scratch_bytes */
+    size_t scratch_bytes;
+} FhResidualNormGradParams;
+int fhk_residual_norm_grad(const FhResidualNormGradParams* p, void* stream);
+size_t fhk_residual_norm_grad_scratch_bytes(const FhResidualNormGradParams* p);
+
 #ifdef __cplusplus
 }
 #endif
