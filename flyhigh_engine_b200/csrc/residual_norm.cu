@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "fh_device.cuh"
 #include "fh_kernels.h"
@@ -27,6 +28,7 @@ using namespace rows;
 namespace {
 
 constexpr int kMaxC = 8192;
+constexpr int kForwardThreads = 1024, kGradThreads = 512;  // threads per SM that the registers are cut for
 
 // the sum over the LPR threads that share a row, in a fixed order, returned to all of them. LPR <= 32: within a warp;
 // above: over the CTA (LPR == its threads), red holding one float per warp and a buffer of its own for each call
@@ -128,10 +130,35 @@ __device__ __forceinline__ void add_vec(float (&v)[8], const void* w, long long 
     for (int j = 0; j < 8; j++) v[j] += t[j];
 }
 
+// A thread's own ring of rows in shared memory: asynchronous 16-byte copies of its chunks, STAGES - 1 rows ahead. A thread
+// reads back only what it copied, so no barrier is needed, and the rows in flight cost no registers. A chunk that is partly
+// (or wholly) outside its row copies the elements inside it and the rest is zero.
+template <typename T, int THREADS, int NCH, int TENSORS, int STAGES>
+struct Ring {
+    uint4* buf;
+    static constexpr size_t kBytes = (size_t)STAGES * TENSORS * NCH * THREADS * 16;
+    __device__ __forceinline__ uint4* slot(int stage, int tensor, int k) const {
+        return buf + ((stage * TENSORS + tensor) * NCH + k) * THREADS + threadIdx.x;
+    }
+    __device__ __forceinline__ void copy(int stage, int tensor, int k, const T* base, long long at, int valid) const {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(slot(stage, tensor, k));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(valid > 0 ? base + at : base),
+                     "r"(valid > 0 ? 2 * valid : 0)
+                     : "memory");
+    }
+    static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory"); }
+    __device__ __forceinline__ void read(int stage, int tensor, int k, float (&v)[8]) const {
+        unpack8<T>(*slot(stage, tensor, k), v);
+    }
+};
+
 // THREADS / LPR rows at a time per CTA
-template <typename T, int THREADS, int LPR, int NCH>
-__global__ void __launch_bounds__(THREADS) k_residual_norm(const FhResidualNormParams p, long long rows_per_gate) {
+template <typename T, int THREADS, int LPR, int NCH, int STAGES>
+__global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual_norm(const FhResidualNormParams p, long long rows_per_gate) {
     __shared__ float red[4 * 64];
+    extern __shared__ uint4 ring_mem[];
+    const Ring<T, THREADS, NCH, 2, STAGES> ring{ring_mem};
     constexpr int RPC = THREADS / LPR;
     const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const float inv_c = 1.0f / (float)p.c;
@@ -140,18 +167,33 @@ __global__ void __launch_bounds__(THREADS) k_residual_norm(const FhResidualNormP
     for (int k = 0; k < NCH; k++) valid[k] = max(0, min(8, p.c - 8 * (l + k * LPR)));
     const T* x = static_cast<const T*>(p.x);
     const T* f = static_cast<const T*>(p.f);
+    const long long first = (long long)blockIdx.x * RPC + sub, step = (long long)gridDim.x * RPC;
+    auto fetch = [&](long long row, int stage) {
+#pragma unroll
+        for (int k = 0; k < NCH; k++) {
+            const int vk = row < p.m ? valid[k] : 0, c = 8 * (l + k * LPR);
+            ring.copy(stage, 0, k, x, row * p.x_pitch + c, vk);
+            if (f) ring.copy(stage, 1, k, f, row * p.f_pitch + c, vk);
+        }
+        ring.commit();
+    };
+#pragma unroll
+    for (int q = 0; q < STAGES - 1; q++) fetch(first + q * step, q);
+    int stage = 0;
     // every thread of a CTA runs the same number of iterations: the sums are CTA-wide barriers or whole-warp shuffles
-    for (long long r0 = (long long)blockIdx.x * RPC; r0 < p.m; r0 += (long long)gridDim.x * RPC) {
-        const long long row = r0 + sub;
+    for (long long row = first; row - sub < p.m; row += step) {
         const bool on = row < p.m;
         float xv[NCH][8], fv[NCH][8];
         int vr[NCH];  // the channels of this thread's row
+        ring.wait();
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
-            const int vk = vr[k] = on ? valid[k] : 0, c = 8 * (l + k * LPR);
-            load8(x + (vk ? row * p.x_pitch + c : 0), vk, xv[k]);
-            if (f) load8(f + (vk ? row * p.f_pitch + c : 0), vk, fv[k]);
+            vr[k] = on ? valid[k] : 0;
+            ring.read(stage, 0, k, xv[k]);
+            if (f) ring.read(stage, 1, k, fv[k]);
         }
+        fetch(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
         if (f) {
             if (p.post != FH_NORM_NONE) normalise<LPR, NCH>(p.post, fv, vr, inv_c, p.eps, red);
             const long long grow = p.gate && on ? row / rows_per_gate * p.gate_pitch : 0;
@@ -214,49 +256,94 @@ struct Split {
 };
 
 // the CTA's column sums, part [cta][4][c]: (A1, A0), or with whole runs (sum gate A1, sum gate A0); then sum dh n_y, sum dh
-template <typename T, int THREADS, int LPR, int NCH>
-__global__ void __launch_bounds__(THREADS) k_residual_norm_grad(const FhResidualNormGradParams p, const Split sp,
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE>
+__global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_norm_grad(const FhResidualNormGradParams p, const Split sp,
                                                                  float* part) {
     constexpr int RPC = THREADS / LPR;
     __shared__ float red[6 * 64];
-    __shared__ float fold[LPR > 32 ? 1 : RPC * LPR * NCH * 8];
+    __shared__ float fold[RPC > 1 ? THREADS * NCH * 8 : 1];
+    extern __shared__ uint4 ring_mem[];
+    const Ring<T, THREADS, NCH, 4, STAGES> ring{ring_mem};
     const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const float inv_c = 1.0f / (float)p.c;
     int valid[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; k++) valid[k] = max(0, min(8, p.c - 8 * (l + k * LPR)));
     const T* f = static_cast<const T*>(p.f);
-    float a1[NCH][8], a0[NCH][8], g1[NCH][8], g0[NCH][8], b1[NCH][8], b0[NCH][8];
+    float a1[NCH][8], a0[NCH][8], b1[NCH][8], b0[NCH][8];
+    float g1[WHOLE ? NCH : 1][8], g0[WHOLE ? NCH : 1][8];
 #pragma unroll
     for (int k = 0; k < NCH; k++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) a1[k][j] = a0[k][j] = g1[k][j] = g0[k][j] = b1[k][j] = b0[k][j] = 0.0f;
+        for (int j = 0; j < 8; j++) {
+            a1[k][j] = a0[k][j] = b1[k][j] = b0[k][j] = 0.0f;
+            if (WHOLE) g1[k][j] = g0[k][j] = 0.0f;
+        }
+    // v summed over the CTA's row groups (in order), returned to all of them
+    auto over_rows = [&](float (&v)[8]) {
+        if (RPC == 1) return;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; j++) fold[(sub * 8 + j) * LPR + l] = v[j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float s = 0.0f;
+#pragma unroll 4
+            for (int i = 0; i < RPC; i++) s += fold[(i * 8 + j) * LPR + l];
+            v[j] = s;
+        }
+    };
 
-    const int first = sp.whole ? blockIdx.x * sp.per_cta : blockIdx.x / sp.slices;
-    const int last = sp.whole ? min(first + sp.per_cta, sp.groups) : first + 1;
+    const int first = WHOLE ? blockIdx.x * sp.per_cta : blockIdx.x / sp.slices;
+    const int last = WHOLE ? min(first + sp.per_cta, sp.groups) : first + 1;
     for (int grp = first; grp < last; grp++) {
         long long lo = (long long)grp * sp.len, hi = lo + sp.len;
-        if (!sp.whole) {
+        if (!WHOLE) {
             const int sl = blockIdx.x % sp.slices;
             const long long base = lo;
             lo = base + sp.len * sl / sp.slices;
             hi = base + sp.len * (sl + 1) / sp.slices;
         }
-        for (long long r0 = lo; r0 < hi; r0 += RPC) {
-            const long long row = r0 + sub;
+        auto fetch = [&](long long row, int stage) {
+#pragma unroll
+            for (int k = 0; k < NCH; k++) {
+                const int vk = row < hi ? valid[k] : 0, c = 8 * (l + k * LPR);
+                if (p.dy) ring.copy(stage, 0, k, static_cast<const T*>(p.dy), row * p.dy_pitch + c, vk);
+                if (p.dh) {
+                    ring.copy(stage, 1, k, static_cast<const T*>(p.dh), row * p.dh_pitch + c, vk);
+                    ring.copy(stage, 2, k, static_cast<const T*>(p.y), row * p.y_pitch + c, vk);
+                }
+                if (f) ring.copy(stage, 3, k, f, row * p.f_pitch + c, vk);
+            }
+            ring.commit();
+        };
+        if (WHOLE) asm volatile("cp.async.wait_all;\n" ::: "memory");  // the last run's copies, before their slots are reused
+#pragma unroll
+        for (int q = 0; q < STAGES - 1; q++) fetch(lo + sub + q * RPC, q);
+        int stage = 0;
+        for (long long row = lo + sub; row - sub < hi; row += RPC) {
             const bool on = row < hi;
             float d[NCH][8], dh[NCH][8], yv[NCH][8], fv[NCH][8];
             int vr[NCH];  // the channels of this thread's row
+            ring.wait();
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
-                const int vk = vr[k] = on ? valid[k] : 0, c = 8 * (l + k * LPR);
-                load8(static_cast<const T*>(p.dy) + (vk ? row * p.dy_pitch + c : 0), p.dy ? vk : 0, d[k]);
-                if (p.dh) {
-                    load8(static_cast<const T*>(p.dh) + (vk ? row * p.dh_pitch + c : 0), vk, dh[k]);
-                    load8(static_cast<const T*>(p.y) + (vk ? row * p.y_pitch + c : 0), vk, yv[k]);
+                vr[k] = on ? valid[k] : 0;
+                if (p.dy) {
+                    ring.read(stage, 0, k, d[k]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) d[k][j] = 0.0f;
                 }
-                if (f) load8(f + (vk ? row * p.f_pitch + c : 0), vk, fv[k]);
+                if (p.dh) {
+                    ring.read(stage, 1, k, dh[k]);
+                    ring.read(stage, 2, k, yv[k]);
+                }
+                if (f) ring.read(stage, 3, k, fv[k]);
             }
+            fetch(row + (STAGES - 1) * RPC, stage == 0 ? STAGES - 1 : stage - 1);
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
             if (p.dh) {
                 const float r = normalise<LPR, NCH>(p.pre, yv, vr, inv_c, p.eps, red);
 #pragma unroll
@@ -308,169 +395,181 @@ __global__ void __launch_bounds__(THREADS) k_residual_norm_grad(const FhResidual
             }
             if (LPR > 32) __syncthreads();
         }
-        if (sp.whole) {  // the run's dgate row, and its share of the sums over gate rows
+        if (WHOLE) {  // the run's dgate row, and its share of the sums over gate rows
             const long long grow = p.gate ? (long long)grp * p.gate_pitch : 0;
 #pragma unroll
-            for (int k = 0; k < NCH; k++) {
+            for (int k = 0; k < (WHOLE ? NCH : 1); k++) {
                 const int c = 8 * (l + k * LPR);
-                float t1[8], t0[8];
+                over_rows(a1[k]);
+                over_rows(a0[k]);
+                if (valid[k] && sub == 0) {
+                    if (p.dgate) {
+                        float q[8], w0[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    t1[j] = a1[k][j];
-                    t0[j] = a0[k][j];
-                    if (LPR <= 32 && RPC > 1) {  // rows of the CTA's other threads
-                        for (int w = 0; w < 2; w++) {
-                            __syncthreads();
-                            fold[sub * LPR + l] = w ? t0[j] : t1[j];
-                            __syncthreads();
-                            float s = 0.0f;
-                            for (int i = 0; i < RPC; i++) s += fold[i * LPR + l];
-                            (w ? t0[j] : t1[j]) = s;
+                        for (int j = 0; j < 8; j++) {
+                            q[j] = a1[k][j];
+                            w0[j] = a0[k][j];
                         }
+                        mul_vec<T>(q, p.w_post, c, valid[k]);
+                        if (p.b_post) {
+                            mul_vec<T>(w0, p.b_post, c, valid[k]);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) q[j] += w0[j];
+                        }
+                        mul_vec<T>(q, p.scale, c, valid[k]);
+                        T* dst = static_cast<T*>(p.dgate) + (long long)grp * p.dgate_pitch + c;
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (j < valid[k]) dst[j] = Elem<T>::from(q[j]);
                     }
-                    a1[k][j] = a0[k][j] = 0.0f;
+                    mul_gate<T>(a1[k], p, grow + c, valid[k]);
+                    mul_gate<T>(a0[k], p, grow + c, valid[k]);
                 }
-                if (!valid[k]) continue;
-                if (p.dgate && sub == 0) {
-                    float q[8], w0[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        q[j] = t1[j];
-                        w0[j] = t0[j];
-                    }
-                    mul_vec<T>(q, p.w_post, c, valid[k]);
-                    if (p.b_post) {
-                        mul_vec<T>(w0, p.b_post, c, valid[k]);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) q[j] += w0[j];
-                    }
-                    mul_vec<T>(q, p.scale, c, valid[k]);
-                    T* dst = static_cast<T*>(p.dgate) + (long long)grp * p.dgate_pitch + c;
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (j < valid[k]) dst[j] = Elem<T>::from(q[j]);
-                }
-                mul_gate<T>(t1, p, grow + c, valid[k]);
-                mul_gate<T>(t0, p, grow + c, valid[k]);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    // every row group of the CTA holds the run's whole sum: only the first keeps it
-                    g1[k][j] += sub == 0 ? t1[j] : 0.0f;
-                    g0[k][j] += sub == 0 ? t0[j] : 0.0f;
+                    // every row group of the CTA holds the run's whole sum: the first keeps it
+                    g1[k][j] += sub == 0 ? a1[k][j] : 0.0f;
+                    g0[k][j] += sub == 0 ? a0[k][j] : 0.0f;
+                    a1[k][j] = a0[k][j] = 0.0f;
                 }
             }
         }
     }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
 
     // the CTA's sums
     float* out = part + (long long)blockIdx.x * 4 * p.c;
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
+    auto put = [&](int q, float (&v)[NCH][8], bool summed) {
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
+            if (!summed) over_rows(v[k]);
             const int c = 8 * (l + k * LPR);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                float v = q == 0 ? (sp.whole ? g1[k][j] : a1[k][j])
-                          : q == 1 ? (sp.whole ? g0[k][j] : a0[k][j])
-                          : q == 2 ? b1[k][j] : b0[k][j];
-                if (LPR <= 32 && RPC > 1) {
-                    __syncthreads();
-                    fold[sub * LPR + l] = v;
-                    __syncthreads();
-                    if (sub == 0) {
-                        v = 0.0f;
-                        for (int i = 0; i < RPC; i++) v += fold[i * LPR + l];
-                    }
-                }
-                if (sub == 0 && j < valid[k]) out[(long long)q * p.c + c + j] = v;
-            }
+            for (int j = 0; j < 8; j++)
+                if (sub == 0 && j < valid[k]) out[(long long)q * p.c + c + j] = v[k][j];
         }
+    };
+    if constexpr (WHOLE) {
+        put(0, g1, true);
+        put(1, g0, true);
+    } else {
+        put(0, a1, false);
+        put(1, a0, false);
     }
+    put(2, b1, false);
+    put(3, b0, false);
 }
 
-// 32 columns per CTA, 8 threads per column over the CTAs' sums; blockIdx.y: 0 the post side, 1 the pre side
+// 32 columns per CTA and 32 warps over the CTAs' sums; blockIdx.y: 0 the post side, 1 the pre side. Up to 32 gate rows at a
+// time, each one's CTAs shared out over 32 / rows warps, whose sums are added in order.
 template <typename T>
-__global__ void __launch_bounds__(256) k_residual_norm_params(const FhResidualNormGradParams p, const Split sp,
-                                                              const float* part) {
-    __shared__ float s1[8][33], s0[8][33];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
-    const bool on = col < p.c;
-    auto sum = [&](int lo, int hi, int which) -> float2 {  // over CTAs lo .. hi, to the threads of w == 0
-        float v1 = 0.0f, v0 = 0.0f;
-        if (on)
-            for (int i = lo + w; i < hi; i += 8) {
-                v1 += part[((long long)i * 4 + which) * p.c + col];
-                v0 += part[((long long)i * 4 + which + 1) * p.c + col];
-            }
-        __syncthreads();
-        s1[w][threadIdx.x & 31] = v1;
-        s0[w][threadIdx.x & 31] = v0;
-        __syncthreads();
-        v1 = v0 = 0.0f;
-        for (int i = 0; i < 8; i++) {
-            v1 += s1[i][threadIdx.x & 31];
-            v0 += s0[i][threadIdx.x & 31];
-        }
-        return make_float2(v1, v0);
-    };
+__global__ void __launch_bounds__(1024) k_residual_norm_params(const FhResidualNormGradParams p, const Split sp,
+                                                               const float* part) {
+    pdl_wait();
+    __shared__ float2 s[32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    const bool on = col < p.c, post = blockIdx.y == 0;
     auto at = [&](const void* v, long long i, float none) { return v && on ? Elem<T>::to(static_cast<const T*>(v)[i]) : none; };
     auto put = [&](void* v, long long i, float x) {
-        if (v && on && w == 0) static_cast<T*>(v)[i] = Elem<T>::from(x);
+        if (v && on) static_cast<T*>(v)[i] = Elem<T>::from(x);
     };
-    if (blockIdx.y == 1) {
-        const float2 b = sum(0, sp.ctas, 2);
-        put(p.dw_pre, col, b.x);
-        put(p.db_pre, col, b.y);
-        return;
-    }
-    const float wp = at(p.w_post, col, 1.0f), bp = at(p.b_post, col, 0.0f), s = at(p.scale, col, 1.0f);
+    // the pre side and whole runs are one sum over all CTAs
+    const int groups = post && !sp.whole ? sp.groups : 1, slices = sp.ctas / groups;
+    const float wp = at(p.w_post, col, 1.0f), bp = at(p.b_post, col, 0.0f), sc = at(p.scale, col, 1.0f);
     float g1 = 0.0f, g0 = 0.0f;
-    if (sp.whole) {
-        const float2 a = sum(0, sp.ctas, 0);
-        g1 = a.x;
-        g0 = a.y;
-    } else {
-        for (int k = 0; k < sp.groups; k++) {
-            const float2 a = sum(k * sp.slices, (k + 1) * sp.slices, 0);
-            const float g = at(p.gate, (long long)k * p.gate_pitch + col, 1.0f);
-            put(p.dgate, (long long)k * p.dgate_pitch + col, s * (wp * a.x + bp * a.y));
-            g1 += g * a.x;
-            g0 += g * a.y;
+    for (int k0 = 0; k0 < groups; k0 += 32) {
+        const int batch = min(32, groups - k0), parts = 32 / batch;
+        float2 v = make_float2(0.0f, 0.0f);
+        if (on && warp < batch * parts) {
+            const int k = k0 + warp / parts, q = warp % parts;
+            const float* src = part + (post ? 0 : 2 * (long long)p.c) + col;
+            const int lo = k * slices + slices * q / parts, hi = k * slices + slices * (q + 1) / parts;
+#pragma unroll 8
+            for (int i = lo; i < hi; i++) {
+                v.x += src[(long long)i * 4 * p.c];
+                v.y += src[(long long)i * 4 * p.c + p.c];
+            }
         }
+        __syncthreads();
+        s[warp][lane] = v;
+        __syncthreads();
+        if (warp == 0)
+            for (int b = 0; b < batch; b++) {
+                float t1 = 0.0f, t0 = 0.0f;
+                for (int q = 0; q < parts; q++) {
+                    t1 += s[b * parts + q][lane].x;
+                    t0 += s[b * parts + q][lane].y;
+                }
+                if (post && !sp.whole) {
+                    const int k = k0 + b;
+                    const float g = at(p.gate, (long long)k * p.gate_pitch + col, 1.0f);
+                    if (p.gate) put(p.dgate, (long long)k * p.dgate_pitch + col, sc * (wp * t1 + bp * t0));
+                    t1 *= g;
+                    t0 *= g;
+                }
+                g1 += t1;
+                g0 += t0;
+            }
     }
-    put(p.dscale, col, wp * g1 + bp * g0);
-    put(p.dw_post, col, s * g1);
-    put(p.db_post, col, s * g0);
+    if (warp != 0) return;
+    if (post) {
+        put(p.dscale, col, wp * g1 + bp * g0);
+        put(p.dw_post, col, sc * g1);
+        put(p.db_post, col, sc * g0);
+    } else {
+        put(p.dw_pre, col, g1);
+        put(p.db_pre, col, g0);
+    }
 }
 
 constexpr int kSms = 148;
 
-template <typename T, int THREADS, int LPR, int NCH>
+// allows a kernel its dynamic shared memory, once per device
+template <typename K>
+cudaError_t allow(K kernel, size_t bytes, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return e;
+        done[dev].store(true, std::memory_order_release);
+    }
+    return cudaSuccess;
+}
+
+template <typename T, int THREADS, int LPR, int NCH, int STAGES>
 cudaError_t run_forward(const FhResidualNormParams& p, cudaStream_t st) {
+    static std::atomic<bool> done[64];
+    constexpr size_t smem = Ring<T, THREADS, NCH, 2, STAGES>::kBytes;
+    const cudaError_t e = allow(k_residual_norm<T, THREADS, LPR, NCH, STAGES>, smem, done);
+    if (e != cudaSuccess) return e;
     constexpr int RPC = THREADS / LPR;
     const long long want = (p.m + RPC - 1) / RPC;
-    const int grid = (int)std::min<long long>(want, (long long)kSms * 2048 / THREADS);
-    return fhk::launch(k_residual_norm<T, THREADS, LPR, NCH>, dim3(grid), dim3(THREADS), 0, st, p,
+    const int grid = (int)std::min<long long>(want, (long long)kSms * (kForwardThreads / THREADS));
+    return fhk::launch(k_residual_norm<T, THREADS, LPR, NCH, STAGES>, dim3(grid), dim3(THREADS), smem, st, p,
                        p.gate ? p.m / p.gates : p.m);
 }
 
 template <typename T>
 cudaError_t forward(const FhResidualNormParams& p, cudaStream_t st) {
     const int c8 = (p.c + 7) / 8;
-    if (c8 <= 8) return run_forward<T, 256, 8, 1>(p, st);
-    if (c8 <= 32) return run_forward<T, 256, 32, 1>(p, st);
-    if (c8 <= 64) return run_forward<T, 256, 32, 2>(p, st);
-    if (c8 <= 256) return run_forward<T, 128, 128, 2>(p, st);
-    if (c8 <= 512) return run_forward<T, 256, 256, 2>(p, st);
-    return run_forward<T, 512, 512, 2>(p, st);
+    if (c8 <= 8) return run_forward<T, 256, 8, 1, 4>(p, st);
+    if (c8 <= 32) return run_forward<T, 256, 32, 1, 4>(p, st);
+    if (c8 <= 64) return run_forward<T, 256, 32, 2, 3>(p, st);
+    if (c8 <= 128) return run_forward<T, 128, 128, 1, 4>(p, st);
+    if (c8 <= 256) return run_forward<T, 128, 128, 2, 3>(p, st);
+    if (c8 <= 512) return run_forward<T, 256, 256, 2, 3>(p, st);
+    return run_forward<T, 512, 512, 2, 3>(p, st);
 }
 
 Split split_of(long long m, int c, int gates, bool gate) {
     Split s{};
     s.groups = gate ? gates : 1;
     s.len = m / s.groups;
-    const int target = c > 2048 ? kSms : 2 * kSms;
+    // as many CTAs as are resident at once: kGradThreads threads per SM in CTAs of 128, 256 or 512 (grad())
+    const int target = kSms * (c > 2048 ? 1 : c > 1024 || c <= 256 ? 2 : 4);
     s.whole = s.groups > 1 && s.groups >= target;
     if (s.whole) {
         s.slices = 1;
@@ -484,27 +583,36 @@ Split split_of(long long m, int c, int gates, bool gate) {
     return s;
 }
 
-template <typename T, int THREADS, int LPR, int NCH>
-cudaError_t run_grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
-    return fhk::launch(k_residual_norm_grad<T, THREADS, LPR, NCH>, dim3(sp.ctas), dim3(THREADS), 0, st, p, sp,
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE>
+cudaError_t run_grad_as(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
+    static std::atomic<bool> done[64];
+    constexpr size_t smem = Ring<T, THREADS, NCH, 4, STAGES>::kBytes;
+    const cudaError_t e = allow(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE>, smem, done);
+    if (e != cudaSuccess) return e;
+    return fhk::launch(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE>, dim3(sp.ctas), dim3(THREADS), smem, st, p, sp,
                        static_cast<float*>(p.scratch));
+}
+template <typename T, int THREADS, int LPR, int NCH, int STAGES>
+cudaError_t run_grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
+    return sp.whole ? run_grad_as<T, THREADS, LPR, NCH, STAGES, true>(p, sp, st)
+                    : run_grad_as<T, THREADS, LPR, NCH, STAGES, false>(p, sp, st);
 }
 
 template <typename T>
 cudaError_t grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
     const int c8 = (p.c + 7) / 8;
     cudaError_t e;
-    if (c8 <= 8) e = run_grad<T, 256, 8, 1>(p, sp, st);
-    else if (c8 <= 32) e = run_grad<T, 256, 32, 1>(p, sp, st);
-    else if (c8 <= 128) e = run_grad<T, 128, 128, 1>(p, sp, st);
-    else if (c8 <= 256) e = run_grad<T, 256, 256, 1>(p, sp, st);
-    else if (c8 <= 512) e = run_grad<T, 512, 512, 1>(p, sp, st);
-    else e = run_grad<T, 512, 512, 2>(p, sp, st);
+    if (c8 <= 8) e = run_grad<T, 256, 8, 1, 3>(p, sp, st);
+    else if (c8 <= 32) e = run_grad<T, 256, 32, 1, 3>(p, sp, st);
+    else if (c8 <= 128) e = run_grad<T, 128, 128, 1, 3>(p, sp, st);
+    else if (c8 <= 256) e = run_grad<T, 256, 256, 1, 3>(p, sp, st);
+    else if (c8 <= 512) e = run_grad<T, 512, 512, 1, 3>(p, sp, st);
+    else e = run_grad<T, 512, 512, 2, 2>(p, sp, st);
     if (e != cudaSuccess) return e;
     const bool post = p.f && (p.dgate || p.dscale || p.dw_post || p.db_post), pre = p.dw_pre || p.db_pre;
     if (!post && !pre) return cudaSuccess;
-    // blockIdx.y selects the side; the post side's blocks return at once where nothing of it is wanted
-    return fhk::launch(k_residual_norm_params<T>, dim3((p.c + 31) / 32, 2), dim3(256), 0, st, p, sp,
+    fhk::PdlScope pdl(true);  // it waits for the kernel above
+    return fhk::launch(k_residual_norm_params<T>, dim3((p.c + 31) / 32, 2), dim3(1024), 0, st, p, sp,
                        static_cast<const float*>(p.scratch));
 }
 

@@ -34,19 +34,23 @@ struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };
 
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = Elem<T>::to2(w[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
 // 8 elements of a row, `valid` of them inside it (8: one 16-byte access; fewer: element by element, so that nothing
 // past the row's channels is touched). The rest read as 0.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
     if (valid >= 8) {
-        const uint4 q = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = Elem<T>::to2(w[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
+        unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = i < valid ? Elem<T>::to(p[i]) : 0.0f;

@@ -144,7 +144,8 @@ def empty_rows(shape, dtype, device="cuda"):
     boundary (a pitch of channels rounded up to 8, as the feature maps of the convs)."""
     import torch
     *lead, c = shape
-    return torch.empty((*lead, _up8(c)), dtype=dtype, device=device)[..., :c]
+    t = torch.empty((*lead, _up8(c)), dtype=dtype, device=device)
+    return t if c % 8 == 0 else t[..., :c]
 
 
 def _dtype_code(dtype) -> int:
@@ -177,11 +178,19 @@ def _rows(name: str, t, channels: int, dtype, device):
             m *= n
     ptr = t.data_ptr()
     if m <= 1:
-        pitch = _up8(channels)
-    if m and ((channels > 1 and stride[-1] != 1) or pitch < channels or pitch & 7 or ptr & 15):
+        pitch = (channels + 7) // 8 * 8
+    if (pitch < channels or pitch & 7 or ptr & 15 or (stride[-1] != 1 and channels > 1)) and m:
         raise FlyHighError(f"{name}: rows must be contiguous, begin on 16-byte boundaries and not overlap (strides "
                            f"{stride}, pointer {ptr:#x}); empty_rows allocates such tensors")
     return ptr, pitch, m
+
+
+def _like(name: str, t, m: int, channels: int, dtype, device):
+    """(pointer, pitch) of a tensor of m rows."""
+    ptr, pitch, rows = _rows(name, t, channels, dtype, device)
+    if rows != m:
+        raise FlyHighError(f"{name}: {m} rows are expected, got {rows}")
+    return ptr, pitch
 
 
 def _vector(name: str, t, n: int, dtype, device) -> Optional[int]:
@@ -193,20 +202,42 @@ def _vector(name: str, t, n: int, dtype, device) -> Optional[int]:
     return t.data_ptr()
 
 
-def _launch(what: str, fn, p, device) -> None:
-    import torch
-    if torch.cuda.current_device() == device.index:
-        rc = fn(ctypes.byref(p), torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(ctypes.byref(p), torch.cuda.current_stream().cuda_stream)
-    if rc != 0:
-        raise FlyHighError(f"{what} failed: CUDA error {rc}")
+class _Call:
+    """One entry point on the current stream of the tensors' device, and its scratch: the bytes by sizes are asked for
+    once per layer (`sizes`, a dict of its own), the memory is torch's, for this call alone."""
+
+    def __init__(self, what: str, name: str, scratch: Optional[str]):
+        self.what, self.name, self.scratch_name, self.fn = what, name, scratch, None
+
+    def __call__(self, p, device, sizes=None, key=None) -> None:
+        import torch
+        if self.fn is None:
+            if self.scratch_name is not None:
+                self.scratch_bytes = getattr(lib(), self.scratch_name)
+            self.fn = getattr(lib(), self.name)
+        ref, scratch = ctypes.byref(p), None
+        if sizes is not None:
+            n = sizes.get(key)
+            if n is None:
+                if len(sizes) >= 4096:
+                    sizes.clear()
+                n = sizes[key] = self.scratch_bytes(ref)
+            if n:
+                scratch = torch.empty(n, dtype=torch.uint8, device=device)
+                p.scratch, p.scratch_bytes = scratch.data_ptr(), n
+        if torch.cuda.current_device() == device.index:
+            rc = self.fn(ref, torch.cuda.current_stream().cuda_stream)
+        else:
+            with torch.cuda.device(device):
+                rc = self.fn(ref, torch.cuda.current_stream().cuda_stream)
+        if rc != 0:
+            raise FlyHighError(f"{self.what} failed: CUDA error {rc}")
 
 
-def _scratch(nbytes: int, device):
-    import torch
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+_gated_ffn = _Call("gated_ffn", "fhk_gated_ffn", "fhk_gated_ffn_scratch_bytes")
+_gated_ffn_grad = _Call("gated_ffn gradient", "fhk_gated_ffn_grad", "fhk_gated_ffn_grad_scratch_bytes")
+_residual_norm = _Call("residual_norm", "fhk_residual_norm", None)
+_residual_norm_grad = _Call("residual_norm gradient", "fhk_residual_norm_grad", "fhk_residual_norm_grad_scratch_bytes")
 
 
 class GatedFFNSaved(NamedTuple):
@@ -243,32 +274,29 @@ class GatedFFN:
             raise FlyHighError(f"w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and w_down {tuple(w_down.shape)} do not match")
         bias = [_vector(n, b, k, self.dtype, self.device) for n, b, k in
                 (("b_gate", b_gate, self.hidden), ("b_up", b_up, self.hidden), ("b_down", b_down, self.cout))]
-        self._common = dict(w_gate=wg, w_up=wu, w_down=wd, wg_pitch=wgp, wu_pitch=wup, wd_pitch=wdp, cin=self.cin,
-                            hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[act], dtype=code, h_pitch=_up8(self.hidden))
-        self._fixed = dict(self._common, b_gate=bias[0], b_up=bias[1], b_down=bias[2])
-
-    def _out(self, name, t, lead, channels, m):
-        if t is None:
-            t = empty_rows((*lead, channels), self.dtype, self.device)
-        ptr, pitch, rows = _rows(name, t, channels, self.dtype, self.device)
-        if rows != m:
-            raise FlyHighError(f"{name}: {m} rows are expected, got {rows}")
-        return t, ptr, pitch
+        common = dict(w_gate=wg, w_up=wu, w_down=wd, wg_pitch=wgp, wu_pitch=wup, wd_pitch=wdp, cin=self.cin,
+                      hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[act], dtype=code, h_pitch=_up8(self.hidden))
+        # the calls' parameter blocks with all that does not change from call to call
+        self._forward_params = GatedFfnParams(**common, b_gate=bias[0], b_up=bias[1], b_down=bias[2])
+        self._grad_params = GatedFfnGradParams(**common)
+        self._sizes, self._grad_sizes = {}, {}
 
     def _forward(self, x, out, keep: bool):
         import torch
-        xp, x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
-        y, yp, y_pitch = self._out("out", out, x.shape[:-1], self.cout, m)
-        hp = _up8(self.hidden)
+        p = GatedFfnParams.from_buffer_copy(self._forward_params)
+        p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
+        if out is None:
+            out = empty_rows((*x.shape[:-1], self.cout), self.dtype, self.device)
+            p.y, p.y_pitch = out.data_ptr(), _up8(self.cout)
+        else:
+            p.y, p.y_pitch = _like("out", out, m, self.cout, self.dtype, self.device)
+        hp = p.h_pitch
         hid = torch.empty((3 if keep else 1, m, hp), dtype=self.dtype, device=self.device)
-        p = GatedFfnParams(x=xp, x_pitch=x_pitch, y=yp, y_pitch=y_pitch, a=hid.data_ptr(), m=m, **self._fixed)
+        p.a, p.m = hid.data_ptr(), m
         if keep:
             p.g, p.u = hid.data_ptr() + 2 * m * hp, hid.data_ptr() + 4 * m * hp
-        scratch = _scratch(lib().fhk_gated_ffn_scratch_bytes(ctypes.byref(p)), self.device)
-        if scratch is not None:
-            p.scratch, p.scratch_bytes = scratch.data_ptr(), scratch.numel()
-        _launch("gated_ffn", lib().fhk_gated_ffn, p, self.device)
-        return y, hid
+        _gated_ffn(p, self.device, self._sizes, m)
+        return out, hid
 
     def __call__(self, x, out=None):
         """y for x (inference: nothing is kept)."""
@@ -288,31 +316,31 @@ class GatedFFN:
             if not set(want) <= set(names):
                 raise FlyHighError(f"gradients of {sorted(set(want) - set(names))} are not among {names}")
             names = [n for n in names if n in set(want)]
-        xp, x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
-        dyp, dy_pitch, mdy = _rows("dy", dy, self.cout, self.dtype, self.device)
+        p = GatedFfnGradParams.from_buffer_copy(self._grad_params)
+        p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
+        p.dy, p.dy_pitch, mdy = _rows("dy", dy, self.cout, self.dtype, self.device)
         hid = [_rows(n, t, self.hidden, self.dtype, self.device) for n, t in zip(("g", "u", "a"), saved)]
         if mdy != m or any(h[2] != m or (m > 1 and h[1] != hid[0][1]) for h in hid):
             raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({[h[2] for h in hid]}) are not of one call")
-        p = GatedFfnGradParams(x=xp, x_pitch=x_pitch, dy=dyp, dy_pitch=dy_pitch, g=hid[0][0], u=hid[1][0], a=hid[2][0], m=m,
-                               **self._common)
-        p.h_pitch = hid[0][1]
+        p.g, p.u, p.a, p.h_pitch, p.m = hid[0][0], hid[1][0], hid[2][0], hid[0][1], m
         r = {}
         for n in names:
             if n == "x":
-                r[n], p.dx, p.dx_pitch = self._out("dx", None, x.shape[:-1], self.cin, m)
+                r[n] = empty_rows((*x.shape[:-1], self.cin), self.dtype, self.device)
+                p.dx, p.dx_pitch = r[n].data_ptr(), _up8(self.cin)
             elif n == "w_gate":
-                r[n], p.dw_gate, p.dwg_pitch = self._out("dw_gate", None, (self.hidden,), self.cin, self.hidden)
+                r[n] = empty_rows((self.hidden, self.cin), self.dtype, self.device)
+                p.dw_gate, p.dwg_pitch = r[n].data_ptr(), _up8(self.cin)
             elif n == "w_up":
-                r[n], p.dw_up, p.dwu_pitch = self._out("dw_up", None, (self.hidden,), self.cin, self.hidden)
+                r[n] = empty_rows((self.hidden, self.cin), self.dtype, self.device)
+                p.dw_up, p.dwu_pitch = r[n].data_ptr(), _up8(self.cin)
             elif n == "w_down":
-                r[n], p.dw_down, p.dwd_pitch = self._out("dw_down", None, (self.cout,), self.hidden, self.cout)
+                r[n] = empty_rows((self.cout, self.hidden), self.dtype, self.device)
+                p.dw_down, p.dwd_pitch = r[n].data_ptr(), _up8(self.hidden)
             else:
                 r[n] = empty_rows((self.cout if n == "b_down" else self.hidden,), self.dtype, self.device)
                 setattr(p, "d" + n, r[n].data_ptr())
-        scratch = _scratch(lib().fhk_gated_ffn_grad_scratch_bytes(ctypes.byref(p)), self.device)
-        if scratch is not None:
-            p.scratch, p.scratch_bytes = scratch.data_ptr(), scratch.numel()
-        _launch("gated_ffn gradient", lib().fhk_gated_ffn_grad, p, self.device)
+        _gated_ffn_grad(p, self.device, self._grad_sizes, (m, p.h_pitch, *names))
         return r
 
 
@@ -322,7 +350,8 @@ class ResidualNorm:
 
     pre, post: "rms", "layer" or "none"; w_pre, b_pre, w_post, b_post, scale: vectors of `channels` or None (a norm
     without them is only normalised). x, f: (..., channels); gate: (gates, channels) of any alignment, each of its rows
-    for an equal run of rows (one per image of a batch, say), or None. f None: y is x (the norm before a first block). No autograd."""
+    for an equal run of rows (one per image of a batch, say), or None. f None: y is x (the norm before a first block). No
+    autograd."""
 
     def __init__(self, channels: int, dtype, pre: str = "rms", post: str = "none", w_pre=None, b_pre=None, w_post=None,
                  b_post=None, scale=None, eps: float = 1e-6):
@@ -338,23 +367,27 @@ class ResidualNorm:
             raise FlyHighError("a weight or bias was given for a norm that is none")
         self.channels, self.dtype, self.pre, self.post, self.eps = channels, dtype, pre, post, float(eps)
         self.params = {"w_pre": w_pre, "b_pre": b_pre, "w_post": w_post, "b_post": b_post, "scale": scale}
-        self._code = _dtype_code(dtype)
+        code = _dtype_code(dtype)
         given = [t for t in self.params.values() if t is not None]
-        self._ptrs = {}
+        ptrs = {}
         if given:
             if not given[0].is_cuda:
                 raise FlyHighError("the norms' vectors are CUDA tensors")
-            self._ptrs = {n: _vector(n, t, channels, dtype, given[0].device) for n, t in self.params.items() if t is not None}
+            ptrs = {n: _vector(n, t, channels, dtype, given[0].device) for n, t in self.params.items() if t is not None}
         self.device = given[0].device if given else None
+        common = dict(c=channels, pre=NORMS[pre], post=NORMS[post], eps=self.eps, dtype=code)
+        # the calls' parameter blocks with all that does not change from call to call
+        self._forward_params = ResidualNormParams(**common, **ptrs)
+        ptrs.pop("b_pre", None)
+        self._grad_params = ResidualNormGradParams(**common, **ptrs)
+        self._sizes = {}
 
     def _device(self, t):
         if not t.is_cuda or (self.device is not None and t.device != self.device):
             raise FlyHighError(f"a CUDA tensor on {self.device or 'a GPU'} is expected, got one on {t.device}")
         return t.device
 
-    def _gate(self, gate, m, device):
-        if gate is None:
-            return None, 0, 0
+    def _gate(self, p, gate, m, device):
         if gate.dim() != 2:
             raise FlyHighError(f"gate: (gates, {self.channels}) is expected, got {tuple(gate.shape)}")
         n, c = gate.shape
@@ -364,72 +397,63 @@ class ResidualNorm:
                                f"{tuple(gate.shape)} (strides {gate.stride()}) on {gate.device}")
         if n < 1 or m % n:
             raise FlyHighError(f"gate: {n} rows do not divide the {m} rows")
-        return gate.data_ptr(), gate.stride(0) if n > 1 else c, n
-
-    def _like(self, name, t, lead, m, device):
-        if t is None:
-            t = empty_rows((*lead, self.channels), self.dtype, device)
-        ptr, pitch, rows = _rows(name, t, self.channels, self.dtype, device)
-        if rows != m:
-            raise FlyHighError(f"{name}: {m} rows are expected, got {rows}")
-        return t, ptr, pitch
+        p.gate, p.gate_pitch, p.gates = gate.data_ptr(), gate.stride(0) if n > 1 else c, n
 
     def __call__(self, x, f=None, gate=None):
         """(y, h); h is None where pre is "none", and y is x itself where f is None."""
-        dev = self._device(x)
-        xp, x_pitch, m = _rows("x", x, self.channels, self.dtype, dev)
-        p = ResidualNormParams(x=xp, x_pitch=x_pitch, m=m, c=self.channels, pre=NORMS[self.pre], post=NORMS[self.post],
-                               eps=self.eps, dtype=self._code, **self._ptrs)
-        y, h, lead = x, None, x.shape[:-1]
+        dev, c, dt = self._device(x), self.channels, self.dtype
+        p = ResidualNormParams.from_buffer_copy(self._forward_params)
+        p.x, p.x_pitch, m = _rows("x", x, c, dt, dev)
+        p.m = m
+        y, h, shape = x, None, x.shape
         if f is not None:
-            _, p.f, p.f_pitch = self._like("f", f, lead, m, dev)
-            p.gate, p.gate_pitch, p.gates = self._gate(gate, m, dev)
-            y, p.y, p.y_pitch = self._like("y", None, lead, m, dev)
+            p.f, p.f_pitch = _like("f", f, m, c, dt, dev)
+            if gate is not None:
+                self._gate(p, gate, m, dev)
+            y = empty_rows(shape, dt, dev)
+            p.y, p.y_pitch = y.data_ptr(), _up8(c)
         else:
             if gate is not None or self.pre == "none":
                 raise FlyHighError("without f there is no gate, and a norm before the block")
             p.post, p.scale, p.w_post, p.b_post = 0, None, None, None
         if self.pre != "none":
-            h, p.h, p.h_pitch = self._like("h", None, lead, m, dev)
-        _launch("residual_norm", lib().fhk_residual_norm, p, dev)
+            h = empty_rows(shape, dt, dev)
+            p.h, p.h_pitch = h.data_ptr(), _up8(c)
+        _residual_norm(p, dev)
         return y, h
 
     def backward(self, dy, dh, y, f=None, gate=None) -> dict:
         """The gradients for dy and dh (either may be None: zero) of the call that returned y: "x", and with f "f",
         "gate" where there is one, and those of the vectors there are. They are new tensors, each written whole."""
-        first = next((t for t in (dy, dh) if t is not None), None)
+        first = dy if dy is not None else dh
         if first is None or (dh is not None and self.pre == "none"):
             raise FlyHighError("dy or dh is needed, and dh only with a norm before the next block")
-        dev = self._device(first)
-        lead = first.shape[:-1]
-        m = _rows("dy", first, self.channels, self.dtype, dev)[2]
-        names = {n for n, t in self.params.items() if t is not None and (f is not None or n in ("w_pre", "b_pre"))}
-        p = ResidualNormGradParams(m=m, c=self.channels, pre=NORMS[self.pre], post=NORMS[self.post], eps=self.eps,
-                                   dtype=self._code, **{n: v for n, v in self._ptrs.items() if n != "b_pre" and
-                                                        (f is not None or n == "w_pre")})
+        dev, c, dt = self._device(first), self.channels, self.dtype
+        p = ResidualNormGradParams.from_buffer_copy(self._grad_params)
+        ptr, pitch, m = _rows("dy" if dy is not None else "dh", first, c, dt, dev)
+        p.m = m
         if dy is not None:
-            _, p.dy, p.dy_pitch = self._like("dy", dy, lead, m, dev)
+            p.dy, p.dy_pitch = ptr, pitch
         if dh is not None:
-            _, p.dh, p.dh_pitch = self._like("dh", dh, lead, m, dev)
-            _, p.y, p.y_pitch = self._like("y", y, lead, m, dev)
-        r = {}
-        r["x"], p.dx, p.dx_pitch = self._like("dx", None, lead, m, dev)
+            p.dh, p.dh_pitch = (ptr, pitch) if dy is None else _like("dh", dh, m, c, dt, dev)
+            p.y, p.y_pitch = _like("y", y, m, c, dt, dev)
+        r = {"x": empty_rows(first.shape, dt, dev)}
+        p.dx, p.dx_pitch = r["x"].data_ptr(), _up8(c)
         if f is not None:
-            _, p.f, p.f_pitch = self._like("f", f, lead, m, dev)
-            r["f"], p.df, p.df_pitch = self._like("df", None, lead, m, dev)
-            p.gate, p.gate_pitch, p.gates = self._gate(gate, m, dev)
+            p.f, p.f_pitch = _like("f", f, m, c, dt, dev)
+            r["f"] = empty_rows(first.shape, dt, dev)
+            p.df, p.df_pitch = r["f"].data_ptr(), _up8(c)
             if gate is not None:
+                self._gate(p, gate, m, dev)
                 r["gate"] = gate.new_empty(gate.shape)
-                p.dgate, p.dgate_pitch = r["gate"].data_ptr(), self.channels
+                p.dgate, p.dgate_pitch = r["gate"].data_ptr(), c
         else:
             if gate is not None:
                 raise FlyHighError("without f there is no gate")
-            p.post = 0
-        for n in sorted(names):
-            r[n] = empty_rows((self.channels,), self.dtype, dev)
-            setattr(p, "d" + n, r[n].data_ptr())
-        scratch = _scratch(lib().fhk_residual_norm_grad_scratch_bytes(ctypes.byref(p)), dev)
-        if scratch is not None:
-            p.scratch, p.scratch_bytes = scratch.data_ptr(), scratch.numel()
-        _launch("residual_norm gradient", lib().fhk_residual_norm_grad, p, dev)
+            p.post, p.scale, p.w_post, p.b_post = 0, None, None, None
+        for n, t in self.params.items():
+            if t is not None and (f is not None or n == "w_pre" or n == "b_pre"):
+                r[n] = empty_rows((c,), dt, dev)
+                setattr(p, "d" + n, r[n].data_ptr())
+        _residual_norm_grad(p, dev, self._sizes, (m, p.gates))
         return r
