@@ -30,104 +30,140 @@ namespace {
 constexpr int kMaxC = 8192;
 constexpr int kForwardThreads = 1024, kGradThreads = 512;  // threads per SM that the registers are cut for
 
-// the sum over the LPR threads that share a row, in a fixed order, returned to all of them. LPR <= 32: within a warp;
-// above: over the CTA (LPR == its threads), red holding one float per warp and a buffer of its own for each call
-// between two reuses.
+// The sum over the LPR threads that share a row, in a fixed order, returned to all of them. LPR <= 32: within a warp;
+// above: over the CTA (LPR == its threads), red holding one float per warp (every thread adds them up, by 16-byte reads).
+template <int NW>
+__device__ __forceinline__ float add_up(const float* red) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; i += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(red + i);
+        v += (t.x + t.y) + (t.z + t.w);
+    }
+    return v;
+}
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
 #pragma unroll
     for (int o = (LPR < 32 ? LPR : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (LPR > 32) {
-        constexpr int NW = LPR / 32;
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        if (lane == 0) red[warp] = v;
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = lane < NW ? red[lane] : 0.0f;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        v = add_up<LPR / 32>(red);
     }
     return v;
 }
-// two sums at once
+// Two sums at once. The first exchange leaves each half of the lanes with one of them, so the rest of the tree is shared.
 template <int LPR>
 __device__ __forceinline__ float2 row_sum2(float a, float b, float* red) {
+    constexpr int H = (LPR < 32 ? LPR : 32) / 2;
+    const bool hi = threadIdx.x & H;
+    float v = (hi ? b : a) + __shfl_xor_sync(0xffffffffu, hi ? a : b, H);
 #pragma unroll
-    for (int o = (LPR < 32 ? LPR : 32) / 2; o; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
+    for (int o = H / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (LPR > 32) {
-        constexpr int NW = LPR / 32;
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        if (lane == 0) reinterpret_cast<float2*>(red)[warp] = make_float2(a, b);
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if ((lane & 15) == 0) red[(lane ? 32 : 0) + warp] = v;
         __syncthreads();
-        const float2 t = lane < NW ? reinterpret_cast<float2*>(red)[lane] : make_float2(0.0f, 0.0f);
-        a = t.x;
-        b = t.y;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b += __shfl_xor_sync(0xffffffffu, b, o);
-        }
+        return make_float2(add_up<LPR / 32>(red), add_up<LPR / 32>(red + 32));
     }
-    return make_float2(a, b);
+    const float w = __shfl_xor_sync(0xffffffffu, v, H);
+    return hi ? make_float2(w, v) : make_float2(v, w);
 }
 
-// v -> its normalised row n (in place; channels outside the row stay 0, all of them where the thread has no row);
-// returns 1 / the deviation.
-// red: 3 x 64 floats (a sum's buffer is reused only after another sum's barrier)
+// x -> its normalised row n (in place; channels outside the row stay 0, all of them where the thread has no row);
+// returns 1 / the deviation. red: 2 x 64 floats
 template <int LPR, int NCH>
-__device__ __forceinline__ float normalise(int kind, float (&v)[NCH][8], const int (&valid)[NCH], float inv_c, float eps,
-                                           float* red) {
-    float mean = 0.0f;
-    if (kind == FH_NORM_LAYER) {
-        float s = 0.0f;
+__device__ __forceinline__ void center(Chunk (&x)[NCH], const int (&valid)[NCH], float mean) {
 #pragma unroll
-        for (int k = 0; k < NCH; k++)
+    for (int k = 0; k < NCH; k++) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) s += v[k][j];
-        mean = row_sum<LPR>(s, red) * inv_c;
+        for (int j = 0; j < 4; j++) x[k].v[j] = __fadd2_rn(x[k].v[j], make_float2(-mean, -mean));
+        x[k].cut(valid[k]);
     }
-    float q = 0.0f;
+}
+template <int NCH>
+__device__ __forceinline__ float sum_of(const Chunk (&x)[NCH]) {
+    float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < NCH; k++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            v[k][j] = j < valid[k] ? v[k][j] - mean : 0.0f;
-            q += v[k][j] * v[k][j];
-        }
-    const float r = 1.0f / sqrtf(row_sum<LPR>(q, red + 64) * inv_c + eps);
+        for (int j = 0; j < 4; j++) s = __fadd2_rn(s, x[k].v[j]);
+    return s.x + s.y;
+}
+template <int NCH>
+__device__ __forceinline__ float squares_of(const Chunk (&x)[NCH]) {
+    float2 q = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < NCH; k++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[k][j] = j < valid[k] ? v[k][j] * r : 0.0f;
+        for (int j = 0; j < 4; j++) q = __ffma2_rn(x[k].v[j], x[k].v[j], q);
+    return q.x + q.y;
+}
+template <int NCH>
+__device__ __forceinline__ void scale_by(Chunk (&x)[NCH], const int (&valid)[NCH], float r) {
+#pragma unroll
+    for (int k = 0; k < NCH; k++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[k].v[j] = __fmul2_rn(x[k].v[j], make_float2(r, r));
+        x[k].cut(valid[k]);  // r may be infinite
+    }
+}
+template <int LPR, int NCH>
+__device__ __forceinline__ float normalise(int kind, Chunk (&x)[NCH], const int (&valid)[NCH], float inv_c, float eps,
+                                           float* red) {
+    if (kind == FH_NORM_LAYER) center<LPR, NCH>(x, valid, row_sum<LPR>(sum_of(x), red) * inv_c);
+    const float r = rsqrtf(row_sum<LPR>(squares_of(x), red + 64) * inv_c + eps);
+    scale_by(x, valid, r);
+    return r;
+}
+// two rows of the same thread at once, each sum of theirs together with the other's; a kind of none leaves its row as it is
+template <int LPR, int NCH>
+__device__ __forceinline__ float2 normalise2(int kx, Chunk (&x)[NCH], int ky, Chunk (&y)[NCH], const int (&valid)[NCH],
+                                             float inv_c, float eps, float* red) {
+    if (kx == FH_NORM_LAYER || ky == FH_NORM_LAYER) {
+        const float2 s = row_sum2<LPR>(sum_of(x), sum_of(y), red);
+        if (kx == FH_NORM_LAYER) center<LPR, NCH>(x, valid, s.x * inv_c);
+        if (ky == FH_NORM_LAYER) center<LPR, NCH>(y, valid, s.y * inv_c);
+    }
+    const float2 q = row_sum2<LPR>(squares_of(x), squares_of(y), red + 64);
+    const float2 r = make_float2(rsqrtf(q.x * inv_c + eps), rsqrtf(q.y * inv_c + eps));
+    if (kx != FH_NORM_NONE) scale_by(x, valid, r.x);
+    if (ky != FH_NORM_NONE) scale_by(y, valid, r.y);
     return r;
 }
 
+// by (plus) a vector's channels `at`; none: unchanged
 template <typename T>
-__device__ __forceinline__ void mul_vec(float (&v)[8], const void* w, long long at, int valid) {
+__device__ __forceinline__ void mul_vec(Chunk& x, const void* w, long long at, int valid, bool vec = true) {
     if (!w) return;
-    float t[8];
-    load8(static_cast<const T*>(w) + at, valid, t);
+    const Chunk t = load_chunk(static_cast<const T*>(w) + at, valid, vec);
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] *= t[j];
-}
-// by the gate's row, which may begin anywhere
-template <typename T, typename P>
-__device__ __forceinline__ void mul_gate(float (&v)[8], const P& p, long long at, int valid) {
-    if (!p.gate) return;
-    float t[8];
-    load8_any(static_cast<const T*>(p.gate) + at, valid, (p.gate_pitch & 7) == 0 && ((uintptr_t)p.gate & 15) == 0, t);
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] *= t[j];
+    for (int j = 0; j < 4; j++) x.v[j] = __fmul2_rn(x.v[j], t.v[j]);
 }
 template <typename T>
-__device__ __forceinline__ void add_vec(float (&v)[8], const void* w, long long at, int valid) {
+__device__ __forceinline__ void add_vec(Chunk& x, const void* w, long long at, int valid) {
     if (!w) return;
-    float t[8];
-    load8(static_cast<const T*>(w) + at, valid, t);
+    const Chunk t = load_chunk(static_cast<const T*>(w) + at, valid);
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] += t[j];
+    for (int j = 0; j < 4; j++) x.v[j] = __fadd2_rn(x.v[j], t.v[j]);
+}
+__device__ __forceinline__ void add(Chunk& x, const Chunk& y) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) x.v[j] = __fadd2_rn(x.v[j], y.v[j]);
+}
+__device__ __forceinline__ void mul(Chunk& x, const Chunk& y) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) x.v[j] = __fmul2_rn(x.v[j], y.v[j]);
+}
+__device__ __forceinline__ void add_product(Chunk& x, const Chunk& a, const Chunk& b) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) x.v[j] = __ffma2_rn(a.v[j], b.v[j], x.v[j]);
+}
+// whether every gate row begins on a 16-byte boundary
+template <typename P>
+__device__ __forceinline__ bool gate_vec(const P& p) {
+    return (p.gate_pitch & 7) == 0 && ((uintptr_t)p.gate & 15) == 0;
 }
 
 // A thread's own ring of rows in shared memory: asynchronous 16-byte copies of its chunks, STAGES - 1 rows ahead. A thread
@@ -140,23 +176,19 @@ struct Ring {
     __device__ __forceinline__ uint4* slot(int stage, int tensor, int k) const {
         return buf + ((stage * TENSORS + tensor) * NCH + k) * THREADS + threadIdx.x;
     }
-    __device__ __forceinline__ void copy(int stage, int tensor, int k, const T* base, long long at, int valid) const {
+    __device__ __forceinline__ void copy(int stage, int tensor, int k, const T* src, int valid) const {
         const uint32_t dst = (uint32_t)__cvta_generic_to_shared(slot(stage, tensor, k));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(valid > 0 ? base + at : base),
-                     "r"(valid > 0 ? 2 * valid : 0)
-                     : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(2 * valid) : "memory");
     }
     static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
     static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory"); }
-    __device__ __forceinline__ void read(int stage, int tensor, int k, float (&v)[8]) const {
-        unpack8<T>(*slot(stage, tensor, k), v);
-    }
+    __device__ __forceinline__ Chunk read(int stage, int tensor, int k) const { return unpack<T>(*slot(stage, tensor, k)); }
 };
 
 // THREADS / LPR rows at a time per CTA
 template <typename T, int THREADS, int LPR, int NCH, int STAGES>
-__global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual_norm(const FhResidualNormParams p, long long rows_per_gate) {
-    __shared__ float red[4 * 64];
+__global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual_norm(const FhResidualNormParams p, unsigned rows_per_gate) {
+    __shared__ __align__(16) float red[2 * 4 * 64];
     extern __shared__ uint4 ring_mem[];
     const Ring<T, THREADS, NCH, 2, STAGES> ring{ring_mem};
     constexpr int RPC = THREADS / LPR;
@@ -165,85 +197,98 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
     int valid[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; k++) valid[k] = max(0, min(8, p.c - 8 * (l + k * LPR)));
-    const T* x = static_cast<const T*>(p.x);
-    const T* f = static_cast<const T*>(p.f);
-    const long long first = (long long)blockIdx.x * RPC + sub, step = (long long)gridDim.x * RPC;
-    auto fetch = [&](long long row, int stage) {
+    const bool gvec = gate_vec(p), has_f = p.f != nullptr, has_h = p.h != nullptr;
+    const int first = blockIdx.x * RPC + sub, step = gridDim.x * RPC, m = (int)p.m;
+    // running pointers: the row that is copied, and the row that is written
+    const T* x = static_cast<const T*>(p.x) + first * p.x_pitch + 8 * l;
+    const T* f = static_cast<const T*>(p.f) + first * p.f_pitch + 8 * l;
+    T* y = static_cast<T*>(p.y) + first * p.y_pitch + 8 * l;
+    T* h = static_cast<T*>(p.h) + first * p.h_pitch + 8 * l;
+    long long ahead = first;
+    auto fetch = [&](int stage) {
+        const bool on = ahead < m;
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
-            const int vk = row < p.m ? valid[k] : 0, c = 8 * (l + k * LPR);
-            ring.copy(stage, 0, k, x, row * p.x_pitch + c, vk);
-            if (f) ring.copy(stage, 1, k, f, row * p.f_pitch + c, vk);
+            const int vk = on ? valid[k] : 0;
+            ring.copy(stage, 0, k, vk ? x + 8 * k * LPR : static_cast<const T*>(p.x), vk);
+            if (has_f) ring.copy(stage, 1, k, vk ? f + 8 * k * LPR : static_cast<const T*>(p.f), vk);
         }
         ring.commit();
+        ahead += step;
+        x += step * p.x_pitch;
+        f += step * p.f_pitch;
     };
 #pragma unroll
-    for (int q = 0; q < STAGES - 1; q++) fetch(first + q * step, q);
+    for (int q = 0; q < STAGES - 1; q++) fetch(q);
     int stage = 0;
-    // every thread of a CTA runs the same number of iterations: the sums are CTA-wide barriers or whole-warp shuffles
-    for (long long row = first; row - sub < p.m; row += step) {
-        const bool on = row < p.m;
-        float xv[NCH][8], fv[NCH][8];
+    // every thread of a CTA runs the same number of iterations: the sums are CTA-wide barriers or whole-warp shuffles.
+    // A row's sums use the buffers of its parity: between a buffer's uses lies a barrier of the row between them.
+    float* sums = red;
+    for (long long row = first; row - sub < m; row += step) {
+        Chunk xv[NCH], fv[NCH];
         int vr[NCH];  // the channels of this thread's row
         ring.wait();
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
-            vr[k] = on ? valid[k] : 0;
-            ring.read(stage, 0, k, xv[k]);
-            if (f) ring.read(stage, 1, k, fv[k]);
+            vr[k] = row < m ? valid[k] : 0;
+            xv[k] = ring.read(stage, 0, k);
+            if (has_f) fv[k] = ring.read(stage, 1, k);
         }
-        fetch(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+        fetch(stage == 0 ? STAGES - 1 : stage - 1);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-        if (f) {
-            if (p.post != FH_NORM_NONE) normalise<LPR, NCH>(p.post, fv, vr, inv_c, p.eps, red);
-            const long long grow = p.gate && on ? row / rows_per_gate * p.gate_pitch : 0;
+        if (has_f) {
+            if (p.post != FH_NORM_NONE) normalise<LPR, NCH>(p.post, fv, vr, inv_c, p.eps, sums);
+            const T* gate = static_cast<const T*>(p.gate);
+            if (gate) gate += (unsigned)min((int)row, m - 1) / rows_per_gate * p.gate_pitch;
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
                 const int c = 8 * (l + k * LPR);
-                if (valid[k]) {
-                    mul_vec<T>(fv[k], p.w_post, c, valid[k]);
-                    add_vec<T>(fv[k], p.b_post, c, valid[k]);
-                    mul_vec<T>(fv[k], p.scale, c, valid[k]);
-                    mul_gate<T>(fv[k], p, grow + c, valid[k]);
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) xv[k][j] += j < valid[k] ? fv[k][j] : 0.0f;
-                if (p.y && on && valid[k]) store8(static_cast<T*>(p.y) + row * p.y_pitch + c, valid[k], xv[k]);
+                if (!vr[k]) continue;
+                mul_vec<T>(fv[k], p.w_post, c, vr[k]);
+                add_vec<T>(fv[k], p.b_post, c, vr[k]);
+                mul_vec<T>(fv[k], p.scale, c, vr[k]);
+                mul_vec<T>(fv[k], gate, c, vr[k], gvec);
+                add(xv[k], fv[k]);
+                store_chunk(y + 8 * k * LPR, vr[k], xv[k]);
             }
+            y += step * p.y_pitch;
         }
-        if (p.h) {
-            normalise<LPR, NCH>(p.pre, xv, vr, inv_c, p.eps, red + 128);
+        if (has_h) {
+            normalise<LPR, NCH>(p.pre, xv, vr, inv_c, p.eps, sums + 128);
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
                 const int c = 8 * (l + k * LPR);
-                if (!valid[k]) continue;
-                mul_vec<T>(xv[k], p.w_pre, c, valid[k]);
-                add_vec<T>(xv[k], p.b_pre, c, valid[k]);
-                if (on) store8(static_cast<T*>(p.h) + row * p.h_pitch + c, valid[k], xv[k]);
+                if (!vr[k]) continue;
+                mul_vec<T>(xv[k], p.w_pre, c, vr[k]);
+                add_vec<T>(xv[k], p.b_pre, c, vr[k]);
+                store_chunk(h + 8 * k * LPR, vr[k], xv[k]);
             }
+            h += step * p.h_pitch;
         }
-        if (LPR > 32) __syncthreads();  // the sums' buffers are free again
+        sums = sums == red ? red + 256 : red;
     }
 }
 
 // dn -> the gradient of the row that n was normalised from
 template <int LPR, int NCH>
-__device__ __forceinline__ void normalise_grad(int kind, float (&dn)[NCH][8], const float (&n)[NCH][8], float r,
-                                               float inv_c, float* red) {
-    float s1 = 0.0f, s0 = 0.0f;
+__device__ __forceinline__ void normalise_grad(int kind, Chunk (&dn)[NCH], const Chunk (&n)[NCH], float r, float inv_c, float* red) {
+    float2 s1 = make_float2(0.0f, 0.0f), s0 = s1;
 #pragma unroll
     for (int k = 0; k < NCH; k++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            s1 += dn[k][j] * n[k][j];
-            s0 += dn[k][j];
+        for (int j = 0; j < 4; j++) {
+            s1 = __ffma2_rn(dn[k].v[j], n[k].v[j], s1);
+            s0 = __fadd2_rn(s0, dn[k].v[j]);
         }
-    const float2 s = row_sum2<LPR>(s1, s0, red);
-    const float m1 = s.x * inv_c, m0 = kind == FH_NORM_LAYER ? s.y * inv_c : 0.0f;
+    const float2 s = row_sum2<LPR>(s1.x + s1.y, s0.x + s0.y, red);
+    const float m1 = -s.x * inv_c, m0 = kind == FH_NORM_LAYER ? -s.y * inv_c : 0.0f;
 #pragma unroll
     for (int k = 0; k < NCH; k++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) dn[k][j] = r * (dn[k][j] - n[k][j] * m1 - m0);
+        for (int j = 0; j < 4; j++) {
+            const float2 t = __ffma2_rn(n[k].v[j], make_float2(m1, m1), __fadd2_rn(dn[k].v[j], make_float2(m0, m0)));
+            dn[k].v[j] = __fmul2_rn(t, make_float2(r, r));
+        }
 }
 
 // How a gradient's rows are shared out. Gate rows are `groups` runs of `len` rows. With few of them each run is cut
@@ -260,7 +305,8 @@ template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE>
 __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_norm_grad(const FhResidualNormGradParams p, const Split sp,
                                                                  float* part) {
     constexpr int RPC = THREADS / LPR;
-    __shared__ float red[6 * 64];
+    __shared__ __align__(16) float red[2 * 6 * 64];
+    float* sums = red;  // a row's sums use the buffers of its parity, as in the forward kernel
     __shared__ float fold[RPC > 1 ? THREADS * NCH * 8 : 1];
     extern __shared__ uint4 ring_mem[];
     const Ring<T, THREADS, NCH, 4, STAGES> ring{ring_mem};
@@ -270,28 +316,27 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
     for (int k = 0; k < NCH; k++) valid[k] = max(0, min(8, p.c - 8 * (l + k * LPR)));
     const T* f = static_cast<const T*>(p.f);
-    float a1[NCH][8], a0[NCH][8], b1[NCH][8], b0[NCH][8];
-    float g1[WHOLE ? NCH : 1][8], g0[WHOLE ? NCH : 1][8];
+    const bool gvec = gate_vec(p);
+    pdl_trigger();  // what follows sums this kernel's parts, once all of it has ended
+    Chunk a1[NCH], a0[NCH], b1[NCH], b0[NCH], g1[WHOLE ? NCH : 1], g0[WHOLE ? NCH : 1];
 #pragma unroll
-    for (int k = 0; k < NCH; k++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            a1[k][j] = a0[k][j] = b1[k][j] = b0[k][j] = 0.0f;
-            if (WHOLE) g1[k][j] = g0[k][j] = 0.0f;
-        }
+    for (int k = 0; k < NCH; k++) {
+        a1[k].zero(), a0[k].zero(), b1[k].zero(), b0[k].zero();
+        if (WHOLE) g1[k].zero(), g0[k].zero();
+    }
     // v summed over the CTA's row groups (in order), returned to all of them
-    auto over_rows = [&](float (&v)[8]) {
+    auto over_rows = [&](Chunk& x) {
         if (RPC == 1) return;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; j++) fold[(sub * 8 + j) * LPR + l] = v[j];
+        for (int j = 0; j < 8; j++) fold[(sub * 8 + j) * LPR + l] = x.get(j);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             float s = 0.0f;
 #pragma unroll 4
             for (int i = 0; i < RPC; i++) s += fold[(i * 8 + j) * LPR + l];
-            v[j] = s;
+            x.set(j, s);
         }
     };
 
@@ -305,95 +350,108 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
             lo = base + sp.len * sl / sp.slices;
             hi = base + sp.len * (sl + 1) / sp.slices;
         }
-        auto fetch = [&](long long row, int stage) {
+        const T* tp[4] = {static_cast<const T*>(p.dy), static_cast<const T*>(p.dh), static_cast<const T*>(p.y), f};
+        const long long pitch[4] = {p.dy_pitch, p.dh_pitch, p.y_pitch, p.f_pitch};
+        const bool has[4] = {p.dy != nullptr, p.dh != nullptr, p.dh != nullptr, f != nullptr};
+        const T* const tp0[4] = {tp[0], tp[1], tp[2], tp[3]};
 #pragma unroll
-            for (int k = 0; k < NCH; k++) {
-                const int vk = row < hi ? valid[k] : 0, c = 8 * (l + k * LPR);
-                if (p.dy) ring.copy(stage, 0, k, static_cast<const T*>(p.dy), row * p.dy_pitch + c, vk);
-                if (p.dh) {
-                    ring.copy(stage, 1, k, static_cast<const T*>(p.dh), row * p.dh_pitch + c, vk);
-                    ring.copy(stage, 2, k, static_cast<const T*>(p.y), row * p.y_pitch + c, vk);
+        for (int t = 0; t < 4; t++) tp[t] += (lo + sub) * pitch[t] + 8 * l;
+        T* dx = static_cast<T*>(p.dx) + (lo + sub) * p.dx_pitch + 8 * l;
+        T* df = static_cast<T*>(p.df) + (lo + sub) * p.df_pitch + 8 * l;
+        long long ahead = lo + sub;
+        auto fetch = [&](int stage) {
+            const bool on = ahead < hi;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                if (!has[t]) continue;
+#pragma unroll
+                for (int k = 0; k < NCH; k++) {
+                    const int vk = on ? valid[k] : 0;
+                    ring.copy(stage, t, k, vk ? tp[t] + 8 * k * LPR : tp0[t], vk);
                 }
-                if (f) ring.copy(stage, 3, k, f, row * p.f_pitch + c, vk);
+                tp[t] += RPC * pitch[t];
             }
             ring.commit();
+            ahead += RPC;
         };
         if (WHOLE) asm volatile("cp.async.wait_all;\n" ::: "memory");  // the last run's copies, before their slots are reused
 #pragma unroll
-        for (int q = 0; q < STAGES - 1; q++) fetch(lo + sub + q * RPC, q);
+        for (int q = 0; q < STAGES - 1; q++) fetch(q);
         int stage = 0;
+        // what a channel's values are multiplied by in every row of the run: scale * gate * w_post, and w_pre
+        Chunk post_w[NCH], pre_w[NCH];
+#pragma unroll
+        for (int k = 0; k < NCH; k++) {
+            const int c = 8 * (l + k * LPR);
+#pragma unroll
+            for (int j = 0; j < 4; j++) post_w[k].v[j] = pre_w[k].v[j] = make_float2(1.0f, 1.0f);
+            if (!valid[k]) continue;
+            mul_vec<T>(post_w[k], p.scale, c, valid[k]);
+            if (p.gate) mul_vec<T>(post_w[k], p.gate, (long long)grp * p.gate_pitch + c, valid[k], gvec);
+            mul_vec<T>(post_w[k], p.w_post, c, valid[k]);
+            mul_vec<T>(pre_w[k], p.w_pre, c, valid[k]);
+        }
         for (long long row = lo + sub; row - sub < hi; row += RPC) {
-            const bool on = row < hi;
-            float d[NCH][8], dh[NCH][8], yv[NCH][8], fv[NCH][8];
+            Chunk d[NCH], dh[NCH], yv[NCH], fv[NCH];
             int vr[NCH];  // the channels of this thread's row
             ring.wait();
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
-                vr[k] = on ? valid[k] : 0;
-                if (p.dy) {
-                    ring.read(stage, 0, k, d[k]);
+                vr[k] = row < hi ? valid[k] : 0;
+                if (has[0]) d[k] = ring.read(stage, 0, k);
+                else d[k].zero();
+                if (has[1]) {
+                    dh[k] = ring.read(stage, 1, k);
+                    yv[k] = ring.read(stage, 2, k);
                 } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) d[k][j] = 0.0f;
+                    yv[k].zero();
                 }
-                if (p.dh) {
-                    ring.read(stage, 1, k, dh[k]);
-                    ring.read(stage, 2, k, yv[k]);
-                }
-                if (f) ring.read(stage, 3, k, fv[k]);
+                if (has[3]) fv[k] = ring.read(stage, 3, k);
+                else fv[k].zero();
             }
-            fetch(row + (STAGES - 1) * RPC, stage == 0 ? STAGES - 1 : stage - 1);
+            fetch(stage == 0 ? STAGES - 1 : stage - 1);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
-            if (p.dh) {
-                const float r = normalise<LPR, NCH>(p.pre, yv, vr, inv_c, p.eps, red);
+            const int kind_y = has[1] ? p.pre : FH_NORM_NONE;
+            float2 r = make_float2(1.0f, 1.0f);
+            if (kind_y != FH_NORM_NONE || p.post != FH_NORM_NONE)
+                r = normalise2<LPR, NCH>(kind_y, yv, p.post, fv, vr, inv_c, p.eps, sums);
+            if (has[1]) {
 #pragma unroll
                 for (int k = 0; k < NCH; k++) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        b1[k][j] += dh[k][j] * yv[k][j];
-                        b0[k][j] += dh[k][j];
-                    }
-                    if (valid[k]) mul_vec<T>(dh[k], p.w_pre, 8 * (l + k * LPR), valid[k]);
+                    add_product(b1[k], dh[k], yv[k]);
+                    add(b0[k], dh[k]);
+                    mul(dh[k], pre_w[k]);
                 }
-                normalise_grad<LPR, NCH>(p.pre, dh, yv, r, inv_c, red + 128);
+                normalise_grad<LPR, NCH>(p.pre, dh, yv, r.x, inv_c, sums + 128);
 #pragma unroll
                 for (int k = 0; k < NCH; k++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) d[k][j] += j < vr[k] ? dh[k][j] : 0.0f;
+                    if (vr[k]) {
+                        add(d[k], dh[k]);
+                        d[k].cut(vr[k]);
+                    }
             }
             if (p.dx) {
 #pragma unroll
                 for (int k = 0; k < NCH; k++)
-                    if (on && valid[k])
-                        store8(static_cast<T*>(p.dx) + row * p.dx_pitch + 8 * (l + k * LPR), valid[k], d[k]);
+                    if (vr[k]) store_chunk(dx + 8 * k * LPR, vr[k], d[k]);
+                dx += RPC * p.dx_pitch;
             }
-            if (f) {
-                float r = 1.0f;
-                if (p.post != FH_NORM_NONE) r = normalise<LPR, NCH>(p.post, fv, vr, inv_c, p.eps, red + 256);
-                const long long grow = p.gate ? (long long)grp * p.gate_pitch : 0;
+            if (has[3]) {
 #pragma unroll
                 for (int k = 0; k < NCH; k++) {
-                    const int c = 8 * (l + k * LPR);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        a1[k][j] += d[k][j] * fv[k][j];
-                        a0[k][j] += d[k][j];
-                    }
-                    if (valid[k]) {
-                        mul_vec<T>(d[k], p.scale, c, valid[k]);
-                        mul_gate<T>(d[k], p, grow + c, valid[k]);
-                        mul_vec<T>(d[k], p.w_post, c, valid[k]);
-                    }
+                    add_product(a1[k], d[k], fv[k]);
+                    add(a0[k], d[k]);
+                    mul(d[k], post_w[k]);
                 }
                 if (p.df) {
-                    if (p.post != FH_NORM_NONE) normalise_grad<LPR, NCH>(p.post, d, fv, r, inv_c, red + 128);
+                    if (p.post != FH_NORM_NONE) normalise_grad<LPR, NCH>(p.post, d, fv, r.y, inv_c, sums + 256);
 #pragma unroll
                     for (int k = 0; k < NCH; k++)
-                        if (on && valid[k])
-                            store8(static_cast<T*>(p.df) + row * p.df_pitch + 8 * (l + k * LPR), valid[k], d[k]);
+                        if (vr[k]) store_chunk(df + 8 * k * LPR, vr[k], d[k]);
+                    df += RPC * p.df_pitch;
                 }
             }
-            if (LPR > 32) __syncthreads();
+            sums = sums == red ? red + 384 : red;
         }
         if (WHOLE) {  // the run's dgate row, and its share of the sums over gate rows
             const long long grow = p.gate ? (long long)grp * p.gate_pitch : 0;
@@ -404,34 +462,24 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
                 over_rows(a0[k]);
                 if (valid[k] && sub == 0) {
                     if (p.dgate) {
-                        float q[8], w0[8];
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            q[j] = a1[k][j];
-                            w0[j] = a0[k][j];
-                        }
+                        Chunk q = a1[k], w0 = a0[k];
                         mul_vec<T>(q, p.w_post, c, valid[k]);
                         if (p.b_post) {
                             mul_vec<T>(w0, p.b_post, c, valid[k]);
-#pragma unroll
-                            for (int j = 0; j < 8; j++) q[j] += w0[j];
+                            add(q, w0);
                         }
                         mul_vec<T>(q, p.scale, c, valid[k]);
-                        T* dst = static_cast<T*>(p.dgate) + (long long)grp * p.dgate_pitch + c;
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (j < valid[k]) dst[j] = Elem<T>::from(q[j]);
+                        store_chunk(static_cast<T*>(p.dgate) + (long long)grp * p.dgate_pitch + c, valid[k], q,
+                                    (p.dgate_pitch & 7) == 0 && ((uintptr_t)p.dgate & 15) == 0);
                     }
-                    mul_gate<T>(a1[k], p, grow + c, valid[k]);
-                    mul_gate<T>(a0[k], p, grow + c, valid[k]);
+                    mul_vec<T>(a1[k], p.gate, grow + c, valid[k], gvec);
+                    mul_vec<T>(a0[k], p.gate, grow + c, valid[k], gvec);
                 }
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    // every row group of the CTA holds the run's whole sum: the first keeps it
-                    g1[k][j] += sub == 0 ? a1[k][j] : 0.0f;
-                    g0[k][j] += sub == 0 ? a0[k][j] : 0.0f;
-                    a1[k][j] = a0[k][j] = 0.0f;
+                if (sub == 0) {  // every row group of the CTA holds the run's whole sum: the first keeps it
+                    add(g1[k], a1[k]);
+                    add(g0[k], a0[k]);
                 }
+                a1[k].zero(), a0[k].zero();
             }
         }
     }
@@ -439,14 +487,14 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 
     // the CTA's sums
     float* out = part + (long long)blockIdx.x * 4 * p.c;
-    auto put = [&](int q, float (&v)[NCH][8], bool summed) {
+    auto put = [&](int q, Chunk (&x)[NCH], bool summed) {
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
-            if (!summed) over_rows(v[k]);
+            if (!summed) over_rows(x[k]);
             const int c = 8 * (l + k * LPR);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (sub == 0 && j < valid[k]) out[(long long)q * p.c + c + j] = v[k][j];
+                if (sub == 0 && j < valid[k]) out[(long long)q * p.c + c + j] = x[k].get(j);
         }
     };
     if constexpr (WHOLE) {
@@ -460,14 +508,13 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
     put(3, b0, false);
 }
 
-// 32 columns per CTA and 32 warps over the CTAs' sums; blockIdx.y: 0 the post side, 1 the pre side. Up to 32 gate rows at a
-// time, each one's CTAs shared out over 32 / rows warps, whose sums are added in order.
+// 16 columns per CTA, 64 threads per column over the CTAs' sums; blockIdx.y: 0 the post side, 1 the pre side. Up to 64 gate
+// rows at a time, each one's CTAs shared out over 64 / rows threads, whose sums are added in order.
 template <typename T>
 __global__ void __launch_bounds__(1024) k_residual_norm_params(const FhResidualNormGradParams p, const Split sp,
                                                                const float* part) {
-    pdl_wait();
-    __shared__ float2 s[32][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    __shared__ float2 s[64][17];
+    const int lane = threadIdx.x & 15, w = threadIdx.x >> 4, col = blockIdx.x * 16 + lane;
     const bool on = col < p.c, post = blockIdx.y == 0;
     auto at = [&](const void* v, long long i, float none) { return v && on ? Elem<T>::to(static_cast<const T*>(v)[i]) : none; };
     auto put = [&](void* v, long long i, float x) {
@@ -476,12 +523,13 @@ __global__ void __launch_bounds__(1024) k_residual_norm_params(const FhResidualN
     // the pre side and whole runs are one sum over all CTAs
     const int groups = post && !sp.whole ? sp.groups : 1, slices = sp.ctas / groups;
     const float wp = at(p.w_post, col, 1.0f), bp = at(p.b_post, col, 0.0f), sc = at(p.scale, col, 1.0f);
+    pdl_wait();
     float g1 = 0.0f, g0 = 0.0f;
-    for (int k0 = 0; k0 < groups; k0 += 32) {
-        const int batch = min(32, groups - k0), parts = 32 / batch;
+    for (int k0 = 0; k0 < groups; k0 += 64) {
+        const int batch = min(64, groups - k0), parts = 64 / batch;
         float2 v = make_float2(0.0f, 0.0f);
-        if (on && warp < batch * parts) {
-            const int k = k0 + warp / parts, q = warp % parts;
+        if (on && w < batch * parts) {
+            const int k = k0 + w / parts, q = w % parts;
             const float* src = part + (post ? 0 : 2 * (long long)p.c) + col;
             const int lo = k * slices + slices * q / parts, hi = k * slices + slices * (q + 1) / parts;
 #pragma unroll 8
@@ -491,27 +539,32 @@ __global__ void __launch_bounds__(1024) k_residual_norm_params(const FhResidualN
             }
         }
         __syncthreads();
-        s[warp][lane] = v;
+        s[w][lane] = v;
         __syncthreads();
-        if (warp == 0)
+        // thread b of a column: gate row k0 + b
+        if (w < batch) {
+            float t1 = 0.0f, t0 = 0.0f;
+            for (int q = 0; q < parts; q++) {
+                t1 += s[w * parts + q][lane].x;
+                t0 += s[w * parts + q][lane].y;
+            }
+            v = make_float2(t1, t0);
+            if (post && !sp.whole && p.gate) {
+                put(p.dgate, (long long)(k0 + w) * p.dgate_pitch + col, sc * (wp * t1 + bp * t0));
+                const float g = at(p.gate, (long long)(k0 + w) * p.gate_pitch + col, 1.0f);
+                v = make_float2(t1 * g, t0 * g);
+            }
+        }
+        __syncthreads();
+        if (w < batch) s[w][lane] = v;
+        __syncthreads();
+        if (w == 0)
             for (int b = 0; b < batch; b++) {
-                float t1 = 0.0f, t0 = 0.0f;
-                for (int q = 0; q < parts; q++) {
-                    t1 += s[b * parts + q][lane].x;
-                    t0 += s[b * parts + q][lane].y;
-                }
-                if (post && !sp.whole) {
-                    const int k = k0 + b;
-                    const float g = at(p.gate, (long long)k * p.gate_pitch + col, 1.0f);
-                    if (p.gate) put(p.dgate, (long long)k * p.dgate_pitch + col, sc * (wp * t1 + bp * t0));
-                    t1 *= g;
-                    t0 *= g;
-                }
-                g1 += t1;
-                g0 += t0;
+                g1 += s[b][lane].x;
+                g0 += s[b][lane].y;
             }
     }
-    if (warp != 0) return;
+    if (w != 0) return;
     if (post) {
         put(p.dscale, col, wp * g1 + bp * g0);
         put(p.dw_post, col, sc * g1);
@@ -549,7 +602,7 @@ cudaError_t run_forward(const FhResidualNormParams& p, cudaStream_t st) {
     const long long want = (p.m + RPC - 1) / RPC;
     const int grid = (int)std::min<long long>(want, (long long)kSms * (kForwardThreads / THREADS));
     return fhk::launch(k_residual_norm<T, THREADS, LPR, NCH, STAGES>, dim3(grid), dim3(THREADS), smem, st, p,
-                       p.gate ? p.m / p.gates : p.m);
+                       (unsigned)(p.gate ? p.m / p.gates : p.m));
 }
 
 template <typename T>
@@ -612,7 +665,7 @@ cudaError_t grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_
     const bool post = p.f && (p.dgate || p.dscale || p.dw_post || p.db_post), pre = p.dw_pre || p.db_pre;
     if (!post && !pre) return cudaSuccess;
     fhk::PdlScope pdl(true);  // it waits for the kernel above
-    return fhk::launch(k_residual_norm_params<T>, dim3((p.c + 31) / 32, 2), dim3(1024), 0, st, p, sp,
+    return fhk::launch(k_residual_norm_params<T>, dim3((p.c + 15) / 16, 2), dim3(1024), 0, st, p, sp,
                        static_cast<const float*>(p.scratch));
 }
 

@@ -34,49 +34,61 @@ struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& q, float (&v)[8]) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// 8 elements of a row as 4 pairs: arithmetic on pairs is one instruction for two elements
+struct Chunk {
+    float2 v[4];
+    __device__ __forceinline__ float get(int i) const { return i & 1 ? v[i / 2].y : v[i / 2].x; }
+    __device__ __forceinline__ void set(int i, float x) { (i & 1 ? v[i / 2].y : v[i / 2].x) = x; }
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = Elem<T>::to2(w[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; i++) v[i] = make_float2(0.0f, 0.0f);
     }
-}
-
-// 8 elements of a row, `valid` of them inside it (8: one 16-byte access; fewer: element by element, so that nothing
-// past the row's channels is touched). The rest read as 0.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
-    if (valid >= 8) {
-        unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
-    } else {
+    // the elements from `valid` on become 0
+    __device__ __forceinline__ void cut(int valid) {
+        if (valid >= 8) return;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < valid ? Elem<T>::to(p[i]) : 0.0f;
+        for (int i = 0; i < 8; i++)
+            if (i >= valid) set(i, 0.0f);
     }
+};
+template <typename T>
+__device__ __forceinline__ Chunk unpack(const uint4& q) {
+    return {{Elem<T>::to2(q.x), Elem<T>::to2(q.y), Elem<T>::to2(q.z), Elem<T>::to2(q.w)}};
+}
+// 8 elements at p, `valid` of them inside the row; vec: p lies on a 16-byte boundary. A whole chunk on a boundary is one
+// 16-byte access; else element by element, so that nothing past the row's channels is touched. The rest read as 0.
+template <typename T>
+__device__ __forceinline__ Chunk load_chunk(const T* p, int valid, bool vec = true) {
+    if (valid >= 8 && vec) return unpack<T>(*reinterpret_cast<const uint4*>(p));
+    Chunk c;
+#pragma unroll
+    for (int i = 0; i < 8; i++) c.set(i, i < valid ? Elem<T>::to(p[i]) : 0.0f);
+    return c;
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {
-    if (valid >= 8) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::from2(v[0], v[1]), Elem<T>::from2(v[2], v[3]),
-                                                  Elem<T>::from2(v[4], v[5]), Elem<T>::from2(v[6], v[7]));
+__device__ __forceinline__ void store_chunk(T* p, int valid, const Chunk& c, bool vec = true) {
+    if (valid >= 8 && vec) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::from2(c.v[0].x, c.v[0].y), Elem<T>::from2(c.v[1].x, c.v[1].y),
+                                                  Elem<T>::from2(c.v[2].x, c.v[2].y), Elem<T>::from2(c.v[3].x, c.v[3].y));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (i < valid) p[i] = Elem<T>::from(v[i]);
+            if (i < valid) p[i] = Elem<T>::from(c.get(i));
     }
 }
-
-// the same for a row that may begin anywhere: `vec` where it is known to begin on a 16-byte boundary
+// the same as 8 floats
 template <typename T>
-__device__ __forceinline__ void load8_any(const T* p, int valid, bool vec, float (&v)[8]) {
-    if (vec) {
-        load8(p, valid, v);
-    } else {
+__device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
+    const Chunk c = load_chunk(p, valid);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < valid ? Elem<T>::to(p[i]) : 0.0f;
-    }
+    for (int i = 0; i < 8; i++) v[i] = c.get(i);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {
+    Chunk c;
+#pragma unroll
+    for (int i = 0; i < 8; i++) c.set(i, v[i]);
+    store_chunk(p, valid, c);
 }
 
 constexpr long long kMaxRows = (1ll << 31) - 256;

@@ -225,11 +225,12 @@ class _Call:
             if n:
                 scratch = torch.empty(n, dtype=torch.uint8, device=device)
                 p.scratch, p.scratch_bytes = scratch.data_ptr(), n
+        stream = torch._C._cuda_getCurrentRawStream(device.index)  # torch.cuda.current_stream(device) without its object
         if torch.cuda.current_device() == device.index:
-            rc = self.fn(ref, torch.cuda.current_stream().cuda_stream)
+            rc = self.fn(ref, stream)
         else:
             with torch.cuda.device(device):
-                rc = self.fn(ref, torch.cuda.current_stream().cuda_stream)
+                rc = self.fn(ref, stream)
         if rc != 0:
             raise FlyHighError(f"{self.what} failed: CUDA error {rc}")
 
