@@ -31,67 +31,116 @@ constexpr int kSms = 148;
 
 __device__ unsigned long long g_ffn_timeouts;
 
-// act(g)
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+// 1 / (1 + exp(-z)): far out the power is 0 or infinite and the quotient 1 or 0
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+    const float2 t = mul2(z, pair(-1.44269504f));  // -log2(e) z
+    const float2 d = add2(make_float2(ex2(t.x), ex2(t.y)), pair(1.0f));
+    return make_float2(rcp(d.x), rcp(d.y));
+}
+// act(g) of a pair. 0.5 (1 + tanh z) = sigmoid(2 z), so the tanh form of gelu is g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3))
 template <int ACT>
-__device__ __forceinline__ float act_of(float g) {
-    if (ACT == FH_ACT_RELU) return g > 0.0f ? g : 0.0f;
-    if (ACT == FH_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
-    // 0.5 (1 + tanh z) = sigmoid(2 z), so the tanh form is g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3))
-    const float z = ACT == FH_ACT_GELU_TANH ? g * (1.59576912f + 0.07135481f * g * g) : g;
-    const float s = __fdividef(1.0f, 1.0f + __expf(-z));
-    return ACT == FH_ACT_SIGMOID ? s : g * s;
+__device__ __forceinline__ float2 act_of(float2 g) {
+    if (ACT == FH_ACT_RELU) return make_float2(g.x > 0.0f ? g.x : 0.0f, g.y > 0.0f ? g.y : 0.0f);
+    if (ACT == FH_ACT_GELU) {
+        const float2 h = mul2(g, pair(0.5f));
+        return fma2(h, make_float2(erff(g.x * 0.70710678f), erff(g.y * 0.70710678f)), h);
+    }
+    float2 z = g;
+    if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(mul2(g, g), pair(0.07135481f), pair(1.59576912f)));
+    const float2 s = sigmoid2(z);
+    return ACT == FH_ACT_SIGMOID ? s : mul2(g, s);
 }
 // act(g) and its derivative
 template <int ACT>
-__device__ __forceinline__ void act_both(float g, float& v, float& dv) {
+__device__ __forceinline__ void act_both(float2 g, float2& v, float2& dv) {
     if (ACT == FH_ACT_RELU) {
-        v = g > 0.0f ? g : 0.0f;
-        dv = g > 0.0f ? 1.0f : 0.0f;
+        v = make_float2(g.x > 0.0f ? g.x : 0.0f, g.y > 0.0f ? g.y : 0.0f);
+        dv = make_float2(g.x > 0.0f ? 1.0f : 0.0f, g.y > 0.0f ? 1.0f : 0.0f);
     } else if (ACT == FH_ACT_GELU) {
-        const float cdf = 0.5f * (1.0f + erff(g * 0.70710678f));
-        v = g * cdf;
-        dv = cdf + g * 0.39894228f * __expf(-0.5f * g * g);
+        const float2 cdf = fma2(make_float2(erff(g.x * 0.70710678f), erff(g.y * 0.70710678f)), pair(0.5f), pair(0.5f));
+        const float2 q = mul2(mul2(g, g), pair(-0.72134752f));  // exp(-g^2 / 2) as a power of two
+        v = mul2(g, cdf);
+        dv = fma2(mul2(g, pair(0.39894228f)), make_float2(ex2(q.x), ex2(q.y)), cdf);
     } else {
-        const float g2 = g * g;
-        const float z = ACT == FH_ACT_GELU_TANH ? g * (1.59576912f + 0.07135481f * g2) : g;
-        const float s = __fdividef(1.0f, 1.0f + __expf(-z));
-        v = ACT == FH_ACT_SIGMOID ? s : g * s;
-        dv = ACT == FH_ACT_SIGMOID ? s * (1.0f - s)
-             : ACT == FH_ACT_SILU  ? s * (1.0f + g * (1.0f - s))
-                                   : s + v * (1.0f - s) * (1.59576912f + 0.21406443f * g2);
+        const float2 g2 = mul2(g, g);
+        float2 z = g;
+        if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(g2, pair(0.07135481f), pair(1.59576912f)));
+        const float2 s = sigmoid2(z), c = fma2(s, pair(-1.0f), pair(1.0f));  // 1 - s
+        if (ACT == FH_ACT_SIGMOID) {
+            v = s;
+            dv = mul2(s, c);
+        } else {
+            v = mul2(g, s);
+            // s + g s (1 - s) dz / dg
+            const float2 w = mul2(v, c);
+            dv = ACT == FH_ACT_SILU ? add2(s, w) : fma2(w, fma2(g2, pair(0.21406443f), pair(1.59576912f)), s);
+        }
     }
 }
 
 enum Tail { PLAIN, GLU, GLU_GRAD };
+constexpr int kGroupM = 8;  // tiles of rows that are walked together, so that their operands stay in L2
+
+// n / d for n < 2^31 by a multiplication: with 2^s >= d > 2^(s - 1) and mul = ceil(2^(31 + s) / d), which is below 2^32, the
+// product's error stays under n / 2^31 of a step, so its upper bits are the quotient (Granlund and Montgomery)
+struct Divider {
+    unsigned mul, shift, d;
+    Divider() = default;
+    __host__ explicit Divider(unsigned by) : d(by) {
+        unsigned s_ = 0;
+        while ((1ull << s_) < by) s_++;
+        shift = s_;
+        mul = (unsigned)(((1ull << (31 + s_)) + by - 1) / by);
+    }
+    __device__ __forceinline__ unsigned div(unsigned n) const { return (unsigned)(((unsigned long long)n * mul) >> (31 + shift)); }
+};
 
 // One product of a launch: out[m][n] = tail(sum over the terms of A[t] B[t]^T). GLU: A[0] with B[0] (gate) and B[1] (up).
 struct alignas(64) Job {
-    CUtensorMap a[2], b[2];
+    CUtensorMap a[2], b[2], o;     // o: out, in boxes of the tails
     int mn_a, mn_b;                // the operand is MN-major
     int kb[2];                     // 64-deep K blocks of the terms
     int m, n;                      // output extents
     int tiles_m, tiles_n, splits;  // tiles, and the parts of K that different CTAs sum
     int first;                     // its first work item
-    void *out, *out1, *out2;       // PLAIN: out; GLU: a, and g, u or NULL; GLU_GRAD: dg, du
+    Divider by_tiles, by_group;    // tiles_m * tiles_n, kGroupM * tiles_n
+    void* out;
     long long pitch;
     const void *bias0, *bias1;  // by column, or NULL
-    const void *g, *u;          // GLU_GRAD
     float* part;                // splits > 1: [split][m][n8] sums in place of out
 };
 constexpr int kJobs = 4;
 struct Work {
     Job job[kJobs];
-    int jobs, items, bn, stages, act;
+    CUtensorMap x[3];  // GLU: where g and u are kept (keep); GLU_GRAD: du out, g and u in
+    void* out[2];      // the same outputs
+    int jobs, items, bn, stages, act, keep;
     long long limit;
 };
 
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kStageA = 128 * 128;  // 128 rows of 64 elements
-constexpr int kRing = 196608;       // shared memory of the operand ring
+constexpr int kRing = 163840;   // shared memory of the operand ring
 constexpr int kMaxStages = 8;
-constexpr int kSmem = 1024 + kRing + 256;
-constexpr int kGroupM = 8;  // tiles of rows that are walked together, so that their operands stay in L2
+constexpr int kTile = 32 * 64;  // a tail's staging tile: 32 rows of 32 columns, 64-byte swizzled
+constexpr int kTiles = 4;       // per warp: two groups of 64 columns in turn
+constexpr int kBars = 512;
+constexpr int kSmem = 1024 + kRing + kEpiWarps * kTiles * kTile + kBars;
 
 struct Item {
     const Job* j;
@@ -102,80 +151,102 @@ __device__ __forceinline__ Item item_of(const Work& w, int i) {
     while (n + 1 < w.jobs && i >= w.job[n + 1].first) n++;
     const Job& j = w.job[n];
     i -= j.first;
-    const int tiles = j.tiles_m * j.tiles_n;
     Item t;
     t.j = &j;
-    t.split = i / tiles;
-    i -= t.split * tiles;
-    const int per = kGroupM * j.tiles_n, grp = i / per;
-    const int rows_ = min(kGroupM, j.tiles_m - grp * kGroupM);
-    i -= grp * per;
-    t.tm = grp * kGroupM + i % rows_;
-    t.tn = i / rows_;
+    t.split = j.by_tiles.div(i);
+    i -= t.split * (int)j.by_tiles.d;
+    const int grp = j.by_group.div(i), rows_ = min(kGroupM, j.tiles_m - grp * kGroupM);
+    i -= grp * (int)j.by_group.d;
+    t.tn = rows_ == kGroupM ? i / kGroupM : i / rows_;
+    t.tm = grp * kGroupM + i - t.tn * rows_;
     const int kb = j.kb[0] + j.kb[1];
-    t.k0 = (int)((long long)kb * t.split / j.splits);
-    t.k1 = (int)((long long)kb * (t.split + 1) / j.splits);
+    t.k0 = 0, t.k1 = kb;
+    if (j.splits > 1) {
+        t.k0 = (int)((long long)kb * t.split / j.splits);
+        t.k1 = (int)((long long)kb * (t.split + 1) / j.splits);
+    }
     return t;
 }
 
-// 16 values of a row into 16 columns, `valid` of them there; wide: the row's columns begin on 32-byte boundaries
+// 16 columns (half h of 32) of this lane's row of a staging tile: chunk c of a row lies at c ^ (row / 2 % 4)
+__device__ __forceinline__ uint32_t tile_at(uint32_t tile, int lane, int h, int c) {
+    return tile + lane * 64 + (((2 * h + c) ^ ((lane >> 1) & 3)) << 4);
+}
 template <typename T>
-__device__ __forceinline__ void store16(T* p, int valid, bool wide, const float (&v)[16]) {
-    if (valid >= 16) {
-        uint32_t q[8];
+__device__ __forceinline__ void tile_put(uint32_t tile, int lane, int h, const float2 (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = Elem<T>::from2(v[2 * i], v[2 * i + 1]);
-        if (wide) {
-            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]),
-                         "r"(q[4]), "r"(q[5]), "r"(q[6]), "r"(q[7])
-                         : "memory");
-        } else {
-            reinterpret_cast<uint4*>(p)[0] = make_uint4(q[0], q[1], q[2], q[3]);
-            reinterpret_cast<uint4*>(p)[1] = make_uint4(q[4], q[5], q[6], q[7]);
+    for (int c = 0; c < 2; c++)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(tile_at(tile, lane, h, c)), "r"(Elem<T>::from2(v[4 * c].x, v[4 * c].y)),
+                     "r"(Elem<T>::from2(v[4 * c + 1].x, v[4 * c + 1].y)), "r"(Elem<T>::from2(v[4 * c + 2].x, v[4 * c + 2].y)),
+                     "r"(Elem<T>::from2(v[4 * c + 3].x, v[4 * c + 3].y))
+                     : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void tile_get(uint32_t tile, int lane, int h, float2 (&v)[8]) {
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        uint32_t q[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                     : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                     : "r"(tile_at(tile, lane, h, c))
+                     : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[4 * c + i] = Elem<T>::to2(q[i]);
+    }
+}
+// this lane's row of a staging tile, `valid` columns of it, to p: in place of a tensor copy, which writes whole 16-byte
+// pieces, where the output's columns end inside one
+template <typename T>
+__device__ __noinline__ void tile_out(uint32_t tile, int lane, T* p, int valid) {
+    for (int c = 0; 8 * c < valid; c++) {
+        uint4 q;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                     : "r"(tile_at(tile, lane, 0, c))
+                     : "memory");
+        store_chunk(p + 8 * c, valid - 8 * c, unpack<T>(q));
+    }
+}
+// 32 columns of a bias (the same for all lanes) as they lie in memory, 0 past `cols` and where there is none
+template <typename T>
+__device__ __forceinline__ void load_bias(const void* bias, int c, int cols, uint32_t (&q)[16]) {
+    const T* p = static_cast<const T*>(bias) + c;
+    if (bias && c + 32 <= cols) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 t = reinterpret_cast<const uint4*>(p)[i];
+            q[4 * i] = t.x, q[4 * i + 1] = t.y, q[4 * i + 2] = t.z, q[4 * i + 3] = t.w;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 16; i++)
-            if (i < valid) p[i] = Elem<T>::from(v[i]);
+            q[i] = Elem<T>::from2(bias && c + 2 * i < cols ? Elem<T>::to(p[2 * i]) : 0.0f,
+                                  bias && c + 2 * i + 1 < cols ? Elem<T>::to(p[2 * i + 1]) : 0.0f);
     }
 }
-template <typename T>
-__device__ __forceinline__ void load16g(const T* p, int valid, float (&v)[16]) {
-    if (valid >= 16) {
-        float t[8];
-        load8(p, 8, t);
+// 16 accumulators as pairs, and a bias added to them
+__device__ __forceinline__ void pairs(const uint32_t* r, float2 (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = t[i];
-        load8(p + 8, 8, t);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[8 + i] = t[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = i < valid ? Elem<T>::to(p[i]) : 0.0f;
-    }
+    for (int i = 0; i < 8; i++) v[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
 }
 template <typename T>
-__device__ __forceinline__ void add_bias16(const void* bias, int c, int valid, float (&v)[16]) {
-    if (!bias) return;
-    float b[16];
-    load16g(static_cast<const T*>(bias) + c, valid, b);
+__device__ __forceinline__ void add_bias(const uint32_t* q, float2 (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] += b[i];
-}
-
-template <int ACT>
-__device__ __forceinline__ void glu16(const float (&g)[16], const float (&u)[16], float (&a)[16]) {
-#pragma unroll
-    for (int i = 0; i < 16; i++) a[i] = act_of<ACT>(g[i]) * u[i];
+    for (int i = 0; i < 8; i++) v[i] = add2(v[i], Elem<T>::to2(q[i]));
 }
 template <int ACT>
-__device__ __forceinline__ void glu_grad16(const float (&da)[16], float (&g)[16], float (&u)[16]) {
+__device__ __forceinline__ void glu16(const float2 (&g)[8], const float2 (&u)[8], float2 (&a)[8]) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        float v, dv;
+    for (int i = 0; i < 8; i++) a[i] = mul2(act_of<ACT>(g[i]), u[i]);
+}
+template <int ACT>
+__device__ __forceinline__ void glu_grad16(const float2 (&da)[8], float2 (&g)[8], float2 (&u)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float2 v, dv;
         act_both<ACT>(g[i], v, dv);
-        g[i] = da[i] * u[i] * dv;
-        u[i] = da[i] * v;
+        g[i] = mul2(mul2(da[i], u[i]), dv);
+        u[i] = mul2(da[i], v);
     }
 }
 
@@ -192,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
     const int bn = w.bn, nb = bn / CTAS, stages = w.stages;
     const uint32_t stage_bytes = kStageA + nb * 128;
-    const uint32_t bars = base + kRing;
+    const uint32_t bars = base + kRing + kEpiWarps * kTiles * kTile;
     const uint32_t full = bars, empty = bars + 8 * kMaxStages, tfull = bars + 16 * kMaxStages, tempty = tfull + 16,
                    slot = tempty + 16;
     const uint32_t cols = 2 * bn;
@@ -206,6 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
             bar_init(tfull + 8 * b, 1);
             bar_init(tempty + 8 * b, kEpiWarps * CTAS);
         }
+        for (int q = 0; q < 2 * kEpiWarps; q++) bar_init(bars + 256 + 8 * q, 1);
         bar_init_fence();
     }
     if (warp == 9) tmem_alloc<CTAS>(slot, cols);
@@ -297,67 +369,101 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
             }
         }
     } else {
+        // the tails: this warp's 32 rows and half of the tile's columns (all of a 32-wide tile for the first half), in groups
+        // of 64 (32 where a group has two or three outputs) that pass through staging tiles of 32 x 32, which tensor
+        // copies store, clipped at the output's edges
+        const bool keep = TAIL == GLU && w.keep;
+        const int group = TAIL == GLU_GRAD || keep ? 32 : 64;
         const int q = warp & 3, half = warp >> 2;
-        int n = 0;
+        const int width = TAIL == GLU ? bn / 2 : bn, span = max(32, width / 2);
+        const int lo = half * span, hi = min(width, lo + span);
+        const uint32_t tiles = base + kRing + warp * kTiles * kTile, gbar = bars + 256 + 16 * warp;
+        int n = 0, turn = 0;  // turn: the next tile (of four) of the ring that they form; GLU_GRAD, PLAIN: the next pair
+        uint32_t gph = 0;
         for (int i = first; i < w.items; i += step, n++) {
             const Item t = item_of(w, i);
-            const Job& j = *t.j;
-            const int b = n & 1;
-            const long long row = (long long)t.tm * 128 * CTAS + rank * 128 + q * 32 + lane;
-            const bool on = row < j.m;
+            const Job* j = t.j;
+            const int b = n & 1, m = j->m, cols_ = j->n, col = t.tn * width;
+            const int row = t.tm * 128 * CTAS + (int)rank * 128 + q * 32;
+            float* part = j->part;
+            const void *bias0 = part ? nullptr : j->bias0, *bias1 = j->bias1;
+            const bool ragged = cols_ & 7, biased = bias0 || bias1;
+            auto live = [&](int c0) { return row < m && c0 < hi && col + c0 < cols_; };
+            // GLU_GRAD: g and u of a group into the tiles of a pair, which dg and du then leave from
+            auto fetch = [&](int c0, int turn_) {
+                if (!live(c0) || lane != 0) return;
+                const uint32_t bar = gbar + 8 * (turn_ & 1), dst = tiles + 2 * (turn_ & 1) * kTile;
+                bar_expect(bar, 2 * kTile);
+                tensor_load<1>(dst, &w.x[1], col + c0, row, bar);
+                tensor_load<1>(dst + kTile, &w.x[2], col + c0, row, bar);
+            };
+            if (TAIL == GLU_GRAD) {
+                if (lane == 0) stores_read<1>();  // all but the last group's stores: the other two tiles
+                fetch(lo, turn);
+            }
             ok = bar_wait(tfull + 8 * b, (n >> 1) & 1, w.limit, &g_ffn_timeouts);
             if (!__all_sync(0xffffffffu, ok)) break;
             fence_after();
             const uint32_t acc = tbase + ((uint32_t)(q * 32) << 16) + b * bn;
-            if (TAIL == GLU) {
-                const bool wide = (j.pitch & 15) == 0 && (((uintptr_t)j.out | (uintptr_t)j.out1 | (uintptr_t)j.out2) & 31) == 0;
-                for (int c0 = half * (bn / 4); c0 < (half + 1) * (bn / 4); c0 += 16) {
-                    uint32_t rg[16], ru[16];
-                    load16(acc + c0, rg);
-                    load16(acc + bn / 2 + c0, ru);
-                    wait_ld();
-                    const int c = t.tn * (bn / 2) + c0, valid = min(16, j.n - c);
-                    if (on && valid > 0) {
-                        float g[16], u[16], a[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e++) g[e] = __uint_as_float(rg[e]), u[e] = __uint_as_float(ru[e]);
-                        add_bias16<T>(j.bias0, c, valid, g);
-                        add_bias16<T>(j.bias1, c, valid, u);
-                        switch (w.act) {
-                            case FH_ACT_SILU: glu16<FH_ACT_SILU>(g, u, a); break;
-                            case FH_ACT_GELU: glu16<FH_ACT_GELU>(g, u, a); break;
-                            case FH_ACT_GELU_TANH: glu16<FH_ACT_GELU_TANH>(g, u, a); break;
-                            case FH_ACT_RELU: glu16<FH_ACT_RELU>(g, u, a); break;
-                            default: glu16<FH_ACT_SIGMOID>(g, u, a); break;
-                        }
-                        const long long at = row * j.pitch + c;
-                        store16(static_cast<T*>(j.out) + at, valid, wide, a);
-                        if (j.out1) {
-                            store16(static_cast<T*>(j.out1) + at, valid, wide, g);
-                            store16(static_cast<T*>(j.out2) + at, valid, wide, u);
-                        }
+            for (int c0 = lo; c0 < hi; c0 += group) {
+                const bool alive = live(c0);
+                // this group's tiles: a pair, or with kept outputs three of the four, one after another
+                uint32_t dst = tiles + 2 * (turn & 1) * kTile, dst1 = dst, dst2 = dst;
+                if (keep) dst = tiles + (turn & 3) * kTile, dst1 = tiles + ((turn + 1) & 3) * kTile, dst2 = tiles + ((turn + 2) & 3) * kTile;
+                if (TAIL == GLU_GRAD) {
+                    if (alive) {
+                        ok = bar_wait(gbar + 8 * (turn & 1), (gph >> (turn & 1)) & 1, w.limit, &g_ffn_timeouts);
+                        gph ^= 1u << (turn & 1);
                     }
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                } else {
+                    // what these tiles held has been read: all but the last group's stores (of kept outputs: the last store)
+                    if (lane == 0) stores_read<1>();
                     __syncwarp();
                 }
-            } else {
-                const bool wide = (j.pitch & 15) == 0 && (((uintptr_t)j.out | (uintptr_t)j.out1) & 31) == 0;
-                for (int c0 = half * (bn / 2); c0 < (half + 1) * (bn / 2); c0 += 16) {
-                    const int c = t.tn * bn + c0, valid = min(16, j.n - c);
-                    const long long at = row * j.pitch + c;
-                    float g[16], u[16];
-                    if (TAIL == GLU_GRAD && on && valid > 0) {
-                        load16g(static_cast<const T*>(j.g) + at, valid, g);
-                        load16g(static_cast<const T*>(j.u) + at, valid, u);
+                const int subs = min(group, hi - c0) / 32;
+                for (int sub = 0; sub < subs; sub++) {
+                    const int cs = c0 + 32 * sub;
+                    uint32_t r0[32], r1[TAIL == GLU ? 32 : 1], q0[16], q1[16];
+                    load32(acc + cs, r0);
+                    if constexpr (TAIL == GLU) load32(acc + bn / 2 + cs, r1);
+                    if (TAIL != GLU_GRAD && biased) {
+                        load_bias<T>(bias0, col + cs, cols_, q0);
+                        if (TAIL == GLU) load_bias<T>(bias1, col + cs, cols_, q1);
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    uint32_t r[16];
-                    load16(acc + c0, r);
                     wait_ld();
-                    if (on && valid > 0) {
-                        float v[16];
+                    if (cs + 32 >= hi) {  // the accumulators have been read
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive_cluster(map_rank(tempty + 8 * b, 0));
+                    }
 #pragma unroll
-                        for (int e = 0; e < 16; e++) v[e] = __uint_as_float(r[e]);
-                        if (TAIL == GLU_GRAD) {
+                    for (int h = 0; h < 2; h++) {
+                        float2 v[8], g[8], u[8];
+                        if constexpr (TAIL == GLU) {
+                            pairs(r0 + 16 * h, g);
+                            pairs(r1 + 16 * h, u);
+                            if (biased) {
+                                add_bias<T>(q0 + 8 * h, g);
+                                add_bias<T>(q1 + 8 * h, u);
+                            }
+                            switch (w.act) {
+                                case FH_ACT_SILU: glu16<FH_ACT_SILU>(g, u, v); break;
+                                case FH_ACT_GELU: glu16<FH_ACT_GELU>(g, u, v); break;
+                                case FH_ACT_GELU_TANH: glu16<FH_ACT_GELU_TANH>(g, u, v); break;
+                                case FH_ACT_RELU: glu16<FH_ACT_RELU>(g, u, v); break;
+                                default: glu16<FH_ACT_SIGMOID>(g, u, v); break;
+                            }
+                            tile_put<T>(dst + sub * kTile, lane, h, v);
+                            if (keep) {
+                                tile_put<T>(dst1, lane, h, g);
+                                tile_put<T>(dst2, lane, h, u);
+                            }
+                        } else if constexpr (TAIL == GLU_GRAD) {
+                            pairs(r0 + 16 * h, v);
+                            tile_get<T>(dst, lane, h, g);
+                            tile_get<T>(dst + kTile, lane, h, u);
                             switch (w.act) {
                                 case FH_ACT_SILU: glu_grad16<FH_ACT_SILU>(v, g, u); break;
                                 case FH_ACT_GELU: glu_grad16<FH_ACT_GELU>(v, g, u); break;
@@ -365,26 +471,76 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                                 case FH_ACT_RELU: glu_grad16<FH_ACT_RELU>(v, g, u); break;
                                 default: glu_grad16<FH_ACT_SIGMOID>(v, g, u); break;
                             }
-                            store16(static_cast<T*>(j.out) + at, valid, wide, g);
-                            store16(static_cast<T*>(j.out1) + at, valid, wide, u);
-                        } else if (j.part) {
-                            const long long n8 = (j.n + 7) & ~7;
-                            float4* p = reinterpret_cast<float4*>(j.part + ((long long)t.split * j.m + row) * n8 + c);
-#pragma unroll
-                            for (int e = 0; e < 4; e++)  // columns up to n8 are the scratch's own
-                                if (4 * e < valid) p[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                            tile_put<T>(dst, lane, h, g);
+                            tile_put<T>(dst + kTile, lane, h, u);
+                            if (h == 0) {  // the next group's, into the tiles that the last group's stores have left by now
+                                if (lane == 0) stores_read<0>();
+                                fetch(c0 + 32, turn + 1);
+                                __syncwarp();
+                            }
                         } else {
-                            add_bias16<T>(j.bias0, c, valid, v);
-                            store16(static_cast<T*>(j.out) + at, valid, wide, v);
+                            pairs(r0 + 16 * h, v);
+                            if (part) {
+                                const int c = col + cs + 16 * h, valid = cols_ - c;
+                                if (row + lane < m) {
+                                    const long long n8 = (cols_ + 7) & ~7;
+                                    float4* o = reinterpret_cast<float4*>(part + ((long long)t.split * m + row + lane) * n8 + c);
+#pragma unroll
+                                    for (int e = 0; e < 4; e++)  // columns up to n8 are the scratch's own
+                                        if (4 * e < valid) o[e] = make_float4(v[2 * e].x, v[2 * e].y, v[2 * e + 1].x, v[2 * e + 1].y);
+                                }
+                                __syncwarp();
+                            } else {
+                                if (biased) add_bias<T>(q0 + 8 * h, v);
+                                tile_put<T>(dst + sub * kTile, lane, h, v);
+                            }
                         }
                     }
-                    __syncwarp();
                 }
+                if (!alive || (TAIL == PLAIN && part)) continue;
+                fence_async();
+                __syncwarp();
+                if (ragged && col + c0 + group > cols_) {  // the columns end inside a 16-byte piece
+                    for (int sub = 0; sub < subs && col + c0 + 32 * sub < cols_; sub++) {
+                        const long long at = (long long)(row + lane) * j->pitch + col + c0 + 32 * sub;
+                        const int valid = min(32, cols_ - col - c0 - 32 * sub);
+                        if (row + lane >= m) continue;
+                        tile_out<T>(dst + sub * kTile, lane, static_cast<T*>(j->out) + at, valid);
+                        if (keep) {
+                            tile_out<T>(dst1, lane, static_cast<T*>(w.out[0]) + at, valid);
+                            tile_out<T>(dst2, lane, static_cast<T*>(w.out[1]) + at, valid);
+                        }
+                        if (TAIL == GLU_GRAD) tile_out<T>(dst + kTile, lane, static_cast<T*>(w.out[0]) + at, valid);
+                    }
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) {  // groups of no stores: the count of those before stays right
+                        stores_commit();
+                        if (keep) stores_commit(), stores_commit();
+                    }
+                } else if (lane == 0) {
+                    for (int sub = 0; sub < subs && col + c0 + 32 * sub < cols_; sub++)
+                        tensor_store(&j->o, col + c0 + 32 * sub, row, dst + sub * kTile);
+                    if (keep) {
+                        stores_commit();
+                        tensor_store(&w.x[0], col + c0, row, dst1);
+                        stores_commit();
+                        tensor_store(&w.x[1], col + c0, row, dst2);
+                    }
+                    if (TAIL == GLU_GRAD) tensor_store(&w.x[0], col + c0, row, dst + kTile);
+                    stores_commit();
+                }
+                turn += keep ? 3 : 1;
             }
-            fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive_cluster(CTAS == 2 ? map_rank(tempty + 8 * b, 0) : map_rank(tempty + 8 * b, rank));
+            if (!__all_sync(0xffffffffu, ok)) break;
+            // a half without columns of a narrow tile
+            if (lo >= hi) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive_cluster(map_rank(tempty + 8 * b, 0));
+            }
         }
+        if (lane == 0) stores_done();
     }
     // a role that gave up leaves copies and matrix instructions in flight: give them time before the memory is let go
     if (!ok) {
@@ -525,15 +681,15 @@ struct Matrix {  // [rows][cols] of 16-bit elements
     int cols;
 };
 
-// boxes of 64 columns x `box` rows
+// boxes of 64 columns x `box` rows, 128-byte swizzled (operands), or of 32 x 32, 64-byte swizzled (box 0: the tails)
 cudaError_t map_of(CUtensorMap* map, const Matrix& x, int box, int dtype) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return cudaErrorNotSupported;
     const cuuint64_t dims[2] = {(cuuint64_t)x.cols, (cuuint64_t)x.rows}, strides[1] = {(cuuint64_t)x.pitch * 2};
-    const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, one[2] = {1, 1};
+    const cuuint32_t boxes[2] = {box ? 64u : 32u, box ? (cuuint32_t)box : 32u}, one[2] = {1, 1};
     const CUresult r = fn(map, dtype == FH_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                           const_cast<void*>(x.p), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          box ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
@@ -644,7 +800,7 @@ template <typename T, int TAIL>
 cudaError_t products(const Product* p, int n, int act, int dtype, long long limit, float* part, cudaStream_t st) {
     const Shape s = shape_of<TAIL>(p, n);
     Work w;
-    w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.limit = limit > 0 ? limit : 2000000000ll;
+    w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.limit = limit > 0 ? limit : 2000000000ll;
     const int nb = s.bn / s.ctas;
     w.stages = std::min(kMaxStages, kRing / (kStageA + nb * 128));
     Joins joins{};
@@ -662,10 +818,24 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
         j.tiles_n = (q.n + cols - 1) / cols;
         j.splits = s.splits[i];
         j.first = w.items;
+        if ((long long)j.tiles_m * j.tiles_n > (1ll << 30) || (long long)j.tiles_n * kGroupM > (1ll << 30)) return cudaErrorInvalidValue;
+        j.by_tiles = Divider((unsigned)(j.tiles_m * j.tiles_n)), j.by_group = Divider((unsigned)(kGroupM * j.tiles_n));
         const long long items = w.items + (long long)j.tiles_m * j.tiles_n * j.splits;
         if (items > (1ll << 30)) return cudaErrorInvalidValue;
         w.items = (int)items;
-        j.out = q.out, j.out1 = q.out1, j.out2 = q.out2, j.pitch = q.pitch, j.bias0 = q.bias0, j.bias1 = q.bias1, j.g = q.g, j.u = q.u;
+        j.out = q.out, j.pitch = q.pitch, j.bias0 = q.bias0, j.bias1 = q.bias1;
+        w.out[0] = q.out1, w.out[1] = q.out2;
+        auto tail_map = [&](CUtensorMap* map, const void* x) { return map_of(map, {x, q.pitch, q.m, q.n}, 0, dtype); };
+        if (TAIL == GLU && q.out1) {
+            w.keep = 1;
+            FH_TRY(tail_map(&w.x[0], q.out1));
+            FH_TRY(tail_map(&w.x[1], q.out2));
+        }
+        if (TAIL == GLU_GRAD) {
+            FH_TRY(tail_map(&w.x[0], q.out1));
+            FH_TRY(tail_map(&w.x[1], q.g));
+            FH_TRY(tail_map(&w.x[2], q.u));
+        }
         j.part = nullptr;
         if (j.splits > 1) {
             j.part = part;
@@ -673,6 +843,8 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
             o = {part, q.out, q.bias0, q.pitch, q.m, q.n, j.splits, joins.total};
             joins.total += q.m * ((q.n + 7) / 8);
             part += part_floats(q, j.splits);
+        } else {
+            FH_TRY(tail_map(&j.o, q.out));
         }
     }
     FH_TRY((s.ctas == 2 ? launch_work<T, 2, TAIL>(w, st) : launch_work<T, 1, TAIL>(w, st)));

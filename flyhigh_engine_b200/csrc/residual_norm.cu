@@ -378,10 +378,12 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
         for (int q = 0; q < STAGES - 1; q++) fetch(q);
         int stage = 0;
-        // what a channel's values are multiplied by in every row of the run: scale * gate * w_post, and w_pre
-        Chunk post_w[NCH], pre_w[NCH];
+        // what a channel's values are multiplied by in every row of the run: scale * gate * w_post, and w_pre. Kept in
+        // registers where a thread has one chunk of a row; with two they are formed again for each row.
+        constexpr bool HOIST = NCH == 1;
+        Chunk post_w[HOIST ? NCH : 1], pre_w[HOIST ? NCH : 1];
 #pragma unroll
-        for (int k = 0; k < NCH; k++) {
+        for (int k = 0; k < (HOIST ? NCH : 0); k++) {
             const int c = 8 * (l + k * LPR);
 #pragma unroll
             for (int j = 0; j < 4; j++) post_w[k].v[j] = pre_w[k].v[j] = make_float2(1.0f, 1.0f);
@@ -420,7 +422,8 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
                 for (int k = 0; k < NCH; k++) {
                     add_product(b1[k], dh[k], yv[k]);
                     add(b0[k], dh[k]);
-                    mul(dh[k], pre_w[k]);
+                    if constexpr (HOIST) mul(dh[k], pre_w[k]);
+                    else if (vr[k]) mul_vec<T>(dh[k], p.w_pre, 8 * (l + k * LPR), vr[k]);
                 }
                 normalise_grad<LPR, NCH>(p.pre, dh, yv, r.x, inv_c, sums + 128);
 #pragma unroll
@@ -441,7 +444,14 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
                 for (int k = 0; k < NCH; k++) {
                     add_product(a1[k], d[k], fv[k]);
                     add(a0[k], d[k]);
-                    mul(d[k], post_w[k]);
+                    if constexpr (HOIST) {
+                        mul(d[k], post_w[k]);
+                    } else if (vr[k]) {
+                        const int c = 8 * (l + k * LPR);
+                        mul_vec<T>(d[k], p.scale, c, vr[k]);
+                        if (p.gate) mul_vec<T>(d[k], p.gate, (long long)grp * p.gate_pitch + c, vr[k], gvec);
+                        mul_vec<T>(d[k], p.w_post, c, vr[k]);
+                    }
                 }
                 if (p.df) {
                     if (p.post != FH_NORM_NONE) normalise_grad<LPR, NCH>(p.post, d, fv, r.y, inv_c, sums + 256);
