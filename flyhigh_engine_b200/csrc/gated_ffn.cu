@@ -556,61 +556,255 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     if (warp == 9) tmem_free<CTAS>(tbase, cols);
 }
 
-// The split sums of a launch's jobs added in order, with the bias: 8 columns per thread
-struct Join {
-    const float* part;
+// ---- few rows ----
+//
+// With up to 32 rows the weights are what has to be read, once, at HBM's rate; a 128-row tile would leave its matrix pipe idle
+// and the grid short of CTAs. Here the weights' rows are the 16 rows of mma.m16n8k16 and x's rows its 8 columns (NT of them
+// side by side), so a CTA of 8 warps produces 16 output channels for all rows. Its warps take 32-wide steps of K in turn and
+// are added in shared memory; where the channels alone would not fill the GPU a cluster's CTAs share K and add over
+// distributed shared memory. Operands go from global memory to fragments: a thread's four k positions of two MMAs are
+// 8 consecutive elements of its row (the same order of k for both operands), one 16-byte load each.
+template <typename T>
+struct RowsArgs {
+    const T *x, *w0, *w1;  // [m][k], [n][k]
+    long long x_pitch, w0_pitch, w1_pitch;
+    const T *bias0, *bias1;
+    T *out, *g, *u;
+    long long pitch;
+    int m, n, k, act, share;  // share: CTAs of a cluster
+};
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                 uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                        uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 elements of a row from k on, 0 past its end (the last steps of K)
+template <typename T>
+__device__ __noinline__ uint4 load_k(const T* row, int k, int end) {
+    if (k >= end) return make_uint4(0, 0, 0, 0);
+    const Chunk c = load_chunk(row + k, end - k);
+    return make_uint4(Elem<T>::from2(c.v[0].x, c.v[0].y), Elem<T>::from2(c.v[1].x, c.v[1].y), Elem<T>::from2(c.v[2].x, c.v[2].y),
+                      Elem<T>::from2(c.v[3].x, c.v[3].y));
+}
+// 16 bytes of a weight: read once, so not kept in L1
+template <typename T>
+__device__ __forceinline__ uint4 load_once(const T* p) {
+    uint4 q;
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
+    return q;
+}
+__device__ __forceinline__ float act_by(int act, float g) {
+    const float2 v = pair(g);
+    switch (act) {
+        case FH_ACT_SILU: return act_of<FH_ACT_SILU>(v).x;
+        case FH_ACT_GELU: return act_of<FH_ACT_GELU>(v).x;
+        case FH_ACT_GELU_TANH: return act_of<FH_ACT_GELU_TANH>(v).x;
+        case FH_ACT_RELU: return act_of<FH_ACT_RELU>(v).x;
+        default: return act_of<FH_ACT_SIGMOID>(v).x;
+    }
+}
+
+template <typename T, int NT, bool GATED>
+__global__ void __launch_bounds__(256, 2) k_rows(const RowsArgs<T> p) {
+    constexpr int NW = GATED ? 2 : 1, COLS = 8 * NT, UNROLL = NT == 1 ? 4 : 2;
+    __shared__ float part[4][NW][COLS][17];  // [warp % 4][matrix][row of x][channel]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int tile = blockIdx.x / p.share, rank = blockIdx.x - tile * p.share;
+    const int steps = (p.k + 31) / 32, lo = steps * rank / p.share, hi = steps * (rank + 1) / p.share, inside = min(hi, p.k / 32);
+    // a row that is not there reads the last one: its results go nowhere
+    const T* w[NW][2];
+    const T* x[NT];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const long long c = min(tile * 16 + g + 8 * e, p.n - 1);
+        w[0][e] = p.w0 + c * p.w0_pitch;
+        if (GATED) w[NW - 1][e] = p.w1 + c * p.w1_pitch;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++) x[i] = p.x + (long long)min(8 * i + g, p.m - 1) * p.x_pitch;
+    float acc[NW][NT][4] = {};
+    uint4 a[UNROLL][NW][2], b[UNROLL][NT];
+    // step s: one of this CTA's, wholly inside K; the last one may not be, and behind hi there is nothing
+    auto load_weights = [&](int s0) {
+        const int k0 = s0 * 32 + 8 * t;
+#pragma unroll
+        for (int q = 0; q < UNROLL; q++) {
+            const int s = s0 + 8 * q;
+#pragma unroll
+            for (int i = 0; i < NW; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    if (s < inside) a[q][i][e] = load_once(w[i][e] + k0 + 256 * q);
+                    else a[q][i][e] = s < hi ? load_k(w[i][e], k0 + 256 * q, p.k) : make_uint4(0, 0, 0, 0);
+                }
+        }
+    };
+    auto load_x = [&](int s0) {
+        const int k0 = s0 * 32 + 8 * t;
+#pragma unroll
+        for (int q = 0; q < UNROLL; q++) {
+            const int s = s0 + 8 * q;
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                if (s < inside) b[q][i] = *reinterpret_cast<const uint4*>(x[i] + k0 + 256 * q);
+                else b[q][i] = s < hi ? load_k(x[i], k0 + 256 * q, p.k) : make_uint4(0, 0, 0, 0);
+            }
+        }
+    };
+    // the weights are no output of the kernel before: they are on their way while it ends
+    load_weights(lo + warp);
+    pdl_wait();
+    pdl_trigger();
+    for (int s0 = lo + warp; s0 < hi; s0 += 8 * UNROLL) {
+        load_x(s0);
+#pragma unroll
+        for (int q = 0; q < UNROLL; q++)
+#pragma unroll
+            for (int i = 0; i < NW; i++)
+#pragma unroll
+                for (int c = 0; c < NT; c++) {
+                    mma16816<T>(acc[i][c], a[q][i][0].x, a[q][i][1].x, a[q][i][0].y, a[q][i][1].y, b[q][c].x, b[q][c].y);
+                    mma16816<T>(acc[i][c], a[q][i][0].z, a[q][i][1].z, a[q][i][0].w, a[q][i][1].w, b[q][c].z, b[q][c].w);
+                }
+        if (s0 + 8 * UNROLL < hi) load_weights(s0 + 8 * UNROLL);
+    }
+    for (int round = 1; round >= 0; round--) {  // the upper four warps' sums, then the lower four's added to them
+        if (warp / 4 == round)
+#pragma unroll
+            for (int i = 0; i < NW; i++)
+#pragma unroll
+                for (int c = 0; c < NT; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float& v = part[warp & 3][i][8 * c + 2 * t + (e & 1)][g + 8 * (e >> 1)];
+                        v = round ? acc[i][c][e] : v + acc[i][c][e];
+                    }
+        __syncthreads();
+    }
+    // the warps' sums in order; in a cluster into the first warp's place, where the other CTAs read them
+    auto added = [&](int mat, int r, int c) {
+        float v = part[0][mat][r][c];
+#pragma unroll
+        for (int q = 1; q < 4; q++) v += part[q][mat][r][c];
+        return v;
+    };
+    if (p.share > 1) {
+        for (int i = threadIdx.x; i < NW * COLS * 16; i += 256) {
+            const int c = i & 15, r = (i >> 4) % COLS, mat = (i >> 4) / COLS;
+            part[0][mat][r][c] = added(mat, r, c);
+        }
+        umma::cluster_sync();
+    }
+    // each CTA of the cluster finishes a share of the rows
+    const int live = min(p.m, COLS), r_lo = live * rank / p.share, r_hi = live * (rank + 1) / p.share;
+    for (int i = r_lo * 16 + threadIdx.x; i < r_hi * 16; i += 256) {
+        const int c = i & 15, r = i >> 4, col = tile * 16 + c;
+        if (col >= p.n) continue;
+        float v[NW];
+#pragma unroll
+        for (int mat = 0; mat < NW; mat++) {
+            if (p.share == 1) {
+                v[mat] = added(mat, r, c);
+                continue;
+            }
+            const uint32_t at = umma::smem_addr(&part[0][mat][r][c]);
+            v[mat] = 0.0f;
+            for (int q = 0; q < p.share; q++) {
+                float f;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(f) : "r"(umma::map_rank(at, q)) : "memory");
+                v[mat] += f;
+            }
+        }
+        if (p.bias0) v[0] += Elem<T>::to(p.bias0[col]);
+        const long long at = r * p.pitch + col;
+        if (GATED) {
+            if (p.bias1) v[NW - 1] += Elem<T>::to(p.bias1[col]);
+            p.out[at] = Elem<T>::from(act_by(p.act, v[0]) * v[NW - 1]);
+            if (p.g) {
+                p.g[at] = Elem<T>::from(v[0]);
+                p.u[at] = Elem<T>::from(v[NW - 1]);
+            }
+        } else {
+            p.out[at] = Elem<T>::from(v[0]);
+        }
+    }
+    if (p.share > 1) umma::cluster_sync();  // the other CTAs may still read this one's sums
+}
+
+// Sums over slices: out[r][c] = bias[c] + sum over s of part[s][r][c], for the split products of a launch and for the
+// gradients of the biases (one row). 4 columns per thread and 8 threads over the slices, added in order.
+struct Sum {
+    const float* part;  // [slices][m][n8]
     void* out;
     const void* bias;
     long long pitch, m;
-    int n, splits;
-    long long first;  // its first group of 8 columns
+    int n, slices;
+    long long first;  // its first group of 4 columns
 };
-struct Joins {
-    Join j[kJobs];
+constexpr int kSums = kJobs + 3;
+struct Sums {
+    Sum s[kSums];
     int n;
     long long total;
 };
 template <typename T>
-__global__ void __launch_bounds__(256) k_join(const Joins w) {
-    pdl_wait();
-    long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= w.total) return;
+__global__ void __launch_bounds__(256) k_sums(const Sums w) {
+    __shared__ float4 fold[8][32];
+    const int lane = threadIdx.x & 31, way = threadIdx.x >> 5;
+    const long long at = (long long)blockIdx.x * 32 + lane;
     int k = 0;
-    while (k + 1 < w.n && i >= w.j[k + 1].first) k++;
-    const Join& j = w.j[k];
-    i -= j.first;
-    const int n8 = (j.n + 7) / 8;
-    const long long row = i / n8;
-    const int c = (int)(i - row * n8) * 8, valid = min(8, j.n - c);
-    float v[8] = {};
-    const float* p = j.part + (row * n8 * 8 + c);
-    for (int s = 0; s < j.splits; s++, p += j.m * n8 * 8) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w, v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+    while (k + 1 < w.n && at >= w.s[k + 1].first) k++;
+    const Sum& j = w.s[k];
+    const int quads = ((j.n + 7) & ~7) / 4;
+    const long long unit = at - j.first, row = unit / quads, slice = j.m * quads;
+    const int c = (int)(unit - row * quads) * 4;
+    pdl_wait();
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (at < w.total) {
+        const float4* p = reinterpret_cast<const float4*>(j.part) + unit;
+#pragma unroll 4
+        for (int s = way; s < j.slices; s += 8) {
+            const float4 t = p[s * slice];
+            v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
+        }
     }
-    if (j.bias) {
-        float b[8];
-        load8(static_cast<const T*>(j.bias) + c, valid, b);
+    fold[way][lane] = v;
+    __syncthreads();
+    if (way != 0 || at >= w.total) return;
+    for (int s = 1; s < 8; s++) {
+        const float4 t = fold[s][lane];
+        v.x += t.x, v.y += t.y, v.z += t.z, v.w += t.w;
+    }
+    T* o = static_cast<T*>(j.out) + row * j.pitch + c;
+    const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += b[e];
-    }
-    store8(static_cast<T*>(j.out) + row * j.pitch + c, valid, v);
+    for (int e = 0; e < 4; e++)
+        if (c + e < j.n) o[e] = Elem<T>::from(r[e] + (j.bias ? Elem<T>::to(static_cast<const T*>(j.bias)[c + e]) : 0.0f));
 }
 
-// Column sums of up to three matrices: a CTA sums a slice of the rows of 64 columns (8 threads of 8 columns by 32 rows),
-// a second kernel the slices in order
+// Column sums of up to three matrices: a CTA sums a slice of the rows of 64 columns (8 threads of 8 columns by 32 rows);
+// k_sums adds the slices
 struct Columns {
     const void* x;
-    void* out;
     long long pitch;
     int n;
-    long long part;  // its first float of the partial sums
+    float* part;  // [slices][n8]
 };
 struct ColumnSums {
     Columns c[3];
     long long m;
     int slices;
-    float* part;
 };
 template <typename T>
 __global__ void __launch_bounds__(256) k_column_parts(const ColumnSums w) {
@@ -622,33 +816,24 @@ __global__ void __launch_bounds__(256) k_column_parts(const ColumnSums w) {
     if (blockIdx.x * 64 >= q.n) return;
     const int valid = max(0, min(8, q.n - c));
     const long long lo = w.m * blockIdx.y / w.slices, hi = w.m * (blockIdx.y + 1) / w.slices;
-    float v[8] = {};
+    Chunk v;
+    v.zero();
     if (valid)
 #pragma unroll 4
         for (long long i = lo + r; i < hi; i += 32) {
-            float t[8];
-            load8(static_cast<const T*>(q.x) + i * q.pitch + c, valid, t);
+            const Chunk t = load_chunk(static_cast<const T*>(q.x) + i * q.pitch + c, valid);
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] += t[e];
+            for (int e = 0; e < 4; e++) v.v[e] = add2(v.v[e], t.v[e]);
         }
 #pragma unroll
-    for (int e = 0; e < 8; e++) s[r][8 * (threadIdx.x & 7) + e] = v[e];
+    for (int e = 0; e < 8; e++) s[r][8 * (threadIdx.x & 7) + e] = v.get(e);
     __syncthreads();
-    if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < q.n) {
+    const int n8 = (q.n + 7) & ~7, col = blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && col < n8) {
         float t = 0.0f;
         for (int i = 0; i < 32; i++) t += s[i][threadIdx.x];
-        w.part[q.part + (long long)blockIdx.y * q.n + blockIdx.x * 64 + threadIdx.x] = t;
+        q.part[(long long)blockIdx.y * n8 + col] = t;
     }
-}
-template <typename T>
-__global__ void __launch_bounds__(128) k_column_join(const ColumnSums w) {
-    pdl_wait();
-    const Columns& q = w.c[blockIdx.y];
-    const int c = blockIdx.x * 128 + threadIdx.x;
-    if (c >= q.n) return;
-    float t = 0.0f;
-    for (int i = 0; i < w.slices; i++) t += w.part[q.part + (long long)i * q.n + c];
-    static_cast<T*>(q.out)[c] = Elem<T>::from(t);
 }
 
 #define FH_TRY(call)                              \
@@ -795,15 +980,14 @@ cudaError_t launch_work(const Work& w, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, k_product<T, CTAS, TAIL>, w);
 }
 
-// the products of one launch (and the launch that joins their split sums); part: scratch_floats
+// the products of one launch; part: scratch_floats, whose sums are added to `sums`
 template <typename T, int TAIL>
-cudaError_t products(const Product* p, int n, int act, int dtype, long long limit, float* part, cudaStream_t st) {
+cudaError_t products(const Product* p, int n, int act, int dtype, long long limit, float* part, Sums* sums, cudaStream_t st) {
     const Shape s = shape_of<TAIL>(p, n);
     Work w;
     w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.limit = limit > 0 ? limit : 2000000000ll;
     const int nb = s.bn / s.ctas;
     w.stages = std::min(kMaxStages, kRing / (kStageA + nb * 128));
-    Joins joins{};
     for (int i = 0; i < n; i++) {
         Job& j = w.job[i];
         const Product& q = p[i];
@@ -839,17 +1023,68 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
         j.part = nullptr;
         if (j.splits > 1) {
             j.part = part;
-            Join& o = joins.j[joins.n++];
-            o = {part, q.out, q.bias0, q.pitch, q.m, q.n, j.splits, joins.total};
-            joins.total += q.m * ((q.n + 7) / 8);
+            sums->s[sums->n++] = {part, q.out, q.bias0, q.pitch, q.m, q.n, j.splits, sums->total};
+            sums->total += q.m * (((q.n + 7) & ~7) / 4);
             part += part_floats(q, j.splits);
         } else {
             FH_TRY(tail_map(&j.o, q.out));
         }
     }
-    FH_TRY((s.ctas == 2 ? launch_work<T, 2, TAIL>(w, st) : launch_work<T, 1, TAIL>(w, st)));
-    if (joins.n) FH_TRY(fhk::launch(k_join<T>, dim3((unsigned)((joins.total + 255) / 256)), dim3(256), 0, st, joins));
-    return cudaSuccess;
+    return s.ctas == 2 ? launch_work<T, 2, TAIL>(w, st) : launch_work<T, 1, TAIL>(w, st);
+}
+template <typename T>
+cudaError_t finish(const Sums& sums, cudaStream_t st) {
+    if (!sums.n) return cudaSuccess;
+    return fhk::launch(k_sums<T>, dim3((unsigned)((sums.total + 31) / 32)), dim3(256), 0, st, sums);
+}
+
+// Whether a forward call takes the form for few rows: by estimates in us of both. It reads the weights at about 5.5 TB/s,
+// slowed as every CTA reads 8 NT rows of x beside its 16 weight rows, with about 4 us of launches and latencies; the tiles
+// need about 12 us and 5.2 TB/s whatever the rows. Measured (bf16, us, this form / tiles): 1 row of 1024 -> 4096 7.2 / 19,
+// 32 rows 13.7 / 19; 2048 -> 8192 24 / 33 with 1 row, 32 / 33 with 16, 41 / 33 with 32; 4096 -> 16384 75 / 89 with 1, 111 / 89
+// with 16.
+bool takes_few_rows(long long m, int cin, int hidden, int cout) {
+    if (m > 32) return false;
+    const double mb = 2e-6 * hidden * (2.0 * cin + cout);
+    const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
+    return 4 + mb / 5.5 * (0.8 + 0.325 * nt) < 12 + mb / 5.2;
+}
+template <typename T, int NT, bool GATED>
+cudaError_t launch_rows(const RowsArgs<T>& p, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((p.n + 15) / 16 * p.share));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    unsigned na = 0;
+    if (p.share > 1) {
+        at[na].id = cudaLaunchAttributeClusterDimension;
+        at[na].val.clusterDim = {(unsigned)p.share, 1, 1};
+        na++;
+    }
+    if (fhk::pdl_flag()) {
+        at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = na;
+    return cudaLaunchKernelEx(&cfg, k_rows<T, NT, GATED>, p);
+}
+template <typename T, bool GATED>
+cudaError_t few_rows(const Product& q, int act, cudaStream_t st) {
+    RowsArgs<T> p{};
+    p.x = static_cast<const T*>(q.a[0].p), p.x_pitch = q.a[0].pitch;
+    p.w0 = static_cast<const T*>(q.b[0].p), p.w0_pitch = q.b[0].pitch;
+    if (GATED) p.w1 = static_cast<const T*>(q.b[1].p), p.w1_pitch = q.b[1].pitch;
+    p.bias0 = static_cast<const T*>(q.bias0), p.bias1 = static_cast<const T*>(q.bias1);
+    p.out = static_cast<T*>(q.out), p.g = static_cast<T*>(q.out1), p.u = static_cast<T*>(q.out2), p.pitch = q.pitch;
+    p.m = (int)q.m, p.n = q.n, p.k = (int)q.k, p.act = act, p.share = 1;
+    // a cluster per 16 channels until there is a CTA for every SM, while each warp keeps two steps of K
+    while (p.share < 8 && (p.n + 15) / 16 * p.share < kSms && (p.k + 31) / 32 >= 32 * p.share) p.share *= 2;
+    if (p.m <= 8) return launch_rows<T, 1, GATED>(p, st);
+    if (p.m <= 16) return launch_rows<T, 2, GATED>(p, st);
+    return launch_rows<T, 4, GATED>(p, st);
 }
 
 template <typename P>
@@ -886,9 +1121,16 @@ Product down_of(const FhGatedFfnParams& p) {
 template <typename T>
 cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {
     const Product glu = glu_of(p), down = down_of(p);
-    FH_TRY((products<T, GLU>(&glu, 1, p.act, p.dtype, p.wait_cycles, nullptr, st)));
+    Sums sums{};
+    if (takes_few_rows(p.m, p.cin, p.hidden, p.cout)) {
+        FH_TRY((few_rows<T, true>(glu, p.act, st)));
+        fhk::PdlScope pdl(true);
+        return few_rows<T, false>(down, p.act, st);
+    }
+    FH_TRY((products<T, GLU>(&glu, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
     fhk::PdlScope pdl(true);  // what follows waits on a kernel of this file
-    return products<T, PLAIN>(&down, 1, p.act, p.dtype, p.wait_cycles, static_cast<float*>(p.scratch), st);
+    FH_TRY((products<T, PLAIN>(&down, 1, p.act, p.dtype, p.wait_cycles, static_cast<float*>(p.scratch), &sums, st)));
+    return finish<T>(sums, st);
 }
 
 // the gradient's scratch: dg and du [m][h_pitch], then the split sums and the partial column sums
@@ -897,6 +1139,7 @@ struct GradPlan {
     int outs;
     size_t hidden_bytes, part_bytes, column_bytes;
     ColumnSums cols;
+    void* db[3];
     int ncols, widest;
 };
 GradPlan grad_plan(const FhGatedFfnGradParams& p) {
@@ -931,8 +1174,8 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
     g.part_bytes = (g.outs ? scratch_floats<PLAIN>(g.out, g.outs) * 4 + 255 : 0) / 256 * 256;
     auto column = [&](const void* x_, long long pitch, int n, void* out) {
         if (!out) return;
-        g.cols.c[g.ncols++] = {x_, out, pitch, n, (long long)g.column_bytes};
-        g.column_bytes += n;
+        g.db[g.ncols] = out;
+        g.cols.c[g.ncols++] = {x_, pitch, n, nullptr};
         g.widest = std::max(g.widest, n);
     };
     column(dg, p.h_pitch, p.hidden, p.db_gate);
@@ -941,11 +1184,13 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
     if (g.ncols) {
         // about four CTAs per SM over the columns, 64 rows to a slice at least
         const long long across = (long long)((g.widest + 63) / 64) * g.ncols;
-        g.cols.slices = (int)std::max<long long>(1, std::min<long long>(std::min<long long>((p.m + 63) / 64, 4 * kSms / across), 1024));
-        for (int i = 0; i < g.ncols; i++) g.cols.c[i].part *= g.cols.slices;
-        g.column_bytes *= (size_t)g.cols.slices * 4;
+        g.cols.slices = (int)std::max<long long>(1, std::min<long long>((p.m + 63) / 64, 4 * kSms / across));
         g.cols.m = p.m;
-        g.cols.part = reinterpret_cast<float*>(dg + 2 * g.hidden_bytes + g.part_bytes);
+        float* at = reinterpret_cast<float*>(dg + 2 * g.hidden_bytes + g.part_bytes);
+        for (int i = 0; i < g.ncols; i++) {
+            g.cols.c[i].part = at + g.column_bytes / 4;
+            g.column_bytes += (size_t)g.cols.slices * ((g.cols.c[i].n + 7) & ~7) * 4;
+        }
     }
     return g;
 }
@@ -954,23 +1199,33 @@ template <typename T>
 cudaError_t gradient(const FhGatedFfnGradParams& p, cudaStream_t st) {
     const GradPlan g = grad_plan(p);
     const bool hidden = p.dx || p.dw_gate || p.dw_up || p.db_gate || p.db_up;  // whether dg or du is read
-    if (hidden) FH_TRY((products<T, GLU_GRAD>(&g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, st)));
-    fhk::PdlScope pdl(hidden);
-    if (g.outs)
+    Sums sums{};
+    if (hidden) FH_TRY((products<T, GLU_GRAD>(&g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    bool mine = hidden;  // whether the stream's last kernel is one of this file's, which the next may wait for itself
+    if (g.outs) {
+        fhk::PdlScope pdl(mine);
         FH_TRY((products<T, PLAIN>(g.out, g.outs, p.act, p.dtype, p.wait_cycles,
-                                   reinterpret_cast<float*>(static_cast<char*>(p.scratch) + 2 * g.hidden_bytes), st)));
-    if (g.ncols) {
-        FH_TRY(fhk::launch(k_column_parts<T>, dim3((g.widest + 63) / 64, g.cols.slices, g.ncols), dim3(256), 0, st, g.cols));
-        fhk::PdlScope own(true);
-        FH_TRY(fhk::launch(k_column_join<T>, dim3((g.widest + 127) / 128, g.ncols), dim3(128), 0, st, g.cols));
+                                   reinterpret_cast<float*>(static_cast<char*>(p.scratch) + 2 * g.hidden_bytes), &sums, st)));
+        mine = true;
     }
-    return cudaSuccess;
+    if (g.ncols) {
+        fhk::PdlScope pdl(mine);
+        FH_TRY(fhk::launch(k_column_parts<T>, dim3((g.widest + 63) / 64, g.cols.slices, g.ncols), dim3(256), 0, st, g.cols));
+        for (int i = 0; i < g.ncols; i++) {
+            const Columns& c = g.cols.c[i];
+            sums.s[sums.n++] = {c.part, g.db[i], nullptr, c.n, 1, c.n, g.cols.slices, sums.total};
+            sums.total += ((c.n + 7) & ~7) / 4;
+        }
+        mine = true;
+    }
+    fhk::PdlScope pdl(mine);
+    return finish<T>(sums, st);
 }
 
 }  // namespace
 
 extern "C" size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p) {
-    if (!p || !good_sizes(p) || p->m == 0) return 0;
+    if (!p || !good_sizes(p) || p->m == 0 || takes_few_rows(p->m, p->cin, p->hidden, p->cout)) return 0;
     const Product down = down_of(*p);
     return scratch_floats<PLAIN>(&down, 1) * 4;
 }

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import Structure, c_float, c_int, c_longlong, c_size_t, c_void_p
-from typing import NamedTuple, Optional
+from typing import Optional
 
 import numpy as np
 
@@ -148,6 +148,20 @@ def empty_rows(shape, dtype, device="cuda"):
     return t if c % 8 == 0 else t[..., :c]
 
 
+def _rows_like(t):
+    """empty_rows of t's shape, type and device; t is a tensor of rows."""
+    import torch
+    c = t.shape[-1]
+    return torch.empty_like(t) if c % 8 == 0 else empty_rows(t.shape, t.dtype, t.device)
+
+
+def _vectors(sizes, dtype, device):
+    """New vectors, each beginning on a 16-byte boundary (of one allocation)."""
+    import torch
+    up = [_up8(n) for n in sizes]
+    return [t if n == k else t[:n] for t, n, k in zip(torch.empty(sum(up), dtype=dtype, device=device).split(up), sizes, up)]
+
+
 def _dtype_code(dtype) -> int:
     import torch
     if dtype == torch.float16:
@@ -241,11 +255,23 @@ _residual_norm = _Call("residual_norm", "fhk_residual_norm", None)
 _residual_norm_grad = _Call("residual_norm gradient", "fhk_residual_norm_grad", "fhk_residual_norm_grad_scratch_bytes")
 
 
-class GatedFFNSaved(NamedTuple):
-    """What a training forward call keeps for the gradient: gate and up projections and their activated product."""
-    g: object
-    u: object
-    a: object
+class GatedFFNSaved:
+    """What a training forward call keeps for the gradient: the activated product a and the projections g and u."""
+
+    def __init__(self, hidden, channels: int):
+        self.rows, self.channels = hidden, channels  # (3, rows, pitch): a, g, u
+
+    @property
+    def a(self):
+        return self.rows[0, :, :self.channels]
+
+    @property
+    def g(self):
+        return self.rows[1, :, :self.channels]
+
+    @property
+    def u(self):
+        return self.rows[2, :, :self.channels]
 
 
 class GatedFFN:
@@ -287,7 +313,7 @@ class GatedFFN:
         p = GatedFfnParams.from_buffer_copy(self._forward_params)
         p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
         if out is None:
-            out = empty_rows((*x.shape[:-1], self.cout), self.dtype, self.device)
+            out = _rows_like(x) if self.cout == self.cin else empty_rows((*x.shape[:-1], self.cout), self.dtype, self.device)
             p.y, p.y_pitch = out.data_ptr(), _up8(self.cout)
         else:
             p.y, p.y_pitch = _like("out", out, m, self.cout, self.dtype, self.device)
@@ -306,8 +332,7 @@ class GatedFFN:
     def forward(self, x, out=None):
         """(y, saved): y, and what `backward` needs beside x."""
         y, hid = self._forward(x, out, True)
-        a, g, u = (h[:, :self.hidden] for h in hid)
-        return y, GatedFFNSaved(g, u, a)
+        return y, GatedFFNSaved(hid, self.hidden)
 
     def backward(self, dy, x, saved: GatedFFNSaved, want=None) -> dict:
         """The gradients for dy of the call that returned `saved`: "x", "w_gate", "w_up", "w_down" and the biases' there
@@ -320,28 +345,31 @@ class GatedFFN:
         p = GatedFfnGradParams.from_buffer_copy(self._grad_params)
         p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
         p.dy, p.dy_pitch, mdy = _rows("dy", dy, self.cout, self.dtype, self.device)
-        hid = [_rows(n, t, self.hidden, self.dtype, self.device) for n, t in zip(("g", "u", "a"), saved)]
-        if mdy != m or any(h[2] != m or (m > 1 and h[1] != hid[0][1]) for h in hid):
-            raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({[h[2] for h in hid]}) are not of one call")
-        p.g, p.u, p.a, p.h_pitch, p.m = hid[0][0], hid[1][0], hid[2][0], hid[0][1], m
+        hid = saved.rows
+        if mdy != m or hid.shape[1] != m or saved.channels != self.hidden or hid.dtype != self.dtype or hid.device != self.device:
+            raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({hid.shape[1]}) are not of one call")
+        at, step = hid.data_ptr(), 2 * m * p.h_pitch
+        p.a, p.g, p.u, p.m = at, at + step, at + 2 * step, m
         r = {}
-        for n in names:
-            if n == "x":
-                r[n] = empty_rows((*x.shape[:-1], self.cin), self.dtype, self.device)
-                p.dx, p.dx_pitch = r[n].data_ptr(), _up8(self.cin)
-            elif n == "w_gate":
-                r[n] = empty_rows((self.hidden, self.cin), self.dtype, self.device)
-                p.dw_gate, p.dwg_pitch = r[n].data_ptr(), _up8(self.cin)
-            elif n == "w_up":
-                r[n] = empty_rows((self.hidden, self.cin), self.dtype, self.device)
-                p.dw_up, p.dwu_pitch = r[n].data_ptr(), _up8(self.cin)
-            elif n == "w_down":
-                r[n] = empty_rows((self.cout, self.hidden), self.dtype, self.device)
-                p.dw_down, p.dwd_pitch = r[n].data_ptr(), _up8(self.hidden)
-            else:
-                r[n] = empty_rows((self.cout if n == "b_down" else self.hidden,), self.dtype, self.device)
-                setattr(p, "d" + n, r[n].data_ptr())
-        _gated_ffn_grad(p, self.device, self._grad_sizes, (m, p.h_pitch, *names))
+        if "x" in names:
+            r["x"] = _rows_like(x)
+            p.dx, p.dx_pitch = r["x"].data_ptr(), _up8(self.cin)
+        if "w_gate" in names:
+            r["w_gate"] = _rows_like(self.weights[0])
+            p.dw_gate, p.dwg_pitch = r["w_gate"].data_ptr(), _up8(self.cin)
+        if "w_up" in names:
+            r["w_up"] = _rows_like(self.weights[1])
+            p.dw_up, p.dwu_pitch = r["w_up"].data_ptr(), _up8(self.cin)
+        if "w_down" in names:
+            r["w_down"] = _rows_like(self.weights[2])
+            p.dw_down, p.dwd_pitch = r["w_down"].data_ptr(), _up8(self.hidden)
+        biases = [n for n in names if n[0] == "b"]
+        if biases:
+            sizes = [self.cout if n == "b_down" else self.hidden for n in biases]
+            for n, t in zip(biases, _vectors(sizes, self.dtype, self.device)):
+                r[n] = t
+                setattr(p, "d" + n, t.data_ptr())
+        _gated_ffn_grad(p, self.device, self._grad_sizes, (m, *names))
         return r
 
 
@@ -381,6 +409,7 @@ class ResidualNorm:
         self._forward_params = ResidualNormParams(**common, **ptrs)
         ptrs.pop("b_pre", None)
         self._grad_params = ResidualNormGradParams(**common, **ptrs)
+        self._names = [n for n, t in self.params.items() if t is not None]
         self._sizes = {}
 
     def _device(self, t):
@@ -406,19 +435,19 @@ class ResidualNorm:
         p = ResidualNormParams.from_buffer_copy(self._forward_params)
         p.x, p.x_pitch, m = _rows("x", x, c, dt, dev)
         p.m = m
-        y, h, shape = x, None, x.shape
+        y, h = x, None
         if f is not None:
             p.f, p.f_pitch = _like("f", f, m, c, dt, dev)
             if gate is not None:
                 self._gate(p, gate, m, dev)
-            y = empty_rows(shape, dt, dev)
+            y = _rows_like(x)
             p.y, p.y_pitch = y.data_ptr(), _up8(c)
         else:
             if gate is not None or self.pre == "none":
                 raise FlyHighError("without f there is no gate, and a norm before the block")
             p.post, p.scale, p.w_post, p.b_post = 0, None, None, None
         if self.pre != "none":
-            h = empty_rows(shape, dt, dev)
+            h = _rows_like(x)
             p.h, p.h_pitch = h.data_ptr(), _up8(c)
         _residual_norm(p, dev)
         return y, h
@@ -438,11 +467,11 @@ class ResidualNorm:
         if dh is not None:
             p.dh, p.dh_pitch = (ptr, pitch) if dy is None else _like("dh", dh, m, c, dt, dev)
             p.y, p.y_pitch = _like("y", y, m, c, dt, dev)
-        r = {"x": empty_rows(first.shape, dt, dev)}
+        r = {"x": _rows_like(first)}
         p.dx, p.dx_pitch = r["x"].data_ptr(), _up8(c)
         if f is not None:
             p.f, p.f_pitch = _like("f", f, m, c, dt, dev)
-            r["f"] = empty_rows(first.shape, dt, dev)
+            r["f"] = _rows_like(first)
             p.df, p.df_pitch = r["f"].data_ptr(), _up8(c)
             if gate is not None:
                 self._gate(p, gate, m, dev)
@@ -452,9 +481,10 @@ class ResidualNorm:
             if gate is not None:
                 raise FlyHighError("without f there is no gate")
             p.post, p.scale, p.w_post, p.b_post = 0, None, None, None
-        for n, t in self.params.items():
-            if t is not None and (f is not None or n == "w_pre" or n == "b_pre"):
-                r[n] = empty_rows((c,), dt, dev)
-                setattr(p, "d" + n, r[n].data_ptr())
+        names = self._names if f is not None else [n for n in self._names if n in ("w_pre", "b_pre")]
+        if names:
+            for n, t in zip(names, _vectors([c] * len(names), dt, dev)):
+                r[n] = t
+                setattr(p, "d" + n, t.data_ptr())
         _residual_norm_grad(p, dev, self._sizes, (m, p.gates))
         return r
