@@ -17,80 +17,12 @@
 #include <type_traits>
 
 #include "fh_device.cuh"
+#include "ffn_parts.cuh"
 #include "fh_kernels.h"
+#include "gated_ffn_map.cuh"
 #include "launch.h"
-#include "row_ops.cuh"
-#include "umma_tile.cuh"
-
-using namespace rows;
 
 namespace {
-
-constexpr int kMaxChannels = 1 << 20;
-constexpr int kSms = 148;
-
-__device__ unsigned long long g_ffn_timeouts;
-
-__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-// 1 / (1 + exp(-z)): far out the power is 0 or infinite and the quotient 1 or 0
-__device__ __forceinline__ float2 sigmoid2(float2 z) {
-    const float2 t = mul2(z, pair(-1.44269504f));  // -log2(e) z
-    const float2 d = add2(make_float2(ex2(t.x), ex2(t.y)), pair(1.0f));
-    return make_float2(rcp(d.x), rcp(d.y));
-}
-// act(g) of a pair. 0.5 (1 + tanh z) = sigmoid(2 z), so the tanh form of gelu is g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3))
-template <int ACT>
-__device__ __forceinline__ float2 act_of(float2 g) {
-    if (ACT == FH_ACT_RELU) return make_float2(g.x > 0.0f ? g.x : 0.0f, g.y > 0.0f ? g.y : 0.0f);
-    if (ACT == FH_ACT_GELU) {
-        const float2 h = mul2(g, pair(0.5f));
-        return fma2(h, make_float2(erff(g.x * 0.70710678f), erff(g.y * 0.70710678f)), h);
-    }
-    float2 z = g;
-    if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(mul2(g, g), pair(0.07135481f), pair(1.59576912f)));
-    const float2 s = sigmoid2(z);
-    return ACT == FH_ACT_SIGMOID ? s : mul2(g, s);
-}
-// act(g) and its derivative
-template <int ACT>
-__device__ __forceinline__ void act_both(float2 g, float2& v, float2& dv) {
-    if (ACT == FH_ACT_RELU) {
-        v = make_float2(g.x > 0.0f ? g.x : 0.0f, g.y > 0.0f ? g.y : 0.0f);
-        dv = make_float2(g.x > 0.0f ? 1.0f : 0.0f, g.y > 0.0f ? 1.0f : 0.0f);
-    } else if (ACT == FH_ACT_GELU) {
-        const float2 cdf = fma2(make_float2(erff(g.x * 0.70710678f), erff(g.y * 0.70710678f)), pair(0.5f), pair(0.5f));
-        const float2 q = mul2(mul2(g, g), pair(-0.72134752f));  // exp(-g^2 / 2) as a power of two
-        v = mul2(g, cdf);
-        dv = fma2(mul2(g, pair(0.39894228f)), make_float2(ex2(q.x), ex2(q.y)), cdf);
-    } else {
-        const float2 g2 = mul2(g, g);
-        float2 z = g;
-        if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(g2, pair(0.07135481f), pair(1.59576912f)));
-        const float2 s = sigmoid2(z), c = fma2(s, pair(-1.0f), pair(1.0f));  // 1 - s
-        if (ACT == FH_ACT_SIGMOID) {
-            v = s;
-            dv = mul2(s, c);
-        } else {
-            v = mul2(g, s);
-            // s + g s (1 - s) dz / dg
-            const float2 w = mul2(v, c);
-            dv = ACT == FH_ACT_SILU ? add2(s, w) : fma2(w, fma2(g2, pair(0.21406443f), pair(1.59576912f)), s);
-        }
-    }
-}
 
 enum Tail { PLAIN, GLU, GLU_GRAD };
 constexpr int kGroupM = 8;  // tiles of rows that are walked together, so that their operands stay in L2
@@ -137,7 +69,6 @@ constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kStageA = 128 * 128;  // 128 rows of 64 elements
 constexpr int kRing = 163840;   // shared memory of the operand ring
 constexpr int kMaxStages = 8;
-constexpr int kTile = 32 * 64;  // a tail's staging tile: 32 rows of 32 columns, 64-byte swizzled
 constexpr int kTiles = 4;       // per warp: two groups of 64 columns in turn
 constexpr int kBars = 512;
 constexpr int kSmem = 1024 + kRing + kEpiWarps * kTiles * kTile + kBars;
@@ -166,88 +97,6 @@ __device__ __forceinline__ Item item_of(const Work& w, int i) {
         t.k1 = (int)((long long)kb * (t.split + 1) / j.splits);
     }
     return t;
-}
-
-// 16 columns (half h of 32) of this lane's row of a staging tile: chunk c of a row lies at c ^ (row / 2 % 4)
-__device__ __forceinline__ uint32_t tile_at(uint32_t tile, int lane, int h, int c) {
-    return tile + lane * 64 + (((2 * h + c) ^ ((lane >> 1) & 3)) << 4);
-}
-template <typename T>
-__device__ __forceinline__ void tile_put(uint32_t tile, int lane, int h, const float2 (&v)[8]) {
-#pragma unroll
-    for (int c = 0; c < 2; c++)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(tile_at(tile, lane, h, c)), "r"(Elem<T>::from2(v[4 * c].x, v[4 * c].y)),
-                     "r"(Elem<T>::from2(v[4 * c + 1].x, v[4 * c + 1].y)), "r"(Elem<T>::from2(v[4 * c + 2].x, v[4 * c + 2].y)),
-                     "r"(Elem<T>::from2(v[4 * c + 3].x, v[4 * c + 3].y))
-                     : "memory");
-}
-template <typename T>
-__device__ __forceinline__ void tile_get(uint32_t tile, int lane, int h, float2 (&v)[8]) {
-#pragma unroll
-    for (int c = 0; c < 2; c++) {
-        uint32_t q[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                     : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                     : "r"(tile_at(tile, lane, h, c))
-                     : "memory");
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[4 * c + i] = Elem<T>::to2(q[i]);
-    }
-}
-// this lane's row of a staging tile, `valid` columns of it, to p: in place of a tensor copy, which writes whole 16-byte
-// pieces, where the output's columns end inside one
-template <typename T>
-__device__ __noinline__ void tile_out(uint32_t tile, int lane, T* p, int valid) {
-    for (int c = 0; 8 * c < valid; c++) {
-        uint4 q;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
-                     : "r"(tile_at(tile, lane, 0, c))
-                     : "memory");
-        store_chunk(p + 8 * c, valid - 8 * c, unpack<T>(q));
-    }
-}
-// 32 columns of a bias (the same for all lanes) as they lie in memory, 0 past `cols` and where there is none
-template <typename T>
-__device__ __forceinline__ void load_bias(const void* bias, int c, int cols, uint32_t (&q)[16]) {
-    const T* p = static_cast<const T*>(bias) + c;
-    if (bias && c + 32 <= cols) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint4 t = reinterpret_cast<const uint4*>(p)[i];
-            q[4 * i] = t.x, q[4 * i + 1] = t.y, q[4 * i + 2] = t.z, q[4 * i + 3] = t.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            q[i] = Elem<T>::from2(bias && c + 2 * i < cols ? Elem<T>::to(p[2 * i]) : 0.0f,
-                                  bias && c + 2 * i + 1 < cols ? Elem<T>::to(p[2 * i + 1]) : 0.0f);
-    }
-}
-// 16 accumulators as pairs, and a bias added to them
-__device__ __forceinline__ void pairs(const uint32_t* r, float2 (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-}
-template <typename T>
-__device__ __forceinline__ void add_bias(const uint32_t* q, float2 (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = add2(v[i], Elem<T>::to2(q[i]));
-}
-template <int ACT>
-__device__ __forceinline__ void glu16(const float2 (&g)[8], const float2 (&u)[8], float2 (&a)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) a[i] = mul2(act_of<ACT>(g[i]), u[i]);
-}
-template <int ACT>
-__device__ __forceinline__ void glu_grad16(const float2 (&da)[8], float2 (&g)[8], float2 (&u)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float2 v, dv;
-        act_both<ACT>(g[i], v, dv);
-        g[i] = mul2(mul2(da[i], u[i]), dv);
-        u[i] = mul2(da[i], v);
-    }
 }
 
 // CTAS = 2: a pair of CTAs computes 256 x bn tiles, each CTA holding 128 rows of A, half the columns' rows of B and the
@@ -589,13 +438,15 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 8 elements of a row from k on, 0 past its end (the last steps of K)
+// 8 elements of a row from k on, 0 past its end (the last step of K). The 16 bytes that hold an element of the row are read
+// whole (they lie inside its pitch) and what is not the row's is masked.
 template <typename T>
-__device__ __noinline__ uint4 load_k(const T* row, int k, int end) {
-    if (k >= end) return make_uint4(0, 0, 0, 0);
-    const Chunk c = load_chunk(row + k, end - k);
-    return make_uint4(Elem<T>::from2(c.v[0].x, c.v[0].y), Elem<T>::from2(c.v[1].x, c.v[1].y), Elem<T>::from2(c.v[2].x, c.v[2].y),
-                      Elem<T>::from2(c.v[3].x, c.v[3].y));
+__device__ __forceinline__ uint4 load_k(const T* row, int k, int end) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (k >= end) return q;
+    q = *reinterpret_cast<const uint4*>(row + k);
+    auto cut = [&](uint32_t w, int first) { return k + first + 1 < end ? w : k + first < end ? w & 0xffffu : 0u; };
+    return make_uint4(cut(q.x, 0), cut(q.y, 2), cut(q.z, 4), cut(q.w, 6));
 }
 // 16 bytes of a weight: read once, so not kept in L1
 template <typename T>
@@ -836,47 +687,7 @@ __global__ void __launch_bounds__(256) k_column_parts(const ColumnSums w) {
     }
 }
 
-#define FH_TRY(call)                              \
-    do {                                          \
-        const cudaError_t e_ = (call);            \
-        if (e_ != cudaSuccess) return e_;         \
-    } while (0)
-
 // ---- host: tensor maps, the choice of tiles, launches ----
-
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
-            r != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeTiled>(p);
-    }();
-    return fn;
-}
-
-struct Matrix {  // [rows][cols] of 16-bit elements
-    const void* p;
-    long long pitch;
-    long long rows;
-    int cols;
-};
-
-// boxes of 64 columns x `box` rows, 128-byte swizzled (operands), or of 32 x 32, 64-byte swizzled (box 0: the tails)
-cudaError_t map_of(CUtensorMap* map, const Matrix& x, int box, int dtype) {
-    const EncodeTiled fn = encode_tiled();
-    if (!fn) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)x.cols, (cuuint64_t)x.rows}, strides[1] = {(cuuint64_t)x.pitch * 2};
-    const cuuint32_t boxes[2] = {box ? 64u : 32u, box ? (cuuint32_t)box : 32u}, one[2] = {1, 1};
-    const CUresult r = fn(map, dtype == FH_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                          const_cast<void*>(x.p), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          box ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
 
 // A product before its tiles are chosen: terms of (A, B) with A [m][k] (or [k][m], mn_a) and B [n][k] (or [k][n], mn_b)
 struct Product {
@@ -1040,14 +851,14 @@ cudaError_t finish(const Sums& sums, cudaStream_t st) {
 
 // Whether a forward call takes the form for few rows: by estimates in us of both. It reads the weights at about 5.5 TB/s,
 // slowed as every CTA reads 8 NT rows of x beside its 16 weight rows, with about 4 us of launches and latencies; the tiles
-// need about 12 us and 5.2 TB/s whatever the rows. Measured (bf16, us, this form / tiles): 1 row of 1024 -> 4096 7.2 / 19,
-// 32 rows 13.7 / 19; 2048 -> 8192 24 / 33 with 1 row, 32 / 33 with 16, 41 / 33 with 32; 4096 -> 16384 75 / 89 with 1, 111 / 89
+// need about 10 us and 5.2 TB/s whatever the rows. Measured (bf16, us, this form / tiles): 1 row of 1024 -> 4096 7.2 / 19,
+// 32 rows 13.6 / 18.5; 2048 -> 8192 24 / 30 with 1 row, 32 / 30 with 16, 41 / 30 with 32; 4096 -> 16384 75 / 84 with 1, 109 / 84
 // with 16.
 bool takes_few_rows(long long m, int cin, int hidden, int cout) {
     if (m > 32) return false;
     const double mb = 2e-6 * hidden * (2.0 * cin + cout);
     const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
-    return 4 + mb / 5.5 * (0.8 + 0.325 * nt) < 12 + mb / 5.2;
+    return 4 + mb / 5.5 * (0.8 + 0.325 * nt) < 10 + mb / 5.2;
 }
 template <typename T, int NT, bool GATED>
 cudaError_t launch_rows(const RowsArgs<T>& p, cudaStream_t st) {
@@ -1118,6 +929,9 @@ Product down_of(const FhGatedFfnParams& p) {
     return q;
 }
 
+// whether a forward call runs as one kernel (gated_ffn_map.cuh): few channels, and nothing of the hidden values is kept
+bool on_map(const FhGatedFfnParams& p) { return !p.g && p.cin <= kMapChannels && p.cout <= kMapChannels; }
+
 template <typename T>
 cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {
     const Product glu = glu_of(p), down = down_of(p);
@@ -1127,6 +941,7 @@ cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {
         fhk::PdlScope pdl(true);
         return few_rows<T, false>(down, p.act, st);
     }
+    if (on_map(p)) return block_on_map<T>(p, st);
     FH_TRY((products<T, GLU>(&glu, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
     fhk::PdlScope pdl(true);  // what follows waits on a kernel of this file
     FH_TRY((products<T, PLAIN>(&down, 1, p.act, p.dtype, p.wait_cycles, static_cast<float*>(p.scratch), &sums, st)));
@@ -1225,7 +1040,7 @@ cudaError_t gradient(const FhGatedFfnGradParams& p, cudaStream_t st) {
 }  // namespace
 
 extern "C" size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p) {
-    if (!p || !good_sizes(p) || p->m == 0 || takes_few_rows(p->m, p->cin, p->hidden, p->cout)) return 0;
+    if (!p || !good_sizes(p) || p->m == 0 || takes_few_rows(p->m, p->cin, p->hidden, p->cout) || on_map(*p)) return 0;
     const Product down = down_of(*p);
     return scratch_floats<PLAIN>(&down, 1) * 4;
 }
