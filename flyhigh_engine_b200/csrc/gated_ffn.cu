@@ -136,30 +136,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     fence_after();
     uint32_t tbase;
     asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tbase) : "r"(slot));
+    tbase = uniform(tbase);
     pdl_wait();
     pdl_trigger();
 
     const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+    // the matrix instructions are issued by the pair's first CTA
+    auto free_accumulators = [&](uint32_t bar) {
+        if (CTAS == 1 || rank == 0) bar_arrive(bar);
+        else bar_arrive_cluster(map_rank(bar, 0));
+    };
     bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {  // by whole warps
+        if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar, parity, w.limit, &g_ffn_timeouts));
+        return ok;
+    };
     if (warp == 8) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 1;  // the ring starts empty
-            for (int i = first; ok && i < w.items; i += step) {
-                const Item t = item_of(w, i);
-                const Job& j = *t.j;
-                const int row = t.tm * 128 * CTAS + (int)rank * 128;
-                for (int k = t.k0; k < t.k1; k++) {
-                    if (!bar_wait(empty + 8 * s, ph, w.limit, &g_ffn_timeouts)) {
-                        ok = false;
-                        break;
-                    }
-                    const int term = TAIL != GLU && k >= j.kb[0], kk = (k - (term ? j.kb[0] : 0)) * BK;
+        int s = 0;
+        uint32_t ph = 1;  // the ring starts empty
+        for (int i = first; ok && i < w.items; i += step) {
+            const Item t = item_of(w, i);
+            const Job& j = *t.j;
+            const int row = t.tm * 128 * CTAS + (int)rank * 128;
+            const int kb0 = j.kb[0];
+            const bool mn_a = j.mn_a, mn_b = j.mn_b;
+            for (int k = t.k0; k < t.k1; k++) {
+                if (!wait(empty + 8 * s, ph)) break;
+                const int term = TAIL != GLU && k >= kb0, kk = (k - (term ? kb0 : 0)) * BK;
+                const uint32_t bar = CTAS == 2 ? map_rank(full + 8 * s, 0) : full + 8 * s;
+                const uint32_t da = base + s * stage_bytes, db = da + kStageA;
+                const CUtensorMap* ma = &j.a[term];
+                const CUtensorMap* mb = &j.b[TAIL == GLU && CTAS == 2 ? rank : term];
+                if (lane == 0) {
                     if (rank == 0) bar_expect(full + 8 * s, CTAS * stage_bytes);
-                    const uint32_t bar = CTAS == 2 ? map_rank(full + 8 * s, 0) : full + 8 * s;
-                    const uint32_t da = base + s * stage_bytes, db = da + kStageA;
-                    const CUtensorMap* ma = &j.a[term];
-                    if (j.mn_a) {
+                    if (mn_a) {
                         tensor_load<CTAS>(da, ma, row, kk, bar);
                         tensor_load<CTAS>(da + 8192, ma, row + 64, kk, bar);
                     } else {
@@ -167,25 +177,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                     }
                     if (TAIL == GLU) {
                         const int c = t.tn * (bn / 2);
-                        if (CTAS == 2) {
-                            tensor_load<CTAS>(db, &j.b[rank], kk, c, bar);
-                        } else {
-                            tensor_load<CTAS>(db, &j.b[0], kk, c, bar);
-                            tensor_load<CTAS>(db + (bn / 2) * 128, &j.b[1], kk, c, bar);
-                        }
+                        tensor_load<CTAS>(db, mb, kk, c, bar);
+                        if (CTAS == 1) tensor_load<CTAS>(db + (bn / 2) * 128, &j.b[1], kk, c, bar);
                     } else {
                         const int c = t.tn * bn + (int)rank * nb;
-                        if (j.mn_b)
-                            for (int q = 0; q < nb / 64; q++) tensor_load<CTAS>(db + q * 8192, &j.b[term], c + 64 * q, kk, bar);
+                        if (mn_b)
+                            for (int q = 0; q < nb / 64; q++) tensor_load<CTAS>(db + q * 8192, mb, c + 64 * q, kk, bar);
                         else
-                            tensor_load<CTAS>(db, &j.b[term], kk, c, bar);
+                            tensor_load<CTAS>(db, mb, kk, c, bar);
                     }
-                    if (++s == stages) s = 0, ph ^= 1;
                 }
+                __syncwarp();
+                if (++s == stages) s = 0, ph ^= 1;
             }
         }
     } else if (warp == 9) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             int s = 0, n = 0;
             uint32_t ph = 0;
             for (int i = first; ok && i < w.items; i += step, n++) {
@@ -193,28 +200,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 const Job& j = *t.j;
                 const int b = n & 1;
                 const uint32_t d = tbase + b * bn;
-                const uint32_t idesc = instr_desc(sizeof(T) == 2 && !std::is_same<T, __half>::value, j.mn_a, j.mn_b, 128 * CTAS, bn);
+                const uint32_t idesc = instr_desc(!std::is_same<T, __half>::value, j.mn_a, j.mn_b, 128 * CTAS, bn);
                 // one K step of 16: 32 bytes along a K-major tile's rows, two 8-k groups of an MN-major one
                 const uint32_t sa = j.mn_a ? 2048 >> 4 : 32 >> 4, sb = j.mn_b ? 2048 >> 4 : 32 >> 4;
-                if (!bar_wait(tempty + 8 * b, ((n >> 1) & 1) ^ 1, w.limit, &g_ffn_timeouts)) {
-                    ok = false;
-                    break;
-                }
+                if (!wait(tempty + 8 * b, ((n >> 1) & 1) ^ 1)) break;
                 fence_after();
                 for (int k = t.k0; k < t.k1; k++) {
-                    if (!bar_wait(full + 8 * s, ph, w.limit, &g_ffn_timeouts)) {
-                        ok = false;
-                        break;
-                    }
+                    if (!wait(full + 8 * s, ph)) break;
                     fence_after();
                     const uint32_t da = base + s * stage_bytes;
                     const uint64_t ad = tile_desc(da, 8192), bd = tile_desc(da + kStageA, 8192);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) mma<CTAS>(d, ad + q * sa, bd + q * sb, idesc, (k > t.k0 || q > 0) ? 1u : 0u);
-                    commit<CTAS>(empty + 8 * s);
+                    for (int q = 0; q < 4; q++)
+                        if (lane == 0) mma<CTAS>(d, ad + q * sa, bd + q * sb, idesc, (k > t.k0 || q > 0) ? 1u : 0u);
+                    if (lane == 0) commit<CTAS>(empty + 8 * s);
                     if (++s == stages) s = 0, ph ^= 1;
                 }
-                if (ok) commit<CTAS>(tfull + 8 * b);
+                if (ok && lane == 0) commit<CTAS>(tfull + 8 * b);
             }
         }
     } else {
@@ -250,8 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 if (lane == 0) stores_read<1>();  // all but the last group's stores: the other two tiles
                 fetch(lo, turn);
             }
-            ok = bar_wait(tfull + 8 * b, (n >> 1) & 1, w.limit, &g_ffn_timeouts);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (!wait(tfull + 8 * b, (n >> 1) & 1)) break;
             fence_after();
             const uint32_t acc = tbase + ((uint32_t)(q * 32) << 16) + b * bn;
             for (int c0 = lo; c0 < hi; c0 += group) {
@@ -261,10 +262,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 if (keep) dst = tiles + (turn & 3) * kTile, dst1 = tiles + ((turn + 1) & 3) * kTile, dst2 = tiles + ((turn + 2) & 3) * kTile;
                 if (TAIL == GLU_GRAD) {
                     if (alive) {
-                        ok = bar_wait(gbar + 8 * (turn & 1), (gph >> (turn & 1)) & 1, w.limit, &g_ffn_timeouts);
+                        wait(gbar + 8 * (turn & 1), (gph >> (turn & 1)) & 1);
                         gph ^= 1u << (turn & 1);
                     }
-                    if (!__all_sync(0xffffffffu, ok)) break;
+                    if (!ok) break;
                 } else {
                     // what these tiles held has been read: all but the last group's stores (of kept outputs: the last store)
                     if (lane == 0) stores_read<1>();
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                     if (cs + 32 >= hi) {  // the accumulators have been read
                         fence_before();
                         __syncwarp();
-                        if (lane == 0) bar_arrive_cluster(map_rank(tempty + 8 * b, 0));
+                        if (lane == 0) free_accumulators(tempty + 8 * b);
                     }
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -381,12 +382,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 }
                 turn += keep ? 3 : 1;
             }
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (!ok) break;
             // a half without columns of a narrow tile
             if (lo >= hi) {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive_cluster(map_rank(tempty + 8 * b, 0));
+                if (lane == 0) free_accumulators(tempty + 8 * b);
             }
         }
         if (lane == 0) stores_done();

@@ -66,86 +66,89 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
     fence_after();
     uint32_t tbase;
     asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(tbase) : "r"(slot_at));
+    tbase = uniform(tbase);
     pdl_wait();
     pdl_trigger();
 
     bool ok = true;
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (ok) ok = bar_wait(bar, parity & 1, w.limit, &g_ffn_timeouts);
+    auto wait = [&](uint32_t bar, uint32_t parity) {  // by whole warps
+        if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar, parity & 1, w.limit, &g_ffn_timeouts));
         return ok;
     };
     if (warp == 16) {
-        if (lane == 0) {
-            int n = 0, wi = 0, s = 0;
-            for (int i = blockIdx.x; ok && i < w.items; i += gridDim.x, n++) {
-                const int b = n % xbufs;
-                if (!wait(xempty + 8 * b, n / xbufs + 1)) break;
+        int n = 0, wi = 0, s = 0;
+        for (int i = blockIdx.x; ok && i < w.items; i += gridDim.x, n++) {
+            const int b = n % xbufs;
+            if (!wait(xempty + 8 * b, n / xbufs + 1)) break;
+            if (lane == 0) {
                 bar_expect(xfull + 8 * b, groups * xtile);
                 for (int g = 0; g < groups; g++)
                     for (int k = 0; k < kb; k++)
                         tensor_load<1>(xs + (b * 2 + g) * xtile + k * 16384, &w.x, k * BK, (i * groups + g) * 128, xfull + 8 * b);
-                if (w.resident && n > 0) continue;
-                for (int c = 0; c < chunks; c++, wi++) {
-                    if (!wait(wempty + 8 * s, wi / w.slots + 1)) break;
-                    const uint32_t at = ws + s * wbytes, bar = wfull + 8 * s;
+            }
+            __syncwarp();
+            if (w.resident && n > 0) continue;
+            for (int c = 0; c < chunks; c++, wi++) {
+                if (!wait(wempty + 8 * s, wi / w.slots + 1)) break;
+                const uint32_t at = ws + s * wbytes, bar = wfull + 8 * s;
+                if (lane == 0) {
                     bar_expect(bar, wbytes);
                     for (int k = 0; k < kb; k++) {
                         tensor_load<1>(at + k * 16384, &w.wg, k * BK, c * kMapChunk, bar);
                         tensor_load<1>(at + k * 16384 + 8192, &w.wu, k * BK, c * kMapChunk, bar);
                     }
                     tensor_load<1>(at + kb * 16384, &w.wd, c * kMapChunk, 0, bar);
-                    if (++s == w.slots) s = 0;
                 }
+                __syncwarp();
+                if (++s == w.slots) s = 0;
             }
         }
     } else if (warp == 17) {
-        if (lane == 0) {
-            const uint32_t id1 = instr_desc(bf16, false, false, 128, 128), id2 = instr_desc(bf16, false, false, 128, w.np);
-            int n = 0, u = 0, s = 0, wi = 0;  // u: chunks so far; s: the ring's slot of the next chunk
-            for (int i = blockIdx.x; ok && i < w.items; i += gridDim.x, n++) {
-                const int b = n % xbufs;
-                if (!wait(xfull + 8 * b, n / xbufs)) break;
-                fence_after();
-                int last = 0;  // the slot of the chunk before
-                for (int c = 0; c <= chunks && ok; c++) {
-                    const int here = w.resident ? c : s;
-                    if (c < chunks) {
-                        if (!w.resident || n == 0) {
-                            if (!wait(wfull + 8 * here, wi / w.slots)) break;
-                            fence_after();
+        const uint32_t id1 = instr_desc(bf16, false, false, 128, 128), id2 = instr_desc(bf16, false, false, 128, w.np);
+        int n = 0, u = 0, s = 0, wi = 0;  // u: chunks so far; s: the ring's slot of the next chunk
+        for (int i = blockIdx.x; ok && i < w.items; i += gridDim.x, n++) {
+            const int b = n % xbufs;
+            if (!wait(xfull + 8 * b, n / xbufs)) break;
+            int last = 0;  // the slot of the chunk before
+            for (int c = 0; c <= chunks && ok; c++) {
+                const int here = w.resident ? c : s;
+                if (c < chunks) {
+                    if ((!w.resident || n == 0) && !wait(wfull + 8 * here, wi / w.slots)) break;
+                    for (int g = 0; g < groups; g++) {
+                        if (!wait(d1empty + 8 * g, u + 1)) break;
+                        fence_after();
+                        uint64_t ad = tile_desc(xs + (b * 2 + g) * xtile, 0), bd = tile_desc(ws + here * wbytes, 0);
+                        for (int k = 0; k < w.ksteps; k++) {
+                            if (lane == 0) mma<1>(tbase + g * 128, ad, bd, id1, k > 0);
+                            const uint32_t step = (k & 3) == 3 ? (16384 - 96) >> 4 : 32 >> 4;  // the next 16 of K, or K block
+                            ad += step, bd += step;
                         }
-                        for (int g = 0; g < groups && ok; g++) {
-                            if (!wait(d1empty + 8 * g, u + 1)) break;
-                            fence_after();
-                            const uint64_t ad = tile_desc(xs + (b * 2 + g) * xtile, 0), bd = tile_desc(ws + here * wbytes, 0);
-                            for (int k = 0; k < w.ksteps; k++) {
-                                const uint32_t o = (k >> 2) * (16384 >> 4) + (k & 3) * (32 >> 4);
-                                mma<1>(tbase + g * 128, ad + o, bd + o, id1, k > 0);
-                            }
-                            commit<1>(d1full + 8 * g);
-                        }
-                        if (!ok) break;
-                        if (c == chunks - 1) commit<1>(xempty + 8 * b);
+                        if (lane == 0) commit<1>(d1full + 8 * g);
                     }
-                    if (c > 0) {
-                        for (int g = 0; g < groups && ok; g++) {
-                            if (!wait(afull + 8 * g, u - 1)) break;
-                            if (c == 1 && !wait(d2empty + 8 * g, n + 1)) break;
-                            fence_after();
-                            const uint64_t ad = tile_desc(as + g * 16384, 0), bd = tile_desc(ws + last * wbytes + kb * 16384, 0);
-                            for (int k = 0; k < 4; k++)
-                                mma<1>(tbase + 256 + g * 128, ad + k * (32 >> 4), bd + k * (32 >> 4), id2, c > 1 || k > 0);
+                    if (!ok) break;
+                    if (c == chunks - 1 && lane == 0) commit<1>(xempty + 8 * b);
+                }
+                if (c > 0) {
+                    for (int g = 0; g < groups; g++) {
+                        if (!wait(afull + 8 * g, u - 1)) break;
+                        if (c == 1 && !wait(d2empty + 8 * g, n + 1)) break;
+                        fence_after();
+                        const uint64_t ad = tile_desc(as + g * 16384, 0), bd = tile_desc(ws + last * wbytes + kb * 16384, 0);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (lane == 0) mma<1>(tbase + 256 + g * 128, ad + k * (32 >> 4), bd + k * (32 >> 4), id2, c > 1 || k > 0);
+                        if (lane == 0) {
                             commit<1>(aempty + 8 * g);
                             if (c == chunks) commit<1>(d2full + 8 * g);
                         }
-                        if (!ok) break;
-                        if (!w.resident) commit<1>(wempty + 8 * last);
                     }
-                    last = here;
-                    if (c < chunks) {
-                        u++, wi++;
-                        if (++s == w.slots) s = 0;
-                    }
+                    if (!ok) break;
+                    if (!w.resident && lane == 0) commit<1>(wempty + 8 * last);
+                }
+                last = here;
+                if (c < chunks) {
+                    u++, wi++;
+                    if (++s == w.slots) s = 0;
                 }
             }
         }
@@ -157,11 +160,10 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
         const int span = w.np <= 64 ? 32 : 64, lo = half * span, hi = min(w.np, lo + span);
         int n = 0;
         uint32_t u = 0;
-        auto all_ok = [&]() { return __all_sync(0xffffffffu, ok); };
         for (int i = blockIdx.x; i < w.items; i += gridDim.x, n++) {
             for (int c = 0; c < chunks; c++, u++) {
                 wait(d1full + 8 * g, u);
-                if (!all_ok()) break;
+                if (!ok) break;
                 fence_after();
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
                     if (h == 1) {
                         fence_before();
                         __syncwarp();
-                        if (lane == 0) bar_arrive_cluster(map_rank(d1empty + 8 * g, 0));
+                        if (lane == 0) bar_arrive(d1empty + 8 * g);
                     }
                     float2 v[8], gv[8], uv[8];
                     pairs(rg, gv);
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
                     }
                     if (h == 0) {  // the down projection of the chunk before has read a's place
                         wait(aempty + 8 * g, u + 1);
-                        if (!all_ok()) break;
+                        if (!ok) break;
                     }
 #pragma unroll
                     for (int e = 0; e < 2; e++)
@@ -206,14 +208,14 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
                                      : "memory");
                     __syncwarp();
                 }
-                if (!all_ok()) break;
+                if (!ok) break;
                 fence_async();
                 __syncwarp();
-                if (lane == 0) bar_arrive_cluster(map_rank(afull + 8 * g, 0));
+                if (lane == 0) bar_arrive(afull + 8 * g);
             }
-            if (!all_ok()) break;
+            if (!ok) break;
             wait(d2full + 8 * g, n);
-            if (!all_ok()) break;
+            if (!ok) break;
             fence_after();
             const int row = (i * groups + g) * 128 + q * 32;
             for (int c0 = lo; c0 < hi; c0 += 32) {
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
                 if (c0 + 32 >= hi) {
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive_cluster(map_rank(d2empty + 8 * g, 0));
+                    if (lane == 0) bar_arrive(d2empty + 8 * g);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
             if (lo >= hi) {
                 fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive_cluster(map_rank(d2empty + 8 * g, 0));
+                if (lane == 0) bar_arrive(d2empty + 8 * g);
             }
         }
         if (lane == 0) stores_done();
