@@ -39,11 +39,12 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// 1 / (1 + exp(-z)): far out the power is 0 or infinite and the quotient 1 or 0
+// 1 / (1 + exp(-z)) of a pair, with one reciprocal for both (the special functions' unit is what bounds the narrow cases):
+// 1 / a = b / (a b). The powers stop at 2^60 so that their product stays finite; beyond (z < -41) the result is 9e-19.
 __device__ __forceinline__ float2 sigmoid2(float2 z) {
     const float2 t = mul2(z, pair(-1.44269504f));  // -log2(e) z
-    const float2 d = add2(make_float2(ex2(t.x), ex2(t.y)), pair(1.0f));
-    return make_float2(rcp(d.x), rcp(d.y));
+    const float2 d = add2(make_float2(ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))), pair(1.0f));
+    return mul2(pair(rcp(d.x * d.y)), make_float2(d.y, d.x));
 }
 // Phi(g) = erfc(-g / sqrt 2) / 2 and exp(-g^2 / 2), by formula 7.1.26 of Abramowitz and Stegun (erfc to 1.5e-7): with
 // z = |g| / sqrt 2 and t = 1 / (1 + p z), erfc(z) = t (a1 + t (a2 + ... + t a5)) exp(-z^2)
@@ -71,7 +72,8 @@ __device__ __forceinline__ float2 act_of(float2 g) {
     float2 z = g;
     if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(mul2(g, g), pair(0.07135481f), pair(1.59576912f)));
     const float2 s = sigmoid2(z);
-    return ACT == FH_ACT_SIGMOID ? s : mul2(g, s);
+    // the smallest of (NaN, 60) is 60: a NaN is put back
+    return ACT == FH_ACT_SIGMOID ? make_float2(g.x != g.x ? g.x : s.x, g.y != g.y ? g.y : s.y) : mul2(g, s);
 }
 // act(g) and its derivative
 template <int ACT>

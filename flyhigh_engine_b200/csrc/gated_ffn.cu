@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         return ok;
     };
     if (warp == 8) {
+        const bool leader = elected();
         int s = 0;
         uint32_t ph = 1;  // the ring starts empty
         for (int i = first; ok && i < w.items; i += step) {
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 const uint32_t da = base + s * stage_bytes, db = da + kStageA;
                 const CUtensorMap* ma = &j.a[term];
                 const CUtensorMap* mb = &j.b[TAIL == GLU && CTAS == 2 ? rank : term];
-                if (lane == 0) {
+                if (leader) {
                     if (rank == 0) bar_expect(full + 8 * s, CTAS * stage_bytes);
                     if (mn_a) {
                         tensor_load<CTAS>(da, ma, row, kk, bar);
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         }
     } else if (warp == 9) {
         if (rank == 0) {
+            const bool leader = elected();
             int s = 0, n = 0;
             uint32_t ph = 0;
             for (int i = first; ok && i < w.items; i += step, n++) {
@@ -210,13 +212,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                     fence_after();
                     const uint32_t da = base + s * stage_bytes;
                     const uint64_t ad = tile_desc(da, 8192), bd = tile_desc(da + kStageA, 8192);
+                    if (leader) {
 #pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        if (lane == 0) mma<CTAS>(d, ad + q * sa, bd + q * sb, idesc, (k > t.k0 || q > 0) ? 1u : 0u);
-                    if (lane == 0) commit<CTAS>(empty + 8 * s);
+                        for (int q = 0; q < 4; q++) mma<CTAS>(d, ad + q * sa, bd + q * sb, idesc, (k > t.k0 || q > 0) ? 1u : 0u);
+                        commit<CTAS>(empty + 8 * s);
+                    }
                     if (++s == stages) s = 0, ph ^= 1;
                 }
-                if (ok && lane == 0) commit<CTAS>(tfull + 8 * b);
+                if (ok && leader) commit<CTAS>(tfull + 8 * b);
             }
         }
     } else {

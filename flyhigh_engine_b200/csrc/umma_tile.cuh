@@ -65,6 +65,12 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, long lon
 // run warp-uniform on such values, which stay in uniform registers, and lane 0 alone issues (a loop of one lane took over
 // 1,000 cycles for four matrix instructions)
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
@@ -132,6 +138,11 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t block) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)((block >> 4) & 0x3FFF) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
+}
+// the same over a tile without swizzle: 8-row x 16-byte core matrices, the two halves of a K step 128 bytes apart, 8-row
+// groups 256 bytes apart
+__device__ __forceinline__ uint64_t plain_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(256 >> 4) << 32) | (1ull << 46);
 }
 // kind::f16, f32 accumulate; bf16 = operands are bfloat16; mn_* = the operand is MN-major; m: rows of the whole MMA
 __device__ __forceinline__ uint32_t instr_desc(bool bf16, bool mn_a, bool mn_b, uint32_t m, uint32_t n) {
