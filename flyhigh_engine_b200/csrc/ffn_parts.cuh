@@ -120,17 +120,27 @@ __device__ __forceinline__ void tile_put(uint32_t tile, int lane, int h, const f
                      "r"(Elem<T>::from2(v[4 * c + 3].x, v[4 * c + 3].y))
                      : "memory");
 }
-template <typename T>
-__device__ __forceinline__ void tile_get(uint32_t tile, int lane, int h, float2 (&v)[8]) {
+// 16 columns in f32 are a staging tile of the same size and swizzle
+__device__ __forceinline__ void tile_put32(uint32_t tile, int lane, const float2 (&v)[8]) {
 #pragma unroll
-    for (int c = 0; c < 2; c++) {
-        uint32_t q[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                     : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                     : "r"(tile_at(tile, lane, h, c))
+    for (int c = 0; c < 4; c++)
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(tile_at(tile, lane, 0, c)), "f"(v[2 * c].x), "f"(v[2 * c].y),
+                     "f"(v[2 * c + 1].x), "f"(v[2 * c + 1].y)
                      : "memory");
+}
+__device__ __forceinline__ void tile_get32(uint32_t tile, int lane, float2 (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[4 * c + i] = Elem<T>::to2(q[i]);
+    for (int c = 0; c < 4; c++)
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+                     : "=f"(v[2 * c].x), "=f"(v[2 * c].y), "=f"(v[2 * c + 1].x), "=f"(v[2 * c + 1].y)
+                     : "r"(tile_at(tile, lane, 0, c))
+                     : "memory");
+}
+__device__ __noinline__ void tile_out32(uint32_t tile, int lane, float* p, int valid) {
+    for (int i = 0; i < valid; i++) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(tile_at(tile, lane, 0, i >> 2) + 4 * (i & 3)) : "memory");
+        p[i] = v;
     }
 }
 // this lane's row of a staging tile, `valid` columns of it, to p: in place of a tensor copy, which writes whole 16-byte
@@ -213,13 +223,15 @@ struct Matrix {  // [rows][cols] of 16-bit elements
     int cols;
 };
 
-// boxes of 64 columns x `box` rows, 128-byte swizzled (operands), or of 32 x 32, 64-byte swizzled (box 0: the tails)
+// boxes of 64 columns x `box` rows, 128-byte swizzled (operands), or of 32 rows of 64 bytes, 64-byte swizzled (box 0: the tails;
+// f32 with dtype kF32)
+constexpr int kF32 = -1;
 cudaError_t map_of(CUtensorMap* map, const Matrix& x, int box, int dtype) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)x.cols, (cuuint64_t)x.rows}, strides[1] = {(cuuint64_t)x.pitch * 2};
-    const cuuint32_t boxes[2] = {box ? 64u : 32u, box ? (cuuint32_t)box : 32u}, one[2] = {1, 1};
-    const CUresult r = fn(map, dtype == FH_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+    const cuuint64_t dims[2] = {(cuuint64_t)x.cols, (cuuint64_t)x.rows}, strides[1] = {(cuuint64_t)x.pitch * (dtype == kF32 ? 4 : 2)};
+    const cuuint32_t boxes[2] = {box ? 64u : dtype == kF32 ? 16u : 32u, box ? (cuuint32_t)box : 32u}, one[2] = {1, 1};
+    const CUresult r = fn(map, dtype == kF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == FH_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                           const_cast<void*>(x.p), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           box ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;

@@ -67,11 +67,14 @@ struct Work {
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kStageA = 128 * 128;  // 128 rows of 64 elements
-constexpr int kRing = 163840;   // shared memory of the operand ring
 constexpr int kMaxStages = 8;
-constexpr int kTiles = 4;       // per warp: two groups of 64 columns in turn
+// shared memory: the operand ring, then each warp's staging tiles. Four of them are two groups of 64 columns in turn; the tails
+// that keep or read g and u in f32 take six.
+constexpr int kOperands = 229376;
+constexpr int tail_tiles(bool f32) { return f32 ? 6 : 4; }
+constexpr int ring_bytes(bool f32) { return kOperands - kEpiWarps * tail_tiles(f32) * kTile; }
 constexpr int kBars = 512;
-constexpr int kSmem = 1024 + kRing + kEpiWarps * kTiles * kTile + kBars;
+constexpr int kSmem = 1024 + kOperands + kBars;
 
 struct Item {
     const Job* j;
@@ -112,7 +115,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
     const int bn = w.bn, nb = bn / CTAS, stages = w.stages;
     const uint32_t stage_bytes = kStageA + nb * 128;
-    const uint32_t bars = base + kRing + kEpiWarps * kTiles * kTile;
+    const bool keep = TAIL == GLU && w.keep, f32 = keep || TAIL == GLU_GRAD;
+    const uint32_t staging = base + ring_bytes(f32), bars = base + kOperands;
     const uint32_t full = bars, empty = bars + 8 * kMaxStages, tfull = bars + 16 * kMaxStages, tempty = tfull + 16,
                    slot = tempty + 16;
     const uint32_t cols = 2 * bn;
@@ -224,15 +228,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         }
     } else {
         // the tails: this warp's 32 rows and half of the tile's columns (all of a 32-wide tile for the first half), in groups
-        // of 64 (32 where a group has two or three outputs) that pass through staging tiles of 32 x 32, which tensor
-        // copies store, clipped at the output's edges
-        const bool keep = TAIL == GLU && w.keep;
-        const int group = TAIL == GLU_GRAD || keep ? 32 : 64;
+        // of 64 (32 where g and u are kept or read) that pass through staging tiles of 32 x 32 (f32: 32 x 16), which tensor
+        // copies store, clipped at the output's edges. g and u are kept in f32: rounded to 16 bits they would put two more
+        // roundings of that size into every gradient behind them (1.8 against 1.4 times the error of one rounding).
+        const int group = f32 ? 32 : 64;
         const int q = warp & 3, half = warp >> 2;
         const int width = TAIL == GLU ? bn / 2 : bn, span = max(32, width / 2);
         const int lo = half * span, hi = min(width, lo + span);
-        const uint32_t tiles = base + kRing + warp * kTiles * kTile, gbar = bars + 256 + 16 * warp;
-        int n = 0, turn = 0;  // turn: the next tile (of four) of the ring that they form; GLU_GRAD, PLAIN: the next pair
+        const uint32_t tiles = staging + warp * tail_tiles(f32) * kTile, gbar = bars + 256 + 16 * warp;
+        int n = 0, turn = 0;  // turn: the pair of four tiles that is next
         uint32_t gph = 0;
         for (int i = first; i < w.items; i += step, n++) {
             const Item t = item_of(w, i);
@@ -243,37 +247,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
             const void *bias0 = part ? nullptr : j->bias0, *bias1 = j->bias1;
             const bool ragged = cols_ & 7, biased = bias0 || bias1;
             auto live = [&](int c0) { return row < m && c0 < hi && col + c0 < cols_; };
-            // GLU_GRAD: g and u of a group into the tiles of a pair, which dg and du then leave from
-            auto fetch = [&](int c0, int turn_) {
+            // GLU_GRAD: g and u of 16 columns into tiles 2 h and 2 h + 1; they are on their way a group ahead
+            auto fetch = [&](int c0, int h) {
                 if (!live(c0) || lane != 0) return;
-                const uint32_t bar = gbar + 8 * (turn_ & 1), dst = tiles + 2 * (turn_ & 1) * kTile;
+                const uint32_t bar = gbar + 8 * h, dst = tiles + 2 * h * kTile;
                 bar_expect(bar, 2 * kTile);
                 tensor_load<1>(dst, &w.x[1], col + c0, row, bar);
                 tensor_load<1>(dst + kTile, &w.x[2], col + c0, row, bar);
             };
             if (TAIL == GLU_GRAD) {
-                if (lane == 0) stores_read<1>();  // all but the last group's stores: the other two tiles
-                fetch(lo, turn);
+                fetch(lo, 0);
+                fetch(lo + 16, 1);
+                __syncwarp();
             }
             if (!wait(tfull + 8 * b, (n >> 1) & 1)) break;
             fence_after();
             const uint32_t acc = tbase + ((uint32_t)(q * 32) << 16) + b * bn;
             for (int c0 = lo; c0 < hi; c0 += group) {
                 const bool alive = live(c0);
-                // this group's tiles: a pair, or with kept outputs three of the four, one after another
-                uint32_t dst = tiles + 2 * (turn & 1) * kTile, dst1 = dst, dst2 = dst;
-                if (keep) dst = tiles + (turn & 3) * kTile, dst1 = tiles + ((turn + 1) & 3) * kTile, dst2 = tiles + ((turn + 2) & 3) * kTile;
-                if (TAIL == GLU_GRAD) {
-                    if (alive) {
-                        wait(gbar + 8 * (turn & 1), (gph >> (turn & 1)) & 1);
-                        gph ^= 1u << (turn & 1);
-                    }
-                    if (!ok) break;
-                } else {
-                    // what these tiles held has been read: all but the last group's stores (of kept outputs: the last store)
-                    if (lane == 0) stores_read<1>();
-                    __syncwarp();
+                // this group's tiles: a pair of 16-bit ones in turn; or a, g (2), u (2); or dg and du behind g's and u's four
+                const uint32_t dst = keep ? tiles : TAIL == GLU_GRAD ? tiles + 4 * kTile : tiles + 2 * (turn & 1) * kTile;
+                if (lane == 0) {  // what they held has been read
+                    if (f32) stores_read<0>();
+                    else stores_read<1>();
                 }
+                __syncwarp();
                 const int subs = min(group, hi - c0) / 32;
                 for (int sub = 0; sub < subs; sub++) {
                     const int cs = c0 + 32 * sub;
@@ -310,13 +308,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                             }
                             tile_put<T>(dst + sub * kTile, lane, h, v);
                             if (keep) {
-                                tile_put<T>(dst1, lane, h, g);
-                                tile_put<T>(dst2, lane, h, u);
+                                tile_put32(dst + (1 + h) * kTile, lane, g);
+                                tile_put32(dst + (3 + h) * kTile, lane, u);
                             }
                         } else if constexpr (TAIL == GLU_GRAD) {
                             pairs(r0 + 16 * h, v);
-                            tile_get<T>(dst, lane, h, g);
-                            tile_get<T>(dst + kTile, lane, h, u);
+                            if (live(cs + 16 * h)) {
+                                wait(gbar + 8 * h, (gph >> h) & 1);
+                                gph ^= 1u << h;
+                            }
+                            if (!ok) break;
+                            tile_get32(tiles + 2 * h * kTile, lane, g);
+                            tile_get32(tiles + (2 * h + 1) * kTile, lane, u);
+                            __syncwarp();
+                            fetch(cs + 32 + 16 * h, h);
+                            __syncwarp();
                             switch (w.act) {
                                 case FH_ACT_SILU: glu_grad16<FH_ACT_SILU>(v, g, u); break;
                                 case FH_ACT_GELU: glu_grad16<FH_ACT_GELU>(v, g, u); break;
@@ -326,11 +332,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                             }
                             tile_put<T>(dst, lane, h, g);
                             tile_put<T>(dst + kTile, lane, h, u);
-                            if (h == 0) {  // the next group's, into the tiles that the last group's stores have left by now
-                                if (lane == 0) stores_read<0>();
-                                fetch(c0 + 32, turn + 1);
-                                __syncwarp();
-                            }
                         } else {
                             pairs(r0 + 16 * h, v);
                             if (part) {
@@ -350,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                         }
                     }
                 }
+                if (!ok) break;
                 if (!alive || (TAIL == PLAIN && part)) continue;
                 fence_async();
                 __syncwarp();
@@ -359,31 +361,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                         const int valid = min(32, cols_ - col - c0 - 32 * sub);
                         if (row + lane >= m) continue;
                         tile_out<T>(dst + sub * kTile, lane, static_cast<T*>(j->out) + at, valid);
-                        if (keep) {
-                            tile_out<T>(dst1, lane, static_cast<T*>(w.out[0]) + at, valid);
-                            tile_out<T>(dst2, lane, static_cast<T*>(w.out[1]) + at, valid);
+                        for (int h = 0; keep && 16 * h < valid; h++) {
+                            tile_out32(dst + (1 + h) * kTile, lane, static_cast<float*>(w.out[0]) + at + 16 * h, min(16, valid - 16 * h));
+                            tile_out32(dst + (3 + h) * kTile, lane, static_cast<float*>(w.out[1]) + at + 16 * h, min(16, valid - 16 * h));
                         }
                         if (TAIL == GLU_GRAD) tile_out<T>(dst + kTile, lane, static_cast<T*>(w.out[0]) + at, valid);
                     }
                     fence_async();
                     __syncwarp();
-                    if (lane == 0) {  // groups of no stores: the count of those before stays right
-                        stores_commit();
-                        if (keep) stores_commit(), stores_commit();
-                    }
+                    if (lane == 0) stores_commit();  // a group of no stores: the count of those before stays right
                 } else if (lane == 0) {
                     for (int sub = 0; sub < subs && col + c0 + 32 * sub < cols_; sub++)
                         tensor_store(&j->o, col + c0 + 32 * sub, row, dst + sub * kTile);
-                    if (keep) {
-                        stores_commit();
-                        tensor_store(&w.x[0], col + c0, row, dst1);
-                        stores_commit();
-                        tensor_store(&w.x[1], col + c0, row, dst2);
+                    for (int h = 0; keep && h < 2 && col + c0 + 16 * h < cols_; h++) {
+                        tensor_store(&w.x[0], col + c0 + 16 * h, row, dst + (1 + h) * kTile);
+                        tensor_store(&w.x[1], col + c0 + 16 * h, row, dst + (3 + h) * kTile);
                     }
                     if (TAIL == GLU_GRAD) tensor_store(&w.x[0], col + c0, row, dst + kTile);
                     stores_commit();
                 }
-                turn += keep ? 3 : 1;
+                turn++;
             }
             if (!ok) break;
             // a half without columns of a narrow tile
@@ -422,7 +419,8 @@ struct RowsArgs {
     const T *x, *w0, *w1;  // [m][k], [n][k]
     long long x_pitch, w0_pitch, w1_pitch;
     const T *bias0, *bias1;
-    T *out, *g, *u;
+    T* out;
+    float *g, *u;
     long long pitch;
     int m, n, k, act, share;  // share: CTAs of a cluster
 };
@@ -587,8 +585,8 @@ __global__ void __launch_bounds__(256, 2) k_rows(const RowsArgs<T> p) {
             if (p.bias1) v[NW - 1] += Elem<T>::to(p.bias1[col]);
             p.out[at] = Elem<T>::from(act_by(p.act, v[0]) * v[NW - 1]);
             if (p.g) {
-                p.g[at] = Elem<T>::from(v[0]);
-                p.u[at] = Elem<T>::from(v[NW - 1]);
+                p.g[at] = v[0];
+                p.u[at] = v[NW - 1];
             }
         } else {
             p.out[at] = Elem<T>::from(v[0]);
@@ -802,7 +800,7 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
     Work w;
     w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.limit = limit > 0 ? limit : 2000000000ll;
     const int nb = s.bn / s.ctas;
-    w.stages = std::min(kMaxStages, kRing / (kStageA + nb * 128));
+    w.stages = std::min(kMaxStages, ring_bytes(TAIL == GLU_GRAD || (TAIL == GLU && p[0].out1)) / (kStageA + nb * 128));
     for (int i = 0; i < n; i++) {
         Job& j = w.job[i];
         const Product& q = p[i];
@@ -824,16 +822,18 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
         w.items = (int)items;
         j.out = q.out, j.pitch = q.pitch, j.bias0 = q.bias0, j.bias1 = q.bias1;
         w.out[0] = q.out1, w.out[1] = q.out2;
-        auto tail_map = [&](CUtensorMap* map, const void* x) { return map_of(map, {x, q.pitch, q.m, q.n}, 0, dtype); };
+        auto tail_map = [&](CUtensorMap* map, const void* x, bool f32 = false) {
+            return map_of(map, {x, q.pitch, q.m, q.n}, 0, f32 ? kF32 : dtype);
+        };
         if (TAIL == GLU && q.out1) {
             w.keep = 1;
-            FH_TRY(tail_map(&w.x[0], q.out1));
-            FH_TRY(tail_map(&w.x[1], q.out2));
+            FH_TRY(tail_map(&w.x[0], q.out1, true));
+            FH_TRY(tail_map(&w.x[1], q.out2, true));
         }
         if (TAIL == GLU_GRAD) {
             FH_TRY(tail_map(&w.x[0], q.out1));
-            FH_TRY(tail_map(&w.x[1], q.g));
-            FH_TRY(tail_map(&w.x[2], q.u));
+            FH_TRY(tail_map(&w.x[1], q.g, true));
+            FH_TRY(tail_map(&w.x[2], q.u, true));
         }
         j.part = nullptr;
         if (j.splits > 1) {
@@ -893,7 +893,7 @@ cudaError_t few_rows(const Product& q, int act, cudaStream_t st) {
     p.w0 = static_cast<const T*>(q.b[0].p), p.w0_pitch = q.b[0].pitch;
     if (GATED) p.w1 = static_cast<const T*>(q.b[1].p), p.w1_pitch = q.b[1].pitch;
     p.bias0 = static_cast<const T*>(q.bias0), p.bias1 = static_cast<const T*>(q.bias1);
-    p.out = static_cast<T*>(q.out), p.g = static_cast<T*>(q.out1), p.u = static_cast<T*>(q.out2), p.pitch = q.pitch;
+    p.out = static_cast<T*>(q.out), p.g = static_cast<float*>(q.out1), p.u = static_cast<float*>(q.out2), p.pitch = q.pitch;
     p.m = (int)q.m, p.n = q.n, p.k = (int)q.k, p.act = act, p.share = 1;
     // a cluster per 16 channels until there is a CTA for every SM, while each warp keeps two steps of K
     while (p.share < 8 && (p.n + 15) / 16 * p.share < kSms && (p.k + 31) / 32 >= 32 * p.share) p.share *= 2;

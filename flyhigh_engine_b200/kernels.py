@@ -256,22 +256,22 @@ _residual_norm_grad = _Call("residual_norm gradient", "fhk_residual_norm_grad", 
 
 
 class GatedFFNSaved:
-    """What a training forward call keeps for the gradient: the activated product a and the projections g and u."""
+    """What a training forward call keeps for the gradient: the activated product a, and the projections g and u in f32."""
 
-    def __init__(self, hidden, channels: int):
-        self.rows, self.channels = hidden, channels  # (3, rows, pitch): a, g, u
+    def __init__(self, a, gu, channels: int):
+        self._a, self._gu, self.channels = a, gu, channels  # (rows, pitch), (2, rows, pitch)
 
     @property
     def a(self):
-        return self.rows[0, :, :self.channels]
+        return self._a[:, :self.channels]
 
     @property
     def g(self):
-        return self.rows[1, :, :self.channels]
+        return self._gu[0, :, :self.channels]
 
     @property
     def u(self):
-        return self.rows[2, :, :self.channels]
+        return self._gu[1, :, :self.channels]
 
 
 class GatedFFN:
@@ -318,12 +318,14 @@ class GatedFFN:
         else:
             p.y, p.y_pitch = _like("out", out, m, self.cout, self.dtype, self.device)
         hp = p.h_pitch
-        hid = torch.empty((3 if keep else 1, m, hp), dtype=self.dtype, device=self.device)
-        p.a, p.m = hid.data_ptr(), m
+        a, saved = torch.empty((m, hp), dtype=self.dtype, device=self.device), None
+        p.a, p.m = a.data_ptr(), m
         if keep:
-            p.g, p.u = hid.data_ptr() + 2 * m * hp, hid.data_ptr() + 4 * m * hp
+            gu = torch.empty((2, m, hp), dtype=torch.float32, device=self.device)
+            p.g, p.u = gu.data_ptr(), gu.data_ptr() + 4 * m * hp
+            saved = GatedFFNSaved(a, gu, self.hidden)
         _gated_ffn(p, self.device, self._sizes, m)
-        return out, hid
+        return out, saved
 
     def __call__(self, x, out=None):
         """y for x (inference: nothing is kept)."""
@@ -331,8 +333,7 @@ class GatedFFN:
 
     def forward(self, x, out=None):
         """(y, saved): y, and what `backward` needs beside x."""
-        y, hid = self._forward(x, out, True)
-        return y, GatedFFNSaved(hid, self.hidden)
+        return self._forward(x, out, True)
 
     def backward(self, dy, x, saved: GatedFFNSaved, want=None) -> dict:
         """The gradients for dy of the call that returned `saved`: "x", "w_gate", "w_up", "w_down" and the biases' there
@@ -345,11 +346,10 @@ class GatedFFN:
         p = GatedFfnGradParams.from_buffer_copy(self._grad_params)
         p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
         p.dy, p.dy_pitch, mdy = _rows("dy", dy, self.cout, self.dtype, self.device)
-        hid = saved.rows
-        if mdy != m or hid.shape[1] != m or saved.channels != self.hidden or hid.dtype != self.dtype or hid.device != self.device:
-            raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({hid.shape[1]}) are not of one call")
-        at, step = hid.data_ptr(), 2 * m * p.h_pitch
-        p.a, p.g, p.u, p.m = at, at + step, at + 2 * step, m
+        a, at = saved._a, saved._gu.data_ptr()
+        if mdy != m or a.shape[0] != m or saved.channels != self.hidden or a.dtype != self.dtype or a.device != self.device:
+            raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({a.shape[0]}) are not of one call")
+        p.a, p.g, p.u, p.m = a.data_ptr(), at, at + 4 * m * p.h_pitch, m
         r = {}
         if "x" in names:
             r["x"] = _rows_like(x)

@@ -145,7 +145,7 @@ size_t fhk_gmhs_noalloc_max_floats(void);
 #define FH_ACT_SIGMOID 4   /* the plain gated linear unit */
 
 /* Gated feed-forward block: g = x w_gate^T + b_gate, u = x w_up^T + b_up, a = act(g) * u, y = a w_down^T + b_down.
- * a is rounded to the element type before the down projection; so are g and u where they are kept. */
+ * a is rounded to the element type before the down projection. */
 typedef struct FhGatedFfnParams {
     const void* x;         /* [m][cin] */
     const void* w_gate;    /* [hidden][cin] */
@@ -156,8 +156,8 @@ typedef struct FhGatedFfnParams {
     const void* b_down;    /* [cout] or NULL */
     void* y;               /* [m][cout] */
     void* a;               /* [m][hidden], pitch h_pitch: written, and read back by the down projection */
-    void* g;               /* [m][hidden], pitch h_pitch: kept for the gradient, or NULL (then u is NULL too) */
-    void* u;
+    float* g;              /* [m][hidden] f32, pitch h_pitch: kept for the gradient, or NULL (then u is NULL too) */
+    float* u;
     long long x_pitch, wg_pitch, wu_pitch, wd_pitch, y_pitch, h_pitch;
     long long m;           /* rows, 0 .. 2^31 - 256; 0 is a call that does nothing */
     int cin, hidden, cout; /* 1 .. 2^20 each */
@@ -176,7 +176,9 @@ size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p); /* of the sizes a
  * Each output may be NULL (not wanted). Every output is written, not added to. With m = 0 the weights' and biases'
  * gradients are set to zero. */
 typedef struct FhGatedFfnGradParams {
-    const void *x, *w_gate, *w_up, *w_down, *g, *u, *a; /* as in FhGatedFfnParams */
+    const void *x, *w_gate, *w_up, *w_down;             /* as in FhGatedFfnParams */
+    const float *g, *u;
+    const void* a;
     const void* dy;                                     /* [m][cout] */
     void* dx;                                           /* [m][cin] */
     void *dw_gate, *dw_up, *dw_down;                    /* the weights' shapes */
