@@ -188,14 +188,17 @@ __device__ __forceinline__ void glu16(const float2 (&g)[8], const float2 (&u)[8]
 #pragma unroll
     for (int i = 0; i < 8; i++) a[i] = mul2(act_of<ACT>(g[i]), u[i]);
 }
+// g and u become dg and du, a = act(g) u (a may be da)
 template <int ACT>
-__device__ __forceinline__ void glu_grad16(const float2 (&da)[8], float2 (&g)[8], float2 (&u)[8]) {
+__device__ __forceinline__ void glu_grad16(const float2 (&da)[8], float2 (&g)[8], float2 (&u)[8], float2 (&a)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         float2 v, dv;
         act_both<ACT>(g[i], v, dv);
         g[i] = mul2(mul2(da[i], u[i]), dv);
-        u[i] = mul2(da[i], v);
+        const float2 d = mul2(da[i], v);
+        a[i] = mul2(v, u[i]);
+        u[i] = d;
     }
 }
 

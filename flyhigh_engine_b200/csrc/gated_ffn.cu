@@ -24,7 +24,7 @@
 
 namespace {
 
-enum Tail { PLAIN, GLU, GLU_GRAD };
+enum Tail { PLAIN, GLU, GLU_GRAD, GLU_AGAIN };
 constexpr int kGroupM = 8;  // tiles of rows that are walked together, so that their operands stay in L2
 
 // n / d for n < 2^31 by a multiplication: with 2^s >= d > 2^(s - 1) and mul = ceil(2^(31 + s) / d), which is below 2^32, the
@@ -42,6 +42,8 @@ struct Divider {
 };
 
 // One product of a launch: out[m][n] = tail(sum over the terms of A[t] B[t]^T). GLU: A[0] with B[0] (gate) and B[1] (up).
+// GLU_AGAIN: A[0] = dy with B[0] = w_down, and A[1] = x with B[1] = gate and x[2] = up, beside each other: the gradient of
+// the activation with g and u formed again instead of read.
 struct alignas(64) Job {
     CUtensorMap a[2], b[2], o;     // o: out, in boxes of the tails
     int mn_a, mn_b;                // the operand is MN-major
@@ -58,7 +60,7 @@ struct alignas(64) Job {
 constexpr int kJobs = 4;
 struct Work {
     Job job[kJobs];
-    CUtensorMap x[3];  // GLU: where g and u are kept (keep); GLU_GRAD: du out, g and u in
+    CUtensorMap x[3];  // GLU: where g and u are kept (keep); GLU_GRAD: du out, g and u in; GLU_AGAIN: du and a out, w_up
     void* out[2];      // the same outputs
     int jobs, items, bn, stages, act, keep;
     long long limit;
@@ -69,10 +71,11 @@ constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kStageA = 128 * 128;  // 128 rows of 64 elements
 constexpr int kMaxStages = 8;
 // shared memory: the operand ring, then each warp's staging tiles. Four of them are two groups of 64 columns in turn; the tails
-// that keep or read g and u in f32 take six.
+// that keep or read g and u in f32, or leave dg, du and a, take six.
 constexpr int kOperands = 229376;
-constexpr int tail_tiles(bool f32) { return f32 ? 6 : 4; }
-constexpr int ring_bytes(bool f32) { return kOperands - kEpiWarps * tail_tiles(f32) * kTile; }
+constexpr int tail_tiles(bool six) { return six ? 6 : 4; }
+constexpr int ring_bytes(bool six) { return kOperands - kEpiWarps * tail_tiles(six) * kTile; }
+constexpr int kAgain = 64;  // GLU_AGAIN: hidden columns of a tile (da, g and u of 64 columns each)
 constexpr int kBars = 512;
 constexpr int kSmem = 1024 + kOperands + kBars;
 
@@ -113,13 +116,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
-    const int bn = w.bn, nb = bn / CTAS, stages = w.stages;
+    // bn: columns of an accumulator; nb: rows of B that this CTA holds
+    const int bn = w.bn, nb = TAIL == GLU_AGAIN ? 2 * kAgain : bn / CTAS, stages = w.stages;
     const uint32_t stage_bytes = kStageA + nb * 128;
-    const bool keep = TAIL == GLU && w.keep, f32 = keep || TAIL == GLU_GRAD;
-    const uint32_t staging = base + ring_bytes(f32), bars = base + kOperands;
+    const bool keep = TAIL == GLU && w.keep, f32 = keep || TAIL == GLU_GRAD, six = f32 || TAIL == GLU_AGAIN;
+    const uint32_t staging = base + ring_bytes(six), bars = base + kOperands;
     const uint32_t full = bars, empty = bars + 8 * kMaxStages, tfull = bars + 16 * kMaxStages, tempty = tfull + 16,
                    slot = tempty + 16;
-    const uint32_t cols = 2 * bn;
+    const uint32_t cols = TAIL == GLU_AGAIN ? 512 : 2 * bn;
 
     if (warp == 8 && lane == 0) {
         for (int s = 0; s < stages; s++) {
@@ -173,14 +177,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 const CUtensorMap* ma = &j.a[term];
                 const CUtensorMap* mb = &j.b[TAIL == GLU && CTAS == 2 ? rank : term];
                 if (leader) {
-                    if (rank == 0) bar_expect(full + 8 * s, CTAS * stage_bytes);
+                    if (rank == 0) bar_expect(full + 8 * s, CTAS * (TAIL == GLU_AGAIN && !term ? stage_bytes - kAgain * 128 : stage_bytes));
                     if (mn_a) {
                         tensor_load<CTAS>(da, ma, row, kk, bar);
                         tensor_load<CTAS>(da + 8192, ma, row + 64, kk, bar);
                     } else {
                         tensor_load<CTAS>(da, ma, kk, row, bar);
                     }
-                    if (TAIL == GLU) {
+                    if (TAIL == GLU_AGAIN) {
+                        const int c = t.tn * kAgain;
+                        tensor_load<CTAS>(db, mb, term ? kk : c, term ? c : kk, bar);
+                        if (term) tensor_load<CTAS>(db + kAgain * 128, &w.x[2], kk, c, bar);
+                    } else if (TAIL == GLU) {
                         const int c = t.tn * (bn / 2);
                         tensor_load<CTAS>(db, mb, kk, c, bar);
                         if (CTAS == 1) tensor_load<CTAS>(db + (bn / 2) * 128, &j.b[1], kk, c, bar);
@@ -216,7 +224,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                     fence_after();
                     const uint32_t da = base + s * stage_bytes;
                     const uint64_t ad = tile_desc(da, 8192), bd = tile_desc(da + kStageA, 8192);
-                    if (leader) {
+                    if (TAIL == GLU_AGAIN) {  // da (w_down is MN-major), then g and u side by side
+                        const bool again = k >= j.kb[0];
+                        const uint32_t id = instr_desc(!std::is_same<T, __half>::value, false, !again, 128, again ? 2 * kAgain : kAgain);
+                        const uint32_t to = again ? d + kAgain : d, step_b = again ? 32 >> 4 : 2048 >> 4;
+                        if (leader) {
+#pragma unroll
+                            for (int q = 0; q < 4; q++)
+                                mma<CTAS>(to, ad + q * (32 >> 4), bd + q * step_b, id, (k > (again ? j.kb[0] : 0) || q > 0) ? 1u : 0u);
+                            commit<CTAS>(empty + 8 * s);
+                        }
+                    } else if (leader) {
 #pragma unroll
                         for (int q = 0; q < 4; q++) mma<CTAS>(d, ad + q * sa, bd + q * sb, idesc, (k > t.k0 || q > 0) ? 1u : 0u);
                         commit<CTAS>(empty + 8 * s);
@@ -231,11 +249,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         // of 64 (32 where g and u are kept or read) that pass through staging tiles of 32 x 32 (f32: 32 x 16), which tensor
         // copies store, clipped at the output's edges. g and u are kept in f32: rounded to 16 bits they would put two more
         // roundings of that size into every gradient behind them (1.8 against 1.4 times the error of one rounding).
-        const int group = f32 ? 32 : 64;
+        const int group = six ? 32 : 64;
         const int q = warp & 3, half = warp >> 2;
-        const int width = TAIL == GLU ? bn / 2 : bn, span = max(32, width / 2);
+        const int width = TAIL == GLU ? bn / 2 : TAIL == GLU_AGAIN ? kAgain : bn, span = max(32, width / 2);
         const int lo = half * span, hi = min(width, lo + span);
-        const uint32_t tiles = staging + warp * tail_tiles(f32) * kTile, gbar = bars + 256 + 16 * warp;
+        const uint32_t tiles = staging + warp * tail_tiles(six) * kTile, gbar = bars + 256 + 16 * warp;
         int n = 0, turn = 0;  // turn: the pair of four tiles that is next
         uint32_t gph = 0;
         for (int i = first; i < w.items; i += step, n++) {
@@ -265,15 +283,56 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
             const uint32_t acc = tbase + ((uint32_t)(q * 32) << 16) + b * bn;
             for (int c0 = lo; c0 < hi; c0 += group) {
                 const bool alive = live(c0);
-                // this group's tiles: a pair of 16-bit ones in turn; or a, g (2), u (2); or dg and du behind g's and u's four
-                const uint32_t dst = keep ? tiles : TAIL == GLU_GRAD ? tiles + 4 * kTile : tiles + 2 * (turn & 1) * kTile;
+                // this group's tiles: a pair of 16-bit ones in turn (three: dg, du, a); or a, g (2), u (2); or dg and du behind
+                // g's and u's four
+                const uint32_t dst = keep ? tiles : TAIL == GLU_GRAD ? tiles + 4 * kTile : tiles + (TAIL == GLU_AGAIN ? 3 : 2) * (turn & 1) * kTile;
                 if (lane == 0) {  // what they held has been read
                     if (f32) stores_read<0>();
                     else stores_read<1>();
                 }
                 __syncwarp();
                 const int subs = min(group, hi - c0) / 32;
-                for (int sub = 0; sub < subs; sub++) {
+                if constexpr (TAIL == GLU_AGAIN) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int cs = c0 + 16 * h;
+                        uint32_t r0[16], r1[16], r2[16], q0[8], q1[8];
+                        load16(acc + cs, r0);
+                        load16(acc + kAgain + cs, r1);
+                        load16(acc + 2 * kAgain + cs, r2);
+                        if (biased) {
+                            load_bias<T>(bias0, col + cs, cols_, q0);
+                            load_bias<T>(bias1, col + cs, cols_, q1);
+                            __syncwarp();
+                        }
+                        wait_ld();
+                        if (h == 1) {
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) free_accumulators(tempty + 8 * b);
+                        }
+                        float2 v[8], g[8], u[8], a[8];
+                        pairs(r0, v);
+                        pairs(r1, g);
+                        pairs(r2, u);
+                        if (biased) {
+                            add_bias<T>(q0, g);
+                            add_bias<T>(q1, u);
+                        }
+                        switch (w.act) {
+                            case FH_ACT_SILU: glu_grad16<FH_ACT_SILU>(v, g, u, a); break;
+                            case FH_ACT_GELU: glu_grad16<FH_ACT_GELU>(v, g, u, a); break;
+                            case FH_ACT_GELU_TANH: glu_grad16<FH_ACT_GELU_TANH>(v, g, u, a); break;
+                            case FH_ACT_RELU: glu_grad16<FH_ACT_RELU>(v, g, u, a); break;
+                            default: glu_grad16<FH_ACT_SIGMOID>(v, g, u, a); break;
+                        }
+                        tile_put<T>(dst, lane, h, g);
+                        tile_put<T>(dst + kTile, lane, h, u);
+                        tile_put<T>(dst + 2 * kTile, lane, h, a);
+                        __syncwarp();
+                    }
+                }
+                for (int sub = 0; TAIL != GLU_AGAIN && sub < subs; sub++) {
                     const int cs = c0 + 32 * sub;
                     uint32_t r0[32], r1[TAIL == GLU ? 32 : 1], q0[16], q1[16];
                     load32(acc + cs, r0);
@@ -324,11 +383,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                             fetch(cs + 32 + 16 * h, h);
                             __syncwarp();
                             switch (w.act) {
-                                case FH_ACT_SILU: glu_grad16<FH_ACT_SILU>(v, g, u); break;
-                                case FH_ACT_GELU: glu_grad16<FH_ACT_GELU>(v, g, u); break;
-                                case FH_ACT_GELU_TANH: glu_grad16<FH_ACT_GELU_TANH>(v, g, u); break;
-                                case FH_ACT_RELU: glu_grad16<FH_ACT_RELU>(v, g, u); break;
-                                default: glu_grad16<FH_ACT_SIGMOID>(v, g, u); break;
+                                case FH_ACT_SILU: glu_grad16<FH_ACT_SILU>(v, g, u, v); break;
+                                case FH_ACT_GELU: glu_grad16<FH_ACT_GELU>(v, g, u, v); break;
+                                case FH_ACT_GELU_TANH: glu_grad16<FH_ACT_GELU_TANH>(v, g, u, v); break;
+                                case FH_ACT_RELU: glu_grad16<FH_ACT_RELU>(v, g, u, v); break;
+                                default: glu_grad16<FH_ACT_SIGMOID>(v, g, u, v); break;
                             }
                             tile_put<T>(dst, lane, h, g);
                             tile_put<T>(dst + kTile, lane, h, u);
@@ -365,7 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                             tile_out32(dst + (1 + h) * kTile, lane, static_cast<float*>(w.out[0]) + at + 16 * h, min(16, valid - 16 * h));
                             tile_out32(dst + (3 + h) * kTile, lane, static_cast<float*>(w.out[1]) + at + 16 * h, min(16, valid - 16 * h));
                         }
-                        if (TAIL == GLU_GRAD) tile_out<T>(dst + kTile, lane, static_cast<T*>(w.out[0]) + at, valid);
+                        if (TAIL == GLU_GRAD || TAIL == GLU_AGAIN) tile_out<T>(dst + kTile, lane, static_cast<T*>(w.out[0]) + at, valid);
+                        if (TAIL == GLU_AGAIN) tile_out<T>(dst + 2 * kTile, lane, static_cast<T*>(w.out[1]) + at, valid);
                     }
                     fence_async();
                     __syncwarp();
@@ -377,7 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                         tensor_store(&w.x[0], col + c0 + 16 * h, row, dst + (1 + h) * kTile);
                         tensor_store(&w.x[1], col + c0 + 16 * h, row, dst + (3 + h) * kTile);
                     }
-                    if (TAIL == GLU_GRAD) tensor_store(&w.x[0], col + c0, row, dst + kTile);
+                    if (TAIL == GLU_GRAD || TAIL == GLU_AGAIN) tensor_store(&w.x[0], col + c0, row, dst + kTile);
+                    if (TAIL == GLU_AGAIN) tensor_store(&w.x[1], col + c0, row, dst + 2 * kTile);
                     stores_commit();
                 }
                 turn++;
@@ -703,6 +764,7 @@ struct Product {
     void *out, *out1, *out2;
     long long pitch;
     const void *bias0, *bias1, *g, *u;
+    Matrix up;  // GLU_AGAIN
 };
 
 struct Shape {
@@ -716,6 +778,11 @@ struct Shape {
 // hide, and split sums are written, read and joined by another launch.
 template <int TAIL>
 Shape shape_of(const Product* p, int n) {
+    if (TAIL == GLU_AGAIN) {  // 128 x 64 by one CTA
+        Shape s{};
+        s.ctas = 1, s.bn = 3 * kAgain, s.splits[0] = 1;
+        return s;
+    }
     static const int kinds[4][2] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
     Shape best{};
     double best_t = 1e300;
@@ -799,19 +866,19 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
     const Shape s = shape_of<TAIL>(p, n);
     Work w;
     w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.limit = limit > 0 ? limit : 2000000000ll;
-    const int nb = s.bn / s.ctas;
-    w.stages = std::min(kMaxStages, ring_bytes(TAIL == GLU_GRAD || (TAIL == GLU && p[0].out1)) / (kStageA + nb * 128));
+    const int nb = TAIL == GLU_AGAIN ? 2 * kAgain : s.bn / s.ctas;
+    w.stages = std::min(kMaxStages, ring_bytes(TAIL == GLU_GRAD || TAIL == GLU_AGAIN || (TAIL == GLU && p[0].out1)) / (kStageA + nb * 128));
     for (int i = 0; i < n; i++) {
         Job& j = w.job[i];
         const Product& q = p[i];
         for (int t = 0; t < (TAIL == GLU ? 2 : q.terms); t++) {
             if (t == 0 || TAIL != GLU) FH_TRY(map_of(&j.a[t], q.a[t], q.mn_a ? 64 : 128, dtype));
-            FH_TRY(map_of(&j.b[t], q.b[t], q.mn_b ? 64 : TAIL == GLU ? s.bn / 2 : nb, dtype));
+            FH_TRY(map_of(&j.b[t], q.b[t], q.mn_b || TAIL == GLU_AGAIN ? 64 : TAIL == GLU ? s.bn / 2 : nb, dtype));
         }
         const int kb = (int)((q.k + 63) / 64);
-        j.mn_a = q.mn_a, j.mn_b = q.mn_b, j.kb[0] = kb, j.kb[1] = q.terms > 1 ? kb : 0, j.m = (int)q.m, j.n = q.n;
+        j.mn_a = q.mn_a, j.mn_b = q.mn_b, j.kb[0] = kb, j.kb[1] = TAIL == GLU_AGAIN ? (q.a[1].cols + 63) / 64 : q.terms > 1 ? kb : 0, j.m = (int)q.m, j.n = q.n;
         j.tiles_m = (int)((q.m + 128 * s.ctas - 1) / (128 * s.ctas));
-        const int cols = TAIL == GLU ? s.bn / 2 : s.bn;
+        const int cols = TAIL == GLU ? s.bn / 2 : TAIL == GLU_AGAIN ? kAgain : s.bn;
         j.tiles_n = (q.n + cols - 1) / cols;
         j.splits = s.splits[i];
         j.first = w.items;
@@ -830,6 +897,11 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
             FH_TRY(tail_map(&w.x[0], q.out1, true));
             FH_TRY(tail_map(&w.x[1], q.out2, true));
         }
+        if (TAIL == GLU_AGAIN) {
+            FH_TRY(tail_map(&w.x[0], q.out1));
+            FH_TRY(tail_map(&w.x[1], q.out2));
+            FH_TRY(map_of(&w.x[2], q.up, 64, dtype));
+        }
         if (TAIL == GLU_GRAD) {
             FH_TRY(tail_map(&w.x[0], q.out1));
             FH_TRY(tail_map(&w.x[1], q.g, true));
@@ -845,7 +917,9 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
             FH_TRY(tail_map(&j.o, q.out));
         }
     }
-    return s.ctas == 2 ? launch_work<T, 2, TAIL>(w, st) : launch_work<T, 1, TAIL>(w, st);
+    if constexpr (TAIL != GLU_AGAIN)
+        if (s.ctas == 2) return launch_work<T, 2, TAIL>(w, st);
+    return launch_work<T, 1, TAIL>(w, st);
 }
 template <typename T>
 cudaError_t finish(const Sums& sums, cudaStream_t st) {
@@ -915,18 +989,21 @@ bool good_weights(const P* p) {
 }
 
 
+// where the activated products go: the caller's a, else the scratch's first bytes
+size_t own_a_bytes(const FhGatedFfnParams& p) { return p.a ? 0 : ((size_t)p.m * p.h_pitch * 2 + 255) / 256 * 256; }
+void* a_of(const FhGatedFfnParams& p) { return p.a ? p.a : p.scratch; }
 Product glu_of(const FhGatedFfnParams& p) {
     Product q{};
     q.a[0] = {p.x, p.x_pitch, p.m, p.cin};
     q.b[0] = {p.w_gate, p.wg_pitch, p.hidden, p.cin};
     q.b[1] = {p.w_up, p.wu_pitch, p.hidden, p.cin};
     q.terms = 1, q.m = p.m, q.n = p.hidden, q.k = p.cin;
-    q.out = p.a, q.out1 = p.g, q.out2 = p.u, q.pitch = p.h_pitch, q.bias0 = p.b_gate, q.bias1 = p.b_up;
+    q.out = a_of(p), q.out1 = p.g, q.out2 = p.u, q.pitch = p.h_pitch, q.bias0 = p.b_gate, q.bias1 = p.b_up;
     return q;
 }
 Product down_of(const FhGatedFfnParams& p) {
     Product q{};
-    q.a[0] = {p.a, p.h_pitch, p.m, p.hidden};
+    q.a[0] = {a_of(p), p.h_pitch, p.m, p.hidden};
     q.b[0] = {p.w_down, p.wd_pitch, p.cout, p.hidden};
     q.terms = 1, q.m = p.m, q.n = p.cout, q.k = p.hidden, q.can_split = true;
     q.out = p.y, q.pitch = p.y_pitch, q.bias0 = p.b_down;
@@ -948,15 +1025,18 @@ cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {
     if (on_map(p)) return block_on_map<T>(p, st);
     FH_TRY((products<T, GLU>(&glu, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
     fhk::PdlScope pdl(true);  // what follows waits on a kernel of this file
-    FH_TRY((products<T, PLAIN>(&down, 1, p.act, p.dtype, p.wait_cycles, static_cast<float*>(p.scratch), &sums, st)));
+    FH_TRY((products<T, PLAIN>(&down, 1, p.act, p.dtype, p.wait_cycles,
+                                reinterpret_cast<float*>(static_cast<char*>(p.scratch) + own_a_bytes(p)), &sums, st)));
     return finish<T>(sums, st);
 }
 
-// the gradient's scratch: dg and du [m][h_pitch], then the split sums and the partial column sums
+// the gradient's scratch: dg and du (and a, where it is formed again) [m][h_pitch], then the split sums and the partial
+// column sums
 struct GradPlan {
     Product da, out[kJobs];
     int outs;
-    size_t hidden_bytes, part_bytes, column_bytes;
+    bool again;
+    size_t hidden_bytes, all_hidden_bytes, part_bytes, column_bytes;
     ColumnSums cols;
     void* db[3];
     int ncols, widest;
@@ -966,11 +1046,22 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
     g.hidden_bytes = ((size_t)p.m * p.h_pitch * 2 + 255) / 256 * 256;
     char* dg = static_cast<char*>(p.scratch);
     char* du = dg + g.hidden_bytes;
+    g.again = !p.g;
+    g.all_hidden_bytes = (g.again ? 3 : 2) * g.hidden_bytes;
+    const void* a = g.again ? du + g.hidden_bytes : p.a;
     g.da.a[0] = {p.dy, p.dy_pitch, p.m, p.cout};
     g.da.b[0] = {p.w_down, p.wd_pitch, p.cout, p.hidden};
     g.da.mn_b = true;
     g.da.terms = 1, g.da.m = p.m, g.da.n = p.hidden, g.da.k = p.cout;
     g.da.out = dg, g.da.out1 = du, g.da.pitch = p.h_pitch, g.da.g = p.g, g.da.u = p.u;
+    if (g.again) {
+        g.da.terms = 2;
+        g.da.a[1] = {p.x, p.x_pitch, p.m, p.cin};
+        g.da.b[1] = {p.w_gate, p.wg_pitch, p.hidden, p.cin};
+        g.da.up = {p.w_up, p.wu_pitch, p.hidden, p.cin};
+        g.da.out2 = const_cast<void*>(a);
+        g.da.bias0 = p.b_gate, g.da.bias1 = p.b_up;
+    }
     if (p.dx) {
         Product& q = g.out[g.outs++];
         q.a[0] = {dg, p.h_pitch, p.m, p.hidden};
@@ -989,7 +1080,7 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
     const Matrix x = {p.x, p.x_pitch, p.m, p.cin};
     weight({dg, p.h_pitch, p.m, p.hidden}, x, p.dw_gate, p.dwg_pitch);
     weight({du, p.h_pitch, p.m, p.hidden}, x, p.dw_up, p.dwu_pitch);
-    weight({p.dy, p.dy_pitch, p.m, p.cout}, {p.a, p.h_pitch, p.m, p.hidden}, p.dw_down, p.dwd_pitch);
+    weight({p.dy, p.dy_pitch, p.m, p.cout}, {a, p.h_pitch, p.m, p.hidden}, p.dw_down, p.dwd_pitch);
     g.part_bytes = (g.outs ? scratch_floats<PLAIN>(g.out, g.outs) * 4 + 255 : 0) / 256 * 256;
     auto column = [&](const void* x_, long long pitch, int n, void* out) {
         if (!out) return;
@@ -1005,7 +1096,7 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
         const long long across = (long long)((g.widest + 63) / 64) * g.ncols;
         g.cols.slices = (int)std::max<long long>(1, std::min<long long>((p.m + 63) / 64, 4 * kSms / across));
         g.cols.m = p.m;
-        float* at = reinterpret_cast<float*>(dg + 2 * g.hidden_bytes + g.part_bytes);
+        float* at = reinterpret_cast<float*>(dg + g.all_hidden_bytes + g.part_bytes);
         for (int i = 0; i < g.ncols; i++) {
             g.cols.c[i].part = at + g.column_bytes / 4;
             g.column_bytes += (size_t)g.cols.slices * ((g.cols.c[i].n + 7) & ~7) * 4;
@@ -1017,14 +1108,16 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
 template <typename T>
 cudaError_t gradient(const FhGatedFfnGradParams& p, cudaStream_t st) {
     const GradPlan g = grad_plan(p);
-    const bool hidden = p.dx || p.dw_gate || p.dw_up || p.db_gate || p.db_up;  // whether dg or du is read
+    // whether dg or du is read (or a, formed with them)
+    const bool hidden = p.dx || p.dw_gate || p.dw_up || p.db_gate || p.db_up || (g.again && p.dw_down);
     Sums sums{};
-    if (hidden) FH_TRY((products<T, GLU_GRAD>(&g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    if (hidden && g.again) FH_TRY((products<T, GLU_AGAIN>(&g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    if (hidden && !g.again) FH_TRY((products<T, GLU_GRAD>(&g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
     bool mine = hidden;  // whether the stream's last kernel is one of this file's, which the next may wait for itself
     if (g.outs) {
         fhk::PdlScope pdl(mine);
         FH_TRY((products<T, PLAIN>(g.out, g.outs, p.act, p.dtype, p.wait_cycles,
-                                   reinterpret_cast<float*>(static_cast<char*>(p.scratch) + 2 * g.hidden_bytes), &sums, st)));
+                                   reinterpret_cast<float*>(static_cast<char*>(p.scratch) + g.all_hidden_bytes), &sums, st)));
         mine = true;
     }
     if (g.ncols) {
@@ -1044,16 +1137,19 @@ cudaError_t gradient(const FhGatedFfnGradParams& p, cudaStream_t st) {
 }  // namespace
 
 extern "C" size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p) {
-    if (!p || !good_sizes(p) || p->m == 0 || takes_few_rows(p->m, p->cin, p->hidden, p->cout) || on_map(*p)) return 0;
+    if (!p || !good_sizes(p) || p->m == 0 || p->h_pitch <= 0) return 0;
+    if (takes_few_rows(p->m, p->cin, p->hidden, p->cout)) return own_a_bytes(*p);
+    if (on_map(*p)) return 0;
     const Product down = down_of(*p);
-    return scratch_floats<PLAIN>(&down, 1) * 4;
+    return own_a_bytes(*p) + scratch_floats<PLAIN>(&down, 1) * 4;
 }
 
 extern "C" int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream) {
     if (!p || !good_sizes(p) || !good_weights(p)) return (int)cudaErrorInvalidValue;
     if (!aligned16(p->b_gate) || !aligned16(p->b_up) || !aligned16(p->b_down)) return (int)cudaErrorInvalidValue;
     if (!good_rows(p->x, p->x_pitch, p->cin, p->m) || !good_rows(p->y, p->y_pitch, p->cout, p->m) ||
-        !good_rows(p->a, p->h_pitch, p->hidden, p->m) || (p->g != nullptr) != (p->u != nullptr) ||
+        !good_rows_or_null(p->a, p->h_pitch, p->hidden, p->m) || (p->g != nullptr) != (p->u != nullptr) || (p->g && !p->a) ||
+        p->h_pitch < p->hidden || (p->h_pitch & 7) || p->h_pitch >= (1ll << 36) ||
         !good_rows_or_null(p->g, p->h_pitch, p->hidden, p->m) || !good_rows_or_null(p->u, p->h_pitch, p->hidden, p->m))
         return (int)cudaErrorInvalidValue;
     const size_t need = fhk_gated_ffn_scratch_bytes(p);
@@ -1066,19 +1162,22 @@ extern "C" int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream) {
 extern "C" size_t fhk_gated_ffn_grad_scratch_bytes(const FhGatedFfnGradParams* p) {
     if (!p || !good_sizes(p) || p->m == 0 || p->h_pitch <= 0) return 0;
     const GradPlan g = grad_plan(*p);
-    return 2 * g.hidden_bytes + g.part_bytes + g.column_bytes;
+    return g.all_hidden_bytes + g.part_bytes + g.column_bytes;
 }
 
 extern "C" int fhk_gated_ffn_grad(const FhGatedFfnGradParams* p, void* stream) {
     if (!p || !good_sizes(p) || !good_weights(p)) return (int)cudaErrorInvalidValue;
     if (!good_rows(p->x, p->x_pitch, p->cin, p->m) || !good_rows(p->dy, p->dy_pitch, p->cout, p->m) ||
-        !good_rows(p->g, p->h_pitch, p->hidden, p->m) || !good_rows(p->u, p->h_pitch, p->hidden, p->m) ||
-        !good_rows(p->a, p->h_pitch, p->hidden, p->m) || !good_rows_or_null(p->dx, p->dx_pitch, p->cin, p->m) ||
+        !good_rows_or_null(p->g, p->h_pitch, p->hidden, p->m) || !good_rows_or_null(p->u, p->h_pitch, p->hidden, p->m) ||
+        !good_rows_or_null(p->a, p->h_pitch, p->hidden, p->m) || (p->g != nullptr) != (p->u != nullptr) ||
+        (p->g != nullptr) != (p->a != nullptr) || p->h_pitch < p->hidden || (p->h_pitch & 7) || p->h_pitch >= (1ll << 36) ||
+        !good_rows_or_null(p->dx, p->dx_pitch, p->cin, p->m) ||
         !good_rows_or_null(p->dw_gate, p->dwg_pitch, p->cin, p->hidden) ||
         !good_rows_or_null(p->dw_up, p->dwu_pitch, p->cin, p->hidden) ||
         !good_rows_or_null(p->dw_down, p->dwd_pitch, p->hidden, p->cout))
         return (int)cudaErrorInvalidValue;
-    if (!aligned16(p->db_gate) || !aligned16(p->db_up) || !aligned16(p->db_down)) return (int)cudaErrorInvalidValue;
+    if (!aligned16(p->db_gate) || !aligned16(p->db_up) || !aligned16(p->db_down) || !aligned16(p->b_gate) || !aligned16(p->b_up))
+        return (int)cudaErrorInvalidValue;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p->m == 0) {  // no rows: the gradients of what all rows share are zero
         auto zero = [&](void* v, long long pitch, int c, int n) {

@@ -116,7 +116,7 @@ class GatedFfnParams(Structure):  # FhGatedFfnParams
 
 
 class GatedFfnGradParams(Structure):  # FhGatedFfnGradParams
-    _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "g", "u", "a", "dy", "dx", "dw_gate", "dw_up",
+    _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "g", "u", "a", "dy", "dx", "dw_gate", "dw_up",
                                         "dw_down", "db_gate", "db_up", "db_down")] + \
         [(n, c_longlong) for n in ("x_pitch", "wg_pitch", "wu_pitch", "wd_pitch", "h_pitch", "dy_pitch", "dx_pitch",
                                    "dwg_pitch", "dwu_pitch", "dwd_pitch", "m")] + \
@@ -152,14 +152,11 @@ def _rows_like(t):
     """empty_rows of t's shape, type and device; t is a tensor of rows."""
     import torch
     c = t.shape[-1]
-    return torch.empty_like(t) if c % 8 == 0 else empty_rows(t.shape, t.dtype, t.device)
-
-
-def _vectors(sizes, dtype, device):
-    """New vectors, each beginning on a 16-byte boundary (of one allocation)."""
-    import torch
-    up = [_up8(n) for n in sizes]
-    return [t if n == k else t[:n] for t, n, k in zip(torch.empty(sum(up), dtype=dtype, device=device).split(up), sizes, up)]
+    if c % 8 == 0:
+        return torch.empty_like(t)
+    if t.dim() == 2:
+        return torch.empty_strided(t.shape, (_up8(c), 1), dtype=t.dtype, device=t.device)
+    return empty_rows(t.shape, t.dtype, t.device)
 
 
 def _dtype_code(dtype) -> int:
@@ -256,22 +253,23 @@ _residual_norm_grad = _Call("residual_norm gradient", "fhk_residual_norm_grad", 
 
 
 class GatedFFNSaved:
-    """What a training forward call keeps for the gradient: the activated product a, and the projections g and u in f32."""
+    """What a training forward call keeps for the gradient: the activated product a, and the projections g and u in f32;
+    nothing (None) where the gradient forms them again."""
 
-    def __init__(self, a, gu, channels: int):
-        self._a, self._gu, self.channels = a, gu, channels  # (rows, pitch), (2, rows, pitch)
+    def __init__(self, rows: int, channels: int, a=None, gu=None):
+        self.rows, self.channels, self._a, self._gu = rows, channels, a, gu  # (rows, pitch), (2, rows, pitch)
 
     @property
     def a(self):
-        return self._a[:, :self.channels]
+        return None if self._a is None else self._a[:, :self.channels]
 
     @property
     def g(self):
-        return self._gu[0, :, :self.channels]
+        return None if self._gu is None else self._gu[0, :, :self.channels]
 
     @property
     def u(self):
-        return self._gu[1, :, :self.channels]
+        return None if self._gu is None else self._gu[1, :, :self.channels]
 
 
 class GatedFFN:
@@ -281,9 +279,11 @@ class GatedFFN:
     w_gate, w_up: [hidden][cin], w_down: [cout][hidden], biases [hidden], [hidden], [cout] or None: CUDA tensors of one
     type (float16 or bfloat16), used where they lie (no copy: an optimiser may update them in place). act: silu, gelu
     (erf), gelu_tanh, relu or sigmoid. x: (..., cin); every tensor's rows begin on 16-byte boundaries (empty_rows).
+    keep: whether a training forward call keeps the hidden values for its gradient (10 bytes each), or the gradient forms
+    them again; None: the faster, which is to form them again up to 128 channels in and out.
     No autograd: forward / backward are called by the training step."""
 
-    def __init__(self, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu"):
+    def __init__(self, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", keep: Optional[bool] = None):
         if act not in ACTIVATIONS:
             raise FlyHighError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
         if w_gate.dim() != 2 or w_down.dim() != 2 or not w_gate.is_cuda:
@@ -305,8 +305,9 @@ class GatedFFN:
                       hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[act], dtype=code, h_pitch=_up8(self.hidden))
         # the calls' parameter blocks with all that does not change from call to call
         self._forward_params = GatedFfnParams(**common, b_gate=bias[0], b_up=bias[1], b_down=bias[2])
-        self._grad_params = GatedFfnGradParams(**common)
+        self._grad_params = GatedFfnGradParams(**common, b_gate=bias[0], b_up=bias[1])
         self._sizes, self._grad_sizes = {}, {}
+        self.keep = max(self.cin, self.cout) > 128 if keep is None else bool(keep)
 
     def _forward(self, x, out, keep: bool):
         import torch
@@ -317,15 +318,16 @@ class GatedFFN:
             p.y, p.y_pitch = out.data_ptr(), _up8(self.cout)
         else:
             p.y, p.y_pitch = _like("out", out, m, self.cout, self.dtype, self.device)
+        p.m = m
+        if not keep:
+            _gated_ffn(p, self.device, self._sizes, m)
+            return out, m
         hp = p.h_pitch
-        a, saved = torch.empty((m, hp), dtype=self.dtype, device=self.device), None
-        p.a, p.m = a.data_ptr(), m
-        if keep:
-            gu = torch.empty((2, m, hp), dtype=torch.float32, device=self.device)
-            p.g, p.u = gu.data_ptr(), gu.data_ptr() + 4 * m * hp
-            saved = GatedFFNSaved(a, gu, self.hidden)
-        _gated_ffn(p, self.device, self._sizes, m)
-        return out, saved
+        a = torch.empty((m, hp), dtype=self.dtype, device=self.device)
+        gu = torch.empty((2, m, hp), dtype=torch.float32, device=self.device)
+        p.a, p.g, p.u = a.data_ptr(), gu.data_ptr(), gu.data_ptr() + 4 * m * hp
+        _gated_ffn(p, self.device, self._sizes, (m, True))
+        return out, GatedFFNSaved(m, self.hidden, a, gu)
 
     def __call__(self, x, out=None):
         """y for x (inference: nothing is kept)."""
@@ -333,11 +335,13 @@ class GatedFFN:
 
     def forward(self, x, out=None):
         """(y, saved): y, and what `backward` needs beside x."""
-        return self._forward(x, out, True)
+        y, saved = self._forward(x, out, self.keep)
+        return y, saved if self.keep else GatedFFNSaved(saved, self.hidden)
 
     def backward(self, dy, x, saved: GatedFFNSaved, want=None) -> dict:
         """The gradients for dy of the call that returned `saved`: "x", "w_gate", "w_up", "w_down" and the biases' there
         are, or those of them that `want` lists. They are new tensors, each written whole."""
+        import torch
         names = ["x", "w_gate", "w_up", "w_down"] + [n for n, b in zip(("b_gate", "b_up", "b_down"), self.biases) if b is not None]
         if want is not None:
             if not set(want) <= set(names):
@@ -346,10 +350,14 @@ class GatedFFN:
         p = GatedFfnGradParams.from_buffer_copy(self._grad_params)
         p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
         p.dy, p.dy_pitch, mdy = _rows("dy", dy, self.cout, self.dtype, self.device)
-        a, at = saved._a, saved._gu.data_ptr()
-        if mdy != m or a.shape[0] != m or saved.channels != self.hidden or a.dtype != self.dtype or a.device != self.device:
-            raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({a.shape[0]}) are not of one call")
-        p.a, p.g, p.u, p.m = a.data_ptr(), at, at + 4 * m * p.h_pitch, m
+        a = saved._a
+        if mdy != m or saved.rows != m or saved.channels != self.hidden or \
+                (a is not None and (a.dtype != self.dtype or a.device != self.device)):
+            raise FlyHighError(f"x ({m} rows), dy ({mdy}) and saved ({saved.rows}) are not of one call")
+        p.m = m
+        if a is not None:
+            at = saved._gu.data_ptr()
+            p.a, p.g, p.u = a.data_ptr(), at, at + 4 * m * p.h_pitch
         r = {}
         if "x" in names:
             r["x"] = _rows_like(x)
@@ -365,11 +373,11 @@ class GatedFFN:
             p.dw_down, p.dwd_pitch = r["w_down"].data_ptr(), _up8(self.hidden)
         biases = [n for n in names if n[0] == "b"]
         if biases:
-            sizes = [self.cout if n == "b_down" else self.hidden for n in biases]
-            for n, t in zip(biases, _vectors(sizes, self.dtype, self.device)):
-                r[n] = t
-                setattr(p, "d" + n, t.data_ptr())
-        _gated_ffn_grad(p, self.device, self._grad_sizes, (m, *names))
+            for n, b in zip(("b_gate", "b_up", "b_down"), self.biases):
+                if n in biases:
+                    r[n] = torch.empty_like(b)
+                    setattr(p, "d" + n, r[n].data_ptr())
+        _gated_ffn_grad(p, self.device, self._grad_sizes, (m, a is None, *names))
         return r
 
 
@@ -455,6 +463,7 @@ class ResidualNorm:
     def backward(self, dy, dh, y, f=None, gate=None) -> dict:
         """The gradients for dy and dh (either may be None: zero) of the call that returned y: "x", and with f "f",
         "gate" where there is one, and those of the vectors there are. They are new tensors, each written whole."""
+        import torch
         first = dy if dy is not None else dh
         if first is None or (dh is not None and self.pre == "none"):
             raise FlyHighError("dy or dh is needed, and dh only with a norm before the next block")
@@ -482,9 +491,8 @@ class ResidualNorm:
                 raise FlyHighError("without f there is no gate")
             p.post, p.scale, p.w_post, p.b_post = 0, None, None, None
         names = self._names if f is not None else [n for n in self._names if n in ("w_pre", "b_pre")]
-        if names:
-            for n, t in zip(names, _vectors([c] * len(names), dt, dev)):
-                r[n] = t
-                setattr(p, "d" + n, t.data_ptr())
+        for n in names:
+            r[n] = torch.empty_like(self.params[n])
+            setattr(p, "d" + n, r[n].data_ptr())
         _residual_norm_grad(p, dev, self._sizes, (m, p.gates))
         return r

@@ -155,7 +155,7 @@ typedef struct FhGatedFfnParams {
     const void* b_up;      /* [hidden] or NULL */
     const void* b_down;    /* [cout] or NULL */
     void* y;               /* [m][cout] */
-    void* a;               /* [m][hidden], pitch h_pitch: written, and read back by the down projection */
+    void* a;               /* [m][hidden], pitch h_pitch: kept for the gradient (with g and u), or NULL: the scratch's */
     float* g;              /* [m][hidden] f32, pitch h_pitch: kept for the gradient, or NULL (then u is NULL too) */
     float* u;
     long long x_pitch, wg_pitch, wu_pitch, wd_pitch, y_pitch, h_pitch;
@@ -168,15 +168,20 @@ typedef struct FhGatedFfnParams {
     long long wait_cycles; /* bound of each wait inside the kernels, SM clock cycles; 0 = 2e9 (about a second) */
 } FhGatedFfnParams;
 int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream);
-size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p); /* of the sizes alone; pointers are not looked at */
+/* Of the sizes, and of whether a and g are NULL. Up to 128 channels in and out the hidden values of a call that keeps nothing
+ * stay on the SMs, and no scratch is needed. */
+size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p);
 
-/* The block's gradient for dy, from x, the weights and what the forward call kept (g, u, a).
+/* The block's gradient for dy, from x, the weights and what the forward call kept (g, u, a), or with all three NULL from x,
+ * the weights and the biases alone: g, u and a are formed again (with few channels this costs less than to keep and read
+ * them; it always costs less memory).
  * da = dy w_down; dg = da * u * act'(g), du = da * act(g), both rounded to the element type;
  * dx = dg w_gate + du w_up; dw_gate = dg^T x; dw_up = du^T x; dw_down = dy^T a; db_* the column sums of dg, du, dy.
  * Each output may be NULL (not wanted). Every output is written, not added to. With m = 0 the weights' and biases'
  * gradients are set to zero. */
 typedef struct FhGatedFfnGradParams {
     const void *x, *w_gate, *w_up, *w_down;             /* as in FhGatedFfnParams */
+    const void *b_gate, *b_up;                          /* read only where g is NULL */
     const float *g, *u;
     const void* a;
     const void* dy;                                     /* [m][cout] */

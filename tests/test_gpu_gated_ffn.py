@@ -28,16 +28,18 @@ def block(m, c, f, o, dtype, bias=True, seed=0):
 
 
 def check(m, c, f, o, dtype, act="silu", bias=True, seed=0, train=True):
+    """Inference, and training with the hidden values kept and formed again."""
     x, w, b, dy = block(m, c, f, o, dtype, bias, seed)
-    layer = GatedFFN(*w, *b, act=act)
     want = ffn(x, *w, *b, act=act, dy=dy if train else None)
-    assert_within("y", layer(x), *want["y"])
-    if train:
+    assert_within("y", GatedFFN(*w, *b, act=act)(x), *want["y"])
+    for keep in (True, False) if train else ():
+        layer = GatedFFN(*w, *b, act=act, keep=keep)
         y, saved = layer.forward(x)
+        assert (saved.g is not None) == keep
         got = {"y": y, **layer.backward(dy, x, saved)}
         assert set(got) == set(want)
         for k in want:
-            assert_within(k, got[k], *want[k])
+            assert_within(f"{k} (keep {keep})", got[k], *want[k])
     assert fh.lib().fhk_gated_ffn_wait_timeouts(0) == 0
 
 
