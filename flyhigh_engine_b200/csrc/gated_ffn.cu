@@ -56,6 +56,8 @@ struct alignas(64) Job {
     long long pitch;
     const void *bias0, *bias1;  // by column, or NULL
     float* part;                // splits > 1: [split][m][n8] sums in place of out
+    void* sums;                 // [m] the rows' sums of A (a bias's gradient), or NULL
+    float* sums_part;           // splits > 1: [split][m8] in its place
 };
 constexpr int kJobs = 4;
 struct Work {
@@ -63,6 +65,7 @@ struct Work {
     CUtensorMap x[3];  // GLU: where g and u are kept (keep); GLU_GRAD: du out, g and u in; GLU_AGAIN: du and a out, w_up
     void* out[2];      // the same outputs
     int jobs, items, bn, stages, act, keep;
+    int sums;  // some job's rows are summed: A times a tile of ones, one matrix instruction of 16 columns beside each
     long long limit;
 };
 
@@ -76,6 +79,7 @@ constexpr int kOperands = 229376;
 constexpr int tail_tiles(bool six) { return six ? 6 : 4; }
 constexpr int ring_bytes(bool six) { return kOperands - kEpiWarps * tail_tiles(six) * kTile; }
 constexpr int kAgain = 64;  // GLU_AGAIN: hidden columns of a tile (da, g and u of 64 columns each)
+constexpr int kOnes = 2048;  // of the ring: 16 rows of ones
 constexpr int kBars = 512;
 constexpr int kSmem = 1024 + kOperands + kBars;
 
@@ -123,7 +127,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
     const uint32_t staging = base + ring_bytes(six), bars = base + kOperands;
     const uint32_t full = bars, empty = bars + 8 * kMaxStages, tfull = bars + 16 * kMaxStages, tempty = tfull + 16,
                    slot = tempty + 16;
-    const uint32_t cols = TAIL == GLU_AGAIN ? 512 : 2 * bn;
+    const uint32_t ones = base + ring_bytes(six) - kOnes;
+    const uint32_t cols = TAIL == GLU_AGAIN ? 512 : TAIL == PLAIN && w.sums ? 4 * bn : 2 * bn;  // sums: 32 beside each 2 bn
 
     if (warp == 8 && lane == 0) {
         for (int s = 0; s < stages; s++) {
@@ -136,6 +141,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
         }
         for (int q = 0; q < 2 * kEpiWarps; q++) bar_init(bars + 256 + 8 * q, 1);
         bar_init_fence();
+    }
+    if (TAIL == PLAIN && w.sums && warp < 4) {  // whatever the order of a tile of ones
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(ones + 16 * threadIdx.x),
+                     "r"(std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u)
+                     : "memory");
+        fence_async();
     }
     if (warp == 9) tmem_alloc<CTAS>(slot, cols);
     fence_before();
@@ -217,6 +228,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 const uint32_t idesc = instr_desc(!std::is_same<T, __half>::value, j.mn_a, j.mn_b, 128 * CTAS, bn);
                 // one K step of 16: 32 bytes along a K-major tile's rows, two 8-k groups of an MN-major one
                 const uint32_t sa = j.mn_a ? 2048 >> 4 : 32 >> 4, sb = j.mn_b ? 2048 >> 4 : 32 >> 4;
+                const bool sums = TAIL == PLAIN && j.sums && t.tn == 0;
+                const uint32_t idsum = instr_desc(!std::is_same<T, __half>::value, j.mn_a, false, 128 * CTAS, 16 * CTAS);
                 if (!wait(tempty + 8 * b, ((n >> 1) & 1) ^ 1)) break;
                 fence_after();
                 for (int k = t.k0; k < t.k1; k++) {
@@ -237,6 +250,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                     } else if (leader) {
 #pragma unroll
                         for (int q = 0; q < 4; q++) mma<CTAS>(d, ad + q * sa, bd + q * sb, idesc, (k > t.k0 || q > 0) ? 1u : 0u);
+                        if (sums)
+#pragma unroll
+                            for (int q = 0; q < 4; q++)
+                                mma<CTAS>(tbase + 2 * bn + 32 * b, ad + q * sa, tile_desc(ones, 0), idsum, (k > t.k0 || q > 0) ? 1u : 0u);
                         commit<CTAS>(empty + 8 * s);
                     }
                     if (++s == stages) s = 0, ph ^= 1;
@@ -281,6 +298,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
             if (!wait(tfull + 8 * b, (n >> 1) & 1)) break;
             fence_after();
             const uint32_t acc = tbase + ((uint32_t)(q * 32) << 16) + b * bn;
+            if (TAIL == PLAIN && j->sums && t.tn == 0 && half == 0) {
+                uint32_t v;
+                load1(tbase + ((uint32_t)(q * 32) << 16) + 2 * bn + 32 * b, v);
+                wait_ld();
+                if (row + lane < m) {
+                    if (part) j->sums_part[(long long)t.split * ((m + 7) & ~7) + row + lane] = __uint_as_float(v);
+                    else static_cast<T*>(j->sums)[row + lane] = Elem<T>::from(__uint_as_float(v));
+                }
+                __syncwarp();
+            }
             for (int c0 = lo; c0 < hi; c0 += group) {
                 const bool alive = live(c0);
                 // this group's tiles: a pair of 16-bit ones in turn (three: dg, du, a); or a, g (2), u (2); or dg and du behind
@@ -666,7 +693,7 @@ struct Sum {
     int n, slices;
     long long first;  // its first group of 4 columns
 };
-constexpr int kSums = kJobs + 3;
+constexpr int kSums = kJobs + 3;  // the products, and three biases
 struct Sums {
     Sum s[kSums];
     int n;
@@ -764,7 +791,8 @@ struct Product {
     void *out, *out1, *out2;
     long long pitch;
     const void *bias0, *bias1, *g, *u;
-    Matrix up;  // GLU_AGAIN
+    Matrix up;   // GLU_AGAIN
+    void* sums;  // of A's rows, with bn <= 128
 };
 
 struct Shape {
@@ -817,8 +845,9 @@ Shape shape_of(const Product* p, int n) {
     return best;
 }
 
+size_t product_part_floats(const Product& p, int splits) { return (size_t)splits * (size_t)p.m * (size_t)((p.n + 7) & ~7); }
 size_t part_floats(const Product& p, int splits) {
-    return splits > 1 ? (size_t)splits * (size_t)p.m * (size_t)((p.n + 7) & ~7) : 0;
+    return splits > 1 ? product_part_floats(p, splits) + (p.sums ? (size_t)splits * (size_t)((p.m + 7) & ~7) : 0) : 0;
 }
 template <int TAIL>
 size_t scratch_floats(const Product* p, int n) {
@@ -865,9 +894,11 @@ template <typename T, int TAIL>
 cudaError_t products(const Product* p, int n, int act, int dtype, long long limit, float* part, Sums* sums, cudaStream_t st) {
     const Shape s = shape_of<TAIL>(p, n);
     Work w;
-    w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.limit = limit > 0 ? limit : 2000000000ll;
+    w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.sums = 0, w.limit = limit > 0 ? limit : 2000000000ll;
     const int nb = TAIL == GLU_AGAIN ? 2 * kAgain : s.bn / s.ctas;
-    w.stages = std::min(kMaxStages, ring_bytes(TAIL == GLU_GRAD || TAIL == GLU_AGAIN || (TAIL == GLU && p[0].out1)) / (kStageA + nb * 128));
+    bool ones = false;
+    for (int i = 0; i < n; i++) ones = ones || p[i].sums;
+    w.stages = std::min(kMaxStages, (-(ones ? kOnes : 0) + ring_bytes(TAIL == GLU_GRAD || TAIL == GLU_AGAIN || (TAIL == GLU && p[0].out1))) / (kStageA + nb * 128));
     for (int i = 0; i < n; i++) {
         Job& j = w.job[i];
         const Product& q = p[i];
@@ -907,11 +938,18 @@ cudaError_t products(const Product* p, int n, int act, int dtype, long long limi
             FH_TRY(tail_map(&w.x[1], q.g, true));
             FH_TRY(tail_map(&w.x[2], q.u, true));
         }
-        j.part = nullptr;
+        j.part = j.sums_part = nullptr;
+        j.sums = q.sums;
+        if (q.sums) w.sums = 1;
         if (j.splits > 1) {
             j.part = part;
             sums->s[sums->n++] = {part, q.out, q.bias0, q.pitch, q.m, q.n, j.splits, sums->total};
             sums->total += q.m * (((q.n + 7) & ~7) / 4);
+            if (q.sums) {
+                j.sums_part = part + product_part_floats(q, j.splits);
+                sums->s[sums->n++] = {j.sums_part, q.sums, nullptr, q.m, 1, (int)q.m, j.splits, sums->total};
+                sums->total += ((q.m + 7) & ~7) / 4;
+            }
             part += part_floats(q, j.splits);
         } else {
             FH_TRY(tail_map(&j.o, q.out));
@@ -1071,9 +1109,12 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
         q.mn_b = true;
         q.terms = 2, q.m = p.m, q.n = p.cin, q.k = p.hidden, q.can_split = true, q.out = p.dx, q.pitch = p.dx_pitch;
     }
+    Product* weights[3] = {};
+    int which = 0;
     auto weight = [&](Matrix left, Matrix right, void* out, long long pitch) {
+        which++;
         if (!out) return;
-        Product& q = g.out[g.outs++];
+        Product& q = *(weights[which - 1] = &g.out[g.outs++]);
         q.a[0] = left, q.b[0] = right, q.mn_a = q.mn_b = true;
         q.terms = 1, q.m = left.cols, q.n = right.cols, q.k = p.m, q.can_split = true, q.out = out, q.pitch = pitch;
     };
@@ -1081,6 +1122,12 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
     weight({dg, p.h_pitch, p.m, p.hidden}, x, p.dw_gate, p.dwg_pitch);
     weight({du, p.h_pitch, p.m, p.hidden}, x, p.dw_up, p.dwu_pitch);
     weight({p.dy, p.dy_pitch, p.m, p.cout}, {a, p.h_pitch, p.m, p.hidden}, p.dw_down, p.dwd_pitch);
+    // a bias's gradient is the row sums of its weight's gradient's left operand: taken along where the tiles leave tensor
+    // memory for it, else by a pass of its own
+    void* const db[3] = {p.db_gate, p.db_up, p.db_down};
+    const bool along = g.outs && shape_of<PLAIN>(g.out, g.outs).bn <= 128;
+    for (int i = 0; i < 3; i++)
+        if (along && weights[i]) weights[i]->sums = db[i];
     g.part_bytes = (g.outs ? scratch_floats<PLAIN>(g.out, g.outs) * 4 + 255 : 0) / 256 * 256;
     auto column = [&](const void* x_, long long pitch, int n, void* out) {
         if (!out) return;
@@ -1088,9 +1135,9 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
         g.cols.c[g.ncols++] = {x_, pitch, n, nullptr};
         g.widest = std::max(g.widest, n);
     };
-    column(dg, p.h_pitch, p.hidden, p.db_gate);
-    column(du, p.h_pitch, p.hidden, p.db_up);
-    column(p.dy, p.dy_pitch, p.cout, p.db_down);
+    if (!along || !weights[0]) column(dg, p.h_pitch, p.hidden, p.db_gate);
+    if (!along || !weights[1]) column(du, p.h_pitch, p.hidden, p.db_up);
+    if (!along || !weights[2]) column(p.dy, p.dy_pitch, p.cout, p.db_down);
     if (g.ncols) {
         // about four CTAs per SM over the columns, 64 rows to a slice at least
         const long long across = (long long)((g.widest + 63) / 64) * g.ncols;

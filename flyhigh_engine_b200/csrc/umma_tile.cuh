@@ -173,7 +173,10 @@ __device__ __forceinline__ void commit(uint32_t bar) {
             " tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n}\n" ::"r"(bar)
             : "memory");
 }
-// 16 or 32 accumulator columns of this warp's 32 lanes, valid after wait_ld
+// 1, 16 or 32 accumulator columns of this warp's 32 lanes, valid after wait_ld
+__device__ __forceinline__ void load1(uint32_t taddr, uint32_t& r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(r) : "r"(taddr));
+}
 __device__ __forceinline__ void load16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
