@@ -28,7 +28,8 @@ using namespace rows;
 namespace {
 
 constexpr int kMaxC = 8192;
-constexpr int kForwardThreads = 1024, kGradThreads = 512;  // threads per SM that the registers are cut for
+// threads per SM that the registers are cut for
+constexpr int kForwardThreads = 640, kGradThreads = 512;
 
 // The sum over the LPR threads that share a row, in a fixed order, returned to all of them. LPR <= 32: within a warp;
 // above: over the CTA (LPR == its threads), red holding one float per warp (every thread adds them up, by 16-byte reads).
@@ -220,6 +221,30 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
     };
 #pragma unroll
     for (int q = 0; q < STAGES - 1; q++) fetch(q);
+    // a channel's factors, kept from row to row: w_post * scale * gate (while the gate's row stays the same; with b_post the
+    // three are applied one after another instead), w_pre
+    const bool folded = has_f && !p.b_post;
+    Chunk post_w[NCH], pre_w[NCH];
+    auto fold = [&](const T* gate) {
+#pragma unroll
+        for (int k = 0; k < NCH; k++) {
+            const int c = 8 * (l + k * LPR);
+#pragma unroll
+            for (int j = 0; j < 4; j++) post_w[k].v[j] = make_float2(1.0f, 1.0f);
+            if (!valid[k]) continue;
+            mul_vec<T>(post_w[k], p.w_post, c, valid[k]);
+            mul_vec<T>(post_w[k], p.scale, c, valid[k]);
+            mul_vec<T>(post_w[k], gate, c, valid[k], gvec);
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < NCH; k++) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) pre_w[k].v[j] = make_float2(1.0f, 1.0f);
+        if (valid[k]) mul_vec<T>(pre_w[k], p.w_pre, 8 * (l + k * LPR), valid[k]);
+    }
+    int gate_row = -1;
+    if (folded && !p.gate) fold(nullptr);
     int stage = 0;
     // every thread of a CTA runs the same number of iterations: the sums are CTA-wide barriers or whole-warp shuffles.
     // A row's sums use the buffers of its parity: between a buffer's uses lies a barrier of the row between them.
@@ -239,16 +264,24 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
         if (has_f) {
             if (p.post != FH_NORM_NONE) normalise<LPR, NCH>(p.post, fv, vr, inv_c, p.eps, sums);
             const T* gate = static_cast<const T*>(p.gate);
-            if (gate) gate += (unsigned)min((int)row, m - 1) / rows_per_gate * p.gate_pitch;
+            if (gate) {
+                const int at = (unsigned)min((int)row, m - 1) / rows_per_gate;
+                gate += at * p.gate_pitch;
+                if (folded && at != gate_row) fold(gate), gate_row = at;
+            }
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
                 const int c = 8 * (l + k * LPR);
                 if (!vr[k]) continue;
-                mul_vec<T>(fv[k], p.w_post, c, vr[k]);
-                add_vec<T>(fv[k], p.b_post, c, vr[k]);
-                mul_vec<T>(fv[k], p.scale, c, vr[k]);
-                mul_vec<T>(fv[k], gate, c, vr[k], gvec);
-                add(xv[k], fv[k]);
+                if (folded) {
+                    add_product(xv[k], fv[k], post_w[k]);
+                } else {
+                    mul_vec<T>(fv[k], p.w_post, c, vr[k]);
+                    add_vec<T>(fv[k], p.b_post, c, vr[k]);
+                    mul_vec<T>(fv[k], p.scale, c, vr[k]);
+                    mul_vec<T>(fv[k], gate, c, vr[k], gvec);
+                    add(xv[k], fv[k]);
+                }
                 store_chunk(y + 8 * k * LPR, vr[k], xv[k]);
             }
             y += step * p.y_pitch;
@@ -259,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
             for (int k = 0; k < NCH; k++) {
                 const int c = 8 * (l + k * LPR);
                 if (!vr[k]) continue;
-                mul_vec<T>(xv[k], p.w_pre, c, vr[k]);
+                mul(xv[k], pre_w[k]);
                 add_vec<T>(xv[k], p.b_pre, c, vr[k]);
                 store_chunk(h + 8 * k * LPR, vr[k], xv[k]);
             }
