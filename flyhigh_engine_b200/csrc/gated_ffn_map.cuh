@@ -216,20 +216,20 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
                 wait(d1full + 8 * g, u);
                 if (!ok) break;
                 fence_after();
+                // all of the chunk's columns at once: the next chunk's projections run while these are worked on
+                uint32_t rg[32], ru[32];
+                load32(acc1, rg);
+                load32(acc1 + 64, ru);
+                wait_ld();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(d1empty + 8 * g);
+                __syncwarp();
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    uint32_t rg[16], ru[16];
-                    load16(acc1 + 16 * h, rg);
-                    load16(acc1 + 64 + 16 * h, ru);
-                    wait_ld();
-                    if (h == 1) {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(d1empty + 8 * g);
-                    }
                     float2 v[8], gv[8], uv[8];
-                    pairs(rg, gv);
-                    pairs(ru, uv);
+                    pairs(rg + 16 * h, gv);
+                    pairs(ru + 16 * h, uv);
                     switch (w.act) {
                         case FH_ACT_SILU: glu16<FH_ACT_SILU>(gv, uv, v); break;
                         case FH_ACT_GELU: glu16<FH_ACT_GELU>(gv, uv, v); break;
