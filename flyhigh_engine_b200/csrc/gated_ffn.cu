@@ -800,10 +800,13 @@ struct Shape {
 };
 
 // The tiles of a launch: 256 x 256 or 256 x 128 by a pair of CTAs, or 128 x 128 or 128 x 64 by one; and into how many
-// parts K is cut where the tiles leave SMs idle. Chosen by an estimate in SM cycles: a K block of 64 takes the larger of the
-// matrix pipe (128 x bn x 16 in bn / 2 cycles, 46 at least) and its operands' way into shared memory (about 56 bytes per
-// cycle and SM), a CTA runs ceil(items / slots) tiles one after another, each followed by a tail that the next tile's products
-// hide, and split sums are written, read and joined by another launch.
+// parts each job's K is cut where the tiles leave SMs idle. Chosen by an estimate in SM cycles: a K block of 64 takes the
+// larger of the matrix pipe (128 x bn x 16 in bn / 2 cycles, 46 at least) and its operands' way into shared memory (about 56
+// bytes per cycle and SM); the tail of an item is hidden by the next item's products, its last one's is not; items go
+// round the CTAs, so that more of them than CTAs cost half a longest item at the end; split sums are written and read at
+// about 1,600 bytes per cycle and cost another launch of about 8,500 cycles. All jobs' items are cut to a like length: the
+// longest K over a few numbers of cuts. Over eight shapes from 300 x 256 -> 1024 to 60,000 x 200 -> 704 the choice took 0 to
+// 6 % longer than the best of all kinds and cuts, forward and gradient, where that took 11 to 208 us.
 template <int TAIL>
 Shape shape_of(const Product* p, int n) {
     if (TAIL == GLU_AGAIN) {  // 128 x 64 by one CTA
@@ -814,33 +817,38 @@ Shape shape_of(const Product* p, int n) {
     static const int kinds[4][2] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
     Shape best{};
     double best_t = 1e300;
+    long long kb[kJobs], longest_kb = 1;
+    for (int i = 0; i < n; i++) {
+        kb[i] = (p[i].k + 63) / 64 * p[i].terms;
+        longest_kb = std::max(longest_kb, kb[i]);
+    }
     for (const auto& kind : kinds) {
         Shape s{};
         s.ctas = kind[0], s.bn = kind[1];
         const int slots = kSms / s.ctas, cols = TAIL == GLU ? s.bn / 2 : s.bn;
         const double per_kb = std::max({2.0 * s.bn, 184.0, (128.0 + s.bn / s.ctas) * 128 / 56});
-        const double tail = 600.0 + s.bn * (TAIL == PLAIN ? 3.0 : TAIL == GLU ? 5.0 : 9.0);
-        double busy = 0, longest = 0, extra = 0;
-        bool split_any = false;
-        for (int i = 0; i < n; i++) {
-            const double tiles = (double)((p[i].m + 128 * s.ctas - 1) / (128 * s.ctas)) * ((p[i].n + cols - 1) / cols);
-            const long long kb = (p[i].k + 63) / 64 * p[i].terms;
-            int sp = 1;
-            if (p[i].can_split && tiles < slots / 2) {
-                sp = (int)std::min<double>(std::min<double>(slots / tiles, kb / 4), 64);
-                if (sp < 2) sp = 1;
+        const double tail = 1200.0 + s.bn * (TAIL == PLAIN ? 5.0 : TAIL == GLU ? 8.0 : 14.0);
+        double tiles[kJobs];
+        for (int i = 0; i < n; i++)
+            tiles[i] = (double)((p[i].m + 128 * s.ctas - 1) / (128 * s.ctas)) * ((p[i].n + cols - 1) / cols);
+        static const int tried[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+        for (const int cuts : tried) {
+            const long long len = (longest_kb + cuts - 1) / cuts;
+            if (cuts > 1 && (len < 4 || TAIL != PLAIN)) break;
+            double busy = 0, longest = 0, extra = 0, items = 0;
+            for (int i = 0; i < n; i++) {
+                const int sp = p[i].can_split ? (int)std::max<long long>(1, std::min<long long>(64, kb[i] / len)) : 1;
+                s.splits[i] = sp;
+                const double item = std::max((double)((kb[i] + sp - 1) / sp) * per_kb, tail);
+                items += tiles[i] * sp;
+                busy += tiles[i] * sp * item;
+                longest = std::max(longest, item);
+                if (sp > 1) extra += 8500.0 * (extra == 0) + (double)p[i].m * p[i].n * 8 * sp / 1600;
             }
-            s.splits[i] = sp;
-            const double item = std::max((double)((kb + sp - 1) / sp) * per_kb, tail);
-            busy += tiles * sp * item;
-            longest = std::max(longest, item);
-            if (sp > 1) {
-                split_any = true;
-                extra += (double)p[i].m * p[i].n * (sp + 0.5) * 4 / 3000;
-            }
+            const double t = (items <= slots ? longest : busy / slots + 0.5 * longest) + tail + extra;
+            if (t < best_t) best_t = t, best = s;
+            if (items >= 4.0 * slots && cuts == 1) break;
         }
-        const double t = std::max(longest, std::ceil(busy / slots / longest - 1e-9) * longest) + tail + (split_any ? 5000 : 0) + extra;
-        if (t < best_t) best_t = t, best = s;
     }
     return best;
 }
@@ -849,9 +857,7 @@ size_t product_part_floats(const Product& p, int splits) { return (size_t)splits
 size_t part_floats(const Product& p, int splits) {
     return splits > 1 ? product_part_floats(p, splits) + (p.sums ? (size_t)splits * (size_t)((p.m + 7) & ~7) : 0) : 0;
 }
-template <int TAIL>
-size_t scratch_floats(const Product* p, int n) {
-    const Shape s = shape_of<TAIL>(p, n);
+size_t scratch_floats(const Shape& s, const Product* p, int n) {
     size_t f = 0;
     for (int i = 0; i < n; i++) f += part_floats(p[i], s.splits[i]);
     return f;
@@ -891,8 +897,8 @@ cudaError_t launch_work(const Work& w, cudaStream_t st) {
 
 // the products of one launch; part: scratch_floats, whose sums are added to `sums`
 template <typename T, int TAIL>
-cudaError_t products(const Product* p, int n, int act, int dtype, long long limit, float* part, Sums* sums, cudaStream_t st) {
-    const Shape s = shape_of<TAIL>(p, n);
+cudaError_t products(const Shape& s, const Product* p, int n, int act, int dtype, long long limit, float* part, Sums* sums,
+                     cudaStream_t st) {
     Work w;
     w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.sums = 0, w.limit = limit > 0 ? limit : 2000000000ll;
     const int nb = TAIL == GLU_AGAIN ? 2 * kAgain : s.bn / s.ctas;
@@ -1061,9 +1067,9 @@ cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {
         return few_rows<T, false>(down, p.act, st);
     }
     if (on_map(p)) return block_on_map<T>(p, st);
-    FH_TRY((products<T, GLU>(&glu, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    FH_TRY((products<T, GLU>(shape_of<GLU>(&glu, 1), &glu, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
     fhk::PdlScope pdl(true);  // what follows waits on a kernel of this file
-    FH_TRY((products<T, PLAIN>(&down, 1, p.act, p.dtype, p.wait_cycles,
+    FH_TRY((products<T, PLAIN>(shape_of<PLAIN>(&down, 1), &down, 1, p.act, p.dtype, p.wait_cycles,
                                 reinterpret_cast<float*>(static_cast<char*>(p.scratch) + own_a_bytes(p)), &sums, st)));
     return finish<T>(sums, st);
 }
@@ -1073,6 +1079,7 @@ cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {
 struct GradPlan {
     Product da, out[kJobs];
     int outs;
+    Shape shape;  // of out
     bool again;
     size_t hidden_bytes, all_hidden_bytes, part_bytes, column_bytes;
     ColumnSums cols;
@@ -1125,10 +1132,11 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
     // a bias's gradient is the row sums of its weight's gradient's left operand: taken along where the tiles leave tensor
     // memory for it, else by a pass of its own
     void* const db[3] = {p.db_gate, p.db_up, p.db_down};
-    const bool along = g.outs && shape_of<PLAIN>(g.out, g.outs).bn <= 128;
+    if (g.outs) g.shape = shape_of<PLAIN>(g.out, g.outs);
+    const bool along = g.outs && g.shape.bn <= 128;
     for (int i = 0; i < 3; i++)
         if (along && weights[i]) weights[i]->sums = db[i];
-    g.part_bytes = (g.outs ? scratch_floats<PLAIN>(g.out, g.outs) * 4 + 255 : 0) / 256 * 256;
+    g.part_bytes = (g.outs ? scratch_floats(g.shape, g.out, g.outs) * 4 + 255 : 0) / 256 * 256;
     auto column = [&](const void* x_, long long pitch, int n, void* out) {
         if (!out) return;
         g.db[g.ncols] = out;
@@ -1153,17 +1161,16 @@ GradPlan grad_plan(const FhGatedFfnGradParams& p) {
 }
 
 template <typename T>
-cudaError_t gradient(const FhGatedFfnGradParams& p, cudaStream_t st) {
-    const GradPlan g = grad_plan(p);
+cudaError_t gradient(const FhGatedFfnGradParams& p, const GradPlan& g, cudaStream_t st) {
     // whether dg or du is read (or a, formed with them)
     const bool hidden = p.dx || p.dw_gate || p.dw_up || p.db_gate || p.db_up || (g.again && p.dw_down);
     Sums sums{};
-    if (hidden && g.again) FH_TRY((products<T, GLU_AGAIN>(&g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
-    if (hidden && !g.again) FH_TRY((products<T, GLU_GRAD>(&g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    if (hidden && g.again) FH_TRY((products<T, GLU_AGAIN>(shape_of<GLU_AGAIN>(&g.da, 1), &g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    if (hidden && !g.again) FH_TRY((products<T, GLU_GRAD>(shape_of<GLU_GRAD>(&g.da, 1), &g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
     bool mine = hidden;  // whether the stream's last kernel is one of this file's, which the next may wait for itself
     if (g.outs) {
         fhk::PdlScope pdl(mine);
-        FH_TRY((products<T, PLAIN>(g.out, g.outs, p.act, p.dtype, p.wait_cycles,
+        FH_TRY((products<T, PLAIN>(g.shape, g.out, g.outs, p.act, p.dtype, p.wait_cycles,
                                    reinterpret_cast<float*>(static_cast<char*>(p.scratch) + g.all_hidden_bytes), &sums, st)));
         mine = true;
     }
@@ -1188,7 +1195,7 @@ extern "C" size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p) {
     if (takes_few_rows(p->m, p->cin, p->hidden, p->cout)) return own_a_bytes(*p);
     if (on_map(*p)) return 0;
     const Product down = down_of(*p);
-    return own_a_bytes(*p) + scratch_floats<PLAIN>(&down, 1) * 4;
+    return own_a_bytes(*p) + scratch_floats(shape_of<PLAIN>(&down, 1), &down, 1) * 4;
 }
 
 extern "C" int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream) {
@@ -1238,9 +1245,10 @@ extern "C" int fhk_gated_ffn_grad(const FhGatedFfnGradParams* p, void* stream) {
         if (e == cudaSuccess) e = zero(p->db_down, p->cout, p->cout, 1);
         return (int)e;
     }
-    const size_t need = fhk_gated_ffn_grad_scratch_bytes(p);
-    if (!p->scratch || !aligned16(p->scratch) || p->scratch_bytes < need) return (int)cudaErrorInvalidValue;
-    return (int)(p->dtype == FH_F16 ? gradient<__half>(*p, st) : gradient<__nv_bfloat16>(*p, st));
+    const GradPlan g = grad_plan(*p);
+    if (!p->scratch || !aligned16(p->scratch) || p->scratch_bytes < g.all_hidden_bytes + g.part_bytes + g.column_bytes)
+        return (int)cudaErrorInvalidValue;
+    return (int)(p->dtype == FH_F16 ? gradient<__half>(*p, g, st) : gradient<__nv_bfloat16>(*p, g, st));
 }
 
 extern "C" long long fhk_gated_ffn_wait_timeouts(int reset) {
