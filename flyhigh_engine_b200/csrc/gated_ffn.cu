@@ -1191,7 +1191,7 @@ cudaError_t gradient(const FhGatedFfnGradParams& p, const GradPlan& g, cudaStrea
 }  // namespace
 
 extern "C" size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p) {
-    if (!p || !good_sizes(p) || p->m == 0 || p->h_pitch <= 0) return 0;
+    if (!p || !good_sizes(p) || p->m == 0 || p->h_pitch <= 0 || p->h_pitch > (1ll << 24)) return 0;
     if (takes_few_rows(p->m, p->cin, p->hidden, p->cout)) return own_a_bytes(*p);
     if (on_map(*p)) return 0;
     const Product down = down_of(*p);
@@ -1203,7 +1203,7 @@ extern "C" int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream) {
     if (!aligned16(p->b_gate) || !aligned16(p->b_up) || !aligned16(p->b_down)) return (int)cudaErrorInvalidValue;
     if (!good_rows(p->x, p->x_pitch, p->cin, p->m) || !good_rows(p->y, p->y_pitch, p->cout, p->m) ||
         !good_rows_or_null(p->a, p->h_pitch, p->hidden, p->m) || (p->g != nullptr) != (p->u != nullptr) || (p->g && !p->a) ||
-        p->h_pitch < p->hidden || (p->h_pitch & 7) || p->h_pitch >= (1ll << 36) ||
+        p->h_pitch < p->hidden || (p->h_pitch & 7) || p->h_pitch > (1ll << 24) ||
         !good_rows_or_null(p->g, p->h_pitch, p->hidden, p->m) || !good_rows_or_null(p->u, p->h_pitch, p->hidden, p->m))
         return (int)cudaErrorInvalidValue;
     const size_t need = fhk_gated_ffn_scratch_bytes(p);
@@ -1214,7 +1214,7 @@ extern "C" int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream) {
 }
 
 extern "C" size_t fhk_gated_ffn_grad_scratch_bytes(const FhGatedFfnGradParams* p) {
-    if (!p || !good_sizes(p) || p->m == 0 || p->h_pitch <= 0) return 0;
+    if (!p || !good_sizes(p) || p->m == 0 || p->h_pitch <= 0 || p->h_pitch > (1ll << 24)) return 0;
     const GradPlan g = grad_plan(*p);
     return g.all_hidden_bytes + g.part_bytes + g.column_bytes;
 }
@@ -1224,7 +1224,7 @@ extern "C" int fhk_gated_ffn_grad(const FhGatedFfnGradParams* p, void* stream) {
     if (!good_rows(p->x, p->x_pitch, p->cin, p->m) || !good_rows(p->dy, p->dy_pitch, p->cout, p->m) ||
         !good_rows_or_null(p->g, p->h_pitch, p->hidden, p->m) || !good_rows_or_null(p->u, p->h_pitch, p->hidden, p->m) ||
         !good_rows_or_null(p->a, p->h_pitch, p->hidden, p->m) || (p->g != nullptr) != (p->u != nullptr) ||
-        (p->g != nullptr) != (p->a != nullptr) || p->h_pitch < p->hidden || (p->h_pitch & 7) || p->h_pitch >= (1ll << 36) ||
+        (p->g != nullptr) != (p->a != nullptr) || p->h_pitch < p->hidden || (p->h_pitch & 7) || p->h_pitch > (1ll << 24) ||
         !good_rows_or_null(p->dx, p->dx_pitch, p->cin, p->m) ||
         !good_rows_or_null(p->dw_gate, p->dwg_pitch, p->cin, p->hidden) ||
         !good_rows_or_null(p->dw_up, p->dwu_pitch, p->cin, p->hidden) ||

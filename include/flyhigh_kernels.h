@@ -160,7 +160,7 @@ typedef struct FhGatedFfnParams {
     float* u;
     long long x_pitch, wg_pitch, wu_pitch, wd_pitch, y_pitch, h_pitch;
     long long m;           /* rows, 0 .. 2^31 - 256; 0 is a call that does nothing */
-    int cin, hidden, cout; /* 1 .. 2^20 each */
+    int cin, hidden, cout; /* 1 .. 2^20 each; h_pitch up to 2^24 */
     int act;
     int dtype;
     void* scratch;         /* fhk_gated_ffn_scratch_bytes; NULL where that is 0 */

@@ -48,7 +48,7 @@ def norm_grad_params(**kw):
 @pytest.mark.parametrize("bad", [
     dict(x=None), dict(w_gate=None), dict(w_up=None), dict(w_down=None), dict(y=None), dict(a=None, g=P, u=P), dict(g=P), dict(u=P),
     dict(x=P + 8), dict(w_down=P + 2), dict(y=P + 4), dict(b_gate=P + 2), dict(b_down=P + 8), dict(x_pitch=40),
-    dict(x_pitch=52), dict(wd_pitch=184), dict(h_pitch=196), dict(y_pitch=0), dict(m=-1), dict(m=1 << 31), dict(cin=0),
+    dict(x_pitch=52), dict(wd_pitch=184), dict(h_pitch=196), dict(h_pitch=1 << 25), dict(y_pitch=0), dict(m=-1), dict(m=1 << 31), dict(cin=0),
     dict(hidden=-4), dict(cout=0), dict(cin=(1 << 20) + 1), dict(act=5), dict(act=-1), dict(dtype=2), dict(dtype=-1),
     dict(wait_cycles=-1)], ids=str)
 def test_gated_ffn_refusals(bad):
@@ -57,7 +57,7 @@ def test_gated_ffn_refusals(bad):
 
 @pytest.mark.parametrize("bad", [
     dict(x=None), dict(g=None), dict(u=None), dict(a=None), dict(g=None, u=None), dict(b_gate=P + 2), dict(dy=None), dict(w_up=None), dict(dx=P + 8), dict(dw_up=P + 2),
-    dict(db_up=P + 6), dict(dx_pitch=44), dict(dwg_pitch=40), dict(dwd_pitch=8), dict(h_pitch=100), dict(m=-5), dict(cin=0),
+    dict(db_up=P + 6), dict(dx_pitch=44), dict(dwg_pitch=40), dict(dwd_pitch=8), dict(h_pitch=100), dict(h_pitch=1 << 40), dict(m=-5), dict(cin=0),
     dict(act=9), dict(dtype=3), dict(scratch=None), dict(scratch=P + 4), dict(scratch_bytes=100)], ids=str)
 def test_gated_ffn_gradient_refusals(bad):
     assert fh.lib().fhk_gated_ffn_grad(ctypes.byref(grad_params(**bad)), None) == INVALID
