@@ -8,7 +8,12 @@
 // the accumulators as they are read back. An operand may be K-major or MN-major, so no transposed copy of a weight, of x
 // or of a gradient is ever made. A forward call is two launches (gate and up projections with activation and
 // product; down projection), a gradient two as well (da with the activation's gradient; dx and all weight gradients as
-// jobs of one persistent launch), plus, where they apply, one that joins split sums and two for the biases' column sums.
+// jobs of one persistent launch, with the biases' gradients beside them), and where K was split one more that adds the
+// parts. Each waits for the one before on the device (programmatic dependent launch). Few rows (k_rows) and feature maps
+// of few channels (gated_ffn_map.cuh) have forms of their own.
+//
+// At 8192 rows of 2048 -> 8192 -> 2048 in bf16 the first launch takes 338 us with the tensor pipe active 93 % of the time
+// (1,626 TFLOP/s), the second 205 us (71 %: 256 tiles in four turns of 74 CTA pairs).
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -129,7 +129,7 @@ size_t fhk_gmhs_noalloc_max_floats(void);
  * `channels` values with a row pitch in elements: an NHWC view of contiguous pixels is one, its pitch the pixel pitch
  * cs. Element type FH_F16 or FH_BF16, the same for every tensor of a call (weights, biases and gradients too). Every
  * tensor begins on a 16-byte boundary and pitches are multiples of 8 elements; vectors are contiguous. Elements
- * between a row's channels and its pitch are never read and never written. All products, sums, statistics and activations are held in
+ * between a row's channels and its pitch have no influence and are never written. All products, sums, statistics and activations are held in
  * f32. A call runs on the current device and on the given stream, allocates nothing, and leaves nothing behind:
  * scratch is the caller's (16-byte aligned, contents of no meaning before or after), and calls that may overlap need
  * scratch of their own. Results do not depend on timing: every sum has a fixed order. Invalid arguments are refused with

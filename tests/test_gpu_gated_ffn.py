@@ -74,6 +74,22 @@ def test_larger():
     check(4500, 64, 256, 64, F16)
 
 
+@pytest.mark.parametrize("shape", [(20300, 64, 640, 64), (20300, 64, 256, 64), (19000, 128, 200, 128), (38100, 100, 333, 37),
+                                   (18945, 16, 24, 96)], ids=str)
+def test_maps(shape):
+    """Maps of more than one 128-row tile per SM, where two tiles share a CTA and some have no second last one, with the
+    weights resident and streamed."""
+    check(*shape, F16, act="gelu_tanh", train=False)
+    check(*shape, BF16, bias=False, train=False)
+
+
+def test_long_sums():
+    """Weight and bias gradients over many rows (K split over CTAs), and a long K in the down projection of few tiles."""
+    check(20000, 160, 200, 136, BF16)
+    check(20000, 48, 96, 48, F16, act="gelu")
+    check(150, 64, 8000, 200, BF16, bias=False)
+
+
 @pytest.mark.parametrize("m", [5, 70, 700])
 def test_extreme_gates(m):
     """Gates far in both tails: act and act' reach their limits without NaN."""
@@ -184,6 +200,28 @@ def test_repeatable_on_another_stream_and_in_a_graph(m):
     assert all(torch.equal(second[k], outs[1][k]) for k in second)
 
 
+def test_overlapping_calls_on_two_streams():
+    """Calls in flight at once share nothing: many of them on two streams, each result as alone."""
+    cases = [block(m, c, f, c, F16, seed=m) for m, c, f in ((3, 256, 512), (700, 64, 192), (1500, 480, 640), (20, 96, 96))]
+    layers = [GatedFFN(*w, *b) for _, w, b, _ in cases]
+
+    def step(layer, x, dy):
+        y, saved = layer.forward(x)
+        return [y, *layer.backward(dy, x, saved).values()]
+
+    alone = [step(layer, x, dy) for layer, (x, _, _, dy) in zip(layers, cases)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 2]):
+            k = (i // 2 + i) % len(cases)
+            got.append((k, step(layers[k], cases[k][0], cases[k][3])))
+    torch.cuda.synchronize()
+    for k, r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, alone[k])), k
+
+
 def test_weights_updated_in_place_are_used():
     x, w, b, _ = block(64, 48, 96, 48, F16)
     layer = GatedFFN(*w, *b)
@@ -231,3 +269,7 @@ def test_refusals():
     y, saved = layer.forward(x)
     with pytest.raises(fh.FlyHighError, match="not of one call"):
         layer.backward(dy[:4], x, saved)
+    with pytest.raises(fh.FlyHighError, match="not of one call"):
+        layer.backward(dy[:4], x[:4], saved)
+    with pytest.raises(fh.FlyHighError, match="16-byte"):
+        layer.backward(dy[:1].expand(8, 40), x, saved)
