@@ -134,6 +134,14 @@ __device__ __forceinline__ float2 normalise2(int kx, Chunk (&x)[NCH], int ky, Ch
     return r;
 }
 
+// How rows fill the threads that hold them: every chunk whole in every thread (no masks), chunks whole or absent, or a last
+// one partly filled. The masks are a third of the instructions where they are not needed.
+constexpr int kAny = 0, kWholeChunks = 1, kFull = 2;
+template <int FILL>
+__device__ __forceinline__ int channels_of(int left) {
+    return FILL == kFull ? 8 : FILL == kWholeChunks ? (left > 0 ? 8 : 0) : max(0, min(8, left));
+}
+
 // by (plus) a vector's channels `at`; none: unchanged
 template <typename T>
 __device__ __forceinline__ void mul_vec(Chunk& x, const void* w, long long at, int valid, bool vec = true) {
@@ -187,7 +195,7 @@ struct Ring {
 };
 
 // THREADS / LPR rows at a time per CTA
-template <typename T, int THREADS, int LPR, int NCH, int STAGES>
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, int FILL>
 __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual_norm(const FhResidualNormParams p, unsigned rows_per_gate) {
     __shared__ __align__(16) float red[2 * 4 * 64];
     extern __shared__ uint4 ring_mem[];
@@ -197,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
     const float inv_c = 1.0f / (float)p.c;
     int valid[NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; k++) valid[k] = max(0, min(8, p.c - 8 * (l + k * LPR)));
+    for (int k = 0; k < NCH; k++) valid[k] = channels_of<FILL>(p.c - 8 * (l + k * LPR));
     const bool gvec = gate_vec(p), has_f = p.f != nullptr, has_h = p.h != nullptr;
     const int first = blockIdx.x * RPC + sub, step = gridDim.x * RPC, m = (int)p.m;
     // running pointers: the row that is copied, and the row that is written
@@ -255,7 +263,7 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
         ring.wait();
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
-            vr[k] = row < m ? valid[k] : 0;
+            vr[k] = (FILL == kFull && RPC == 1) || row < m ? valid[k] : 0;
             xv[k] = ring.read(stage, 0, k);
             if (has_f) fv[k] = ring.read(stage, 1, k);
         }
@@ -334,7 +342,7 @@ struct Split {
 };
 
 // the CTA's column sums, part [cta][4][c]: (A1, A0), or with whole runs (sum gate A1, sum gate A0); then sum dh n_y, sum dh
-template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE>
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int FILL>
 __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_norm_grad(const FhResidualNormGradParams p, const Split sp,
                                                                  float* part) {
     constexpr int RPC = THREADS / LPR;
@@ -347,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
     const float inv_c = 1.0f / (float)p.c;
     int valid[NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; k++) valid[k] = max(0, min(8, p.c - 8 * (l + k * LPR)));
+    for (int k = 0; k < NCH; k++) valid[k] = channels_of<FILL>(p.c - 8 * (l + k * LPR));
     const T* f = static_cast<const T*>(p.f);
     const bool gvec = gate_vec(p);
     pdl_trigger();  // what follows sums this kernel's parts, once all of it has ended
@@ -432,7 +440,7 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
             ring.wait();
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
-                vr[k] = row < hi ? valid[k] : 0;
+                vr[k] = (FILL == kFull && RPC == 1) || row < hi ? valid[k] : 0;
                 if (has[0]) d[k] = ring.read(stage, 0, k);
                 else d[k].zero();
                 if (has[1]) {
@@ -635,17 +643,23 @@ cudaError_t allow(K kernel, size_t bytes, std::atomic<bool> (&done)[64]) {
     return cudaSuccess;
 }
 
-template <typename T, int THREADS, int LPR, int NCH, int STAGES>
-cudaError_t run_forward(const FhResidualNormParams& p, cudaStream_t st) {
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, int FILL>
+cudaError_t run_forward_as(const FhResidualNormParams& p, cudaStream_t st) {
     static std::atomic<bool> done[64];
     constexpr size_t smem = Ring<T, THREADS, NCH, 2, STAGES>::kBytes;
-    const cudaError_t e = allow(k_residual_norm<T, THREADS, LPR, NCH, STAGES>, smem, done);
+    const cudaError_t e = allow(k_residual_norm<T, THREADS, LPR, NCH, STAGES, FILL>, smem, done);
     if (e != cudaSuccess) return e;
     constexpr int RPC = THREADS / LPR;
     const long long want = (p.m + RPC - 1) / RPC;
     const int grid = (int)std::min<long long>(want, (long long)kSms * (kForwardThreads / THREADS));
-    return fhk::launch(k_residual_norm<T, THREADS, LPR, NCH, STAGES>, dim3(grid), dim3(THREADS), smem, st, p,
+    return fhk::launch(k_residual_norm<T, THREADS, LPR, NCH, STAGES, FILL>, dim3(grid), dim3(THREADS), smem, st, p,
                        (unsigned)(p.gate ? p.m / p.gates : p.m));
+}
+template <typename T, int THREADS, int LPR, int NCH, int STAGES>
+cudaError_t run_forward(const FhResidualNormParams& p, cudaStream_t st) {
+    if (p.c == 8 * LPR * NCH) return run_forward_as<T, THREADS, LPR, NCH, STAGES, kFull>(p, st);
+    return p.c % 8 ? run_forward_as<T, THREADS, LPR, NCH, STAGES, kAny>(p, st)
+                   : run_forward_as<T, THREADS, LPR, NCH, STAGES, kWholeChunks>(p, st);
 }
 
 template <typename T>
@@ -679,19 +693,21 @@ Split split_of(long long m, int c, int gates, bool gate) {
     return s;
 }
 
-template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE>
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int FILL>
 cudaError_t run_grad_as(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
     static std::atomic<bool> done[64];
     constexpr size_t smem = Ring<T, THREADS, NCH, 4, STAGES>::kBytes;
-    const cudaError_t e = allow(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE>, smem, done);
+    const cudaError_t e = allow(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL>, smem, done);
     if (e != cudaSuccess) return e;
-    return fhk::launch(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE>, dim3(sp.ctas), dim3(THREADS), smem, st, p, sp,
+    return fhk::launch(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL>, dim3(sp.ctas), dim3(THREADS), smem, st, p, sp,
                        static_cast<float*>(p.scratch));
 }
 template <typename T, int THREADS, int LPR, int NCH, int STAGES>
 cudaError_t run_grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
-    return sp.whole ? run_grad_as<T, THREADS, LPR, NCH, STAGES, true>(p, sp, st)
-                    : run_grad_as<T, THREADS, LPR, NCH, STAGES, false>(p, sp, st);
+    if (sp.whole) return run_grad_as<T, THREADS, LPR, NCH, STAGES, true, kAny>(p, sp, st);
+    if (p.c == 8 * LPR * NCH) return run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kFull>(p, sp, st);
+    return p.c % 8 ? run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kAny>(p, sp, st)
+                   : run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kWholeChunks>(p, sp, st);
 }
 
 template <typename T>
