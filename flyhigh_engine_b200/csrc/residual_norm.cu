@@ -35,6 +35,7 @@ constexpr int kForwardThreads = 640, kGradThreads = 512;
 // above: over the CTA (LPR == its threads), red holding one float per warp (every thread adds them up, by 16-byte reads).
 template <int NW>
 __device__ __forceinline__ float add_up(const float* red) {
+    if (NW == 2) return red[0] + red[1];
     float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < NW; i += 4) {
@@ -338,11 +339,12 @@ __device__ __forceinline__ void normalise_grad(int kind, Chunk (&dn)[NCH], const
 struct Split {
     long long len;
     int groups, slices, per_cta, ctas;
-    bool whole;  // CTAs finish their runs' dgate
+    bool whole;   // CTAs finish their runs' dgate
+    bool zeroth;  // sum d and sum dh are wanted (a bias is there, or its gradient)
 };
 
 // the CTA's column sums, part [cta][4][c]: (A1, A0), or with whole runs (sum gate A1, sum gate A0); then sum dh n_y, sum dh
-template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int FILL>
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int FILL, bool ZEROTH>
 __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_norm_grad(const FhResidualNormGradParams p, const Split sp,
                                                                  float* part) {
     constexpr int RPC = THREADS / LPR;
@@ -359,10 +361,11 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
     const T* f = static_cast<const T*>(p.f);
     const bool gvec = gate_vec(p);
     pdl_trigger();  // what follows sums this kernel's parts, once all of it has ended
-    Chunk a1[NCH], a0[NCH], b1[NCH], b0[NCH], g1[WHOLE ? NCH : 1], g0[WHOLE ? NCH : 1];
+    Chunk a1[NCH], a0[ZEROTH ? NCH : 1], b1[NCH], b0[ZEROTH ? NCH : 1], g1[WHOLE ? NCH : 1], g0[WHOLE ? NCH : 1];
 #pragma unroll
     for (int k = 0; k < NCH; k++) {
-        a1[k].zero(), a0[k].zero(), b1[k].zero(), b0[k].zero();
+        a1[k].zero(), b1[k].zero();
+        if (ZEROTH) a0[k].zero(), b0[k].zero();
         if (WHOLE) g1[k].zero(), g0[k].zero();
     }
     // v summed over the CTA's row groups (in order), returned to all of them
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
                 for (int k = 0; k < NCH; k++) {
                     add_product(b1[k], dh[k], yv[k]);
-                    add(b0[k], dh[k]);
+                    if (ZEROTH) add(b0[k], dh[k]);
                     if constexpr (HOIST) mul(dh[k], pre_w[k]);
                     else if (vr[k]) mul_vec<T>(dh[k], p.w_pre, 8 * (l + k * LPR), vr[k]);
                 }
@@ -484,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
                 for (int k = 0; k < NCH; k++) {
                     add_product(a1[k], d[k], fv[k]);
-                    add(a0[k], d[k]);
+                    if (ZEROTH) add(a0[k], d[k]);
                     if constexpr (HOIST) {
                         mul(d[k], post_w[k]);
                     } else if (vr[k]) {
@@ -553,10 +556,10 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
         put(1, g0, true);
     } else {
         put(0, a1, false);
-        put(1, a0, false);
+        if constexpr (ZEROTH) put(1, a0, false);
     }
     put(2, b1, false);
-    put(3, b0, false);
+    if constexpr (ZEROTH) put(3, b0, false);
 }
 
 // 16 columns per CTA, 64 threads per column over the CTAs' sums; blockIdx.y: 0 the post side, 1 the pre side. Up to 64 gate
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(1024) k_residual_norm_params(const FhResidualN
 #pragma unroll 8
             for (int i = lo; i < hi; i++) {
                 v.x += src[(long long)i * 4 * p.c];
-                v.y += src[(long long)i * 4 * p.c + p.c];
+                if (sp.zeroth) v.y += src[(long long)i * 4 * p.c + p.c];
             }
         }
         __syncthreads();
@@ -666,6 +669,7 @@ template <typename T>
 cudaError_t forward(const FhResidualNormParams& p, cudaStream_t st) {
     const int c8 = (p.c + 7) / 8;
     if (c8 <= 8) return run_forward<T, 256, 8, 1, 4>(p, st);
+    if (c8 <= 16) return run_forward<T, 256, 16, 1, 4>(p, st);
     if (c8 <= 32) return run_forward<T, 256, 32, 1, 4>(p, st);
     if (c8 <= 64) return run_forward<T, 256, 32, 2, 3>(p, st);
     if (c8 <= 128) return run_forward<T, 128, 128, 1, 4>(p, st);
@@ -678,8 +682,8 @@ Split split_of(long long m, int c, int gates, bool gate) {
     Split s{};
     s.groups = gate ? gates : 1;
     s.len = m / s.groups;
-    // as many CTAs as are resident at once: kGradThreads threads per SM in CTAs of 128, 256 or 512 (grad())
-    const int target = kSms * (c > 2048 ? 1 : c > 1024 || c <= 256 ? 2 : 4);
+    // as many CTAs as are resident at once: kGradThreads threads per SM in CTAs of 64 to 512 (grad())
+    const int target = kSms * (c > 2048 ? 1 : c > 1024 || c <= 256 ? 2 : c > 512 ? 4 : 8);
     s.whole = s.groups > 1 && s.groups >= target;
     if (s.whole) {
         s.slices = 1;
@@ -693,21 +697,26 @@ Split split_of(long long m, int c, int gates, bool gate) {
     return s;
 }
 
-template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int FILL>
+template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int FILL, bool ZEROTH>
 cudaError_t run_grad_as(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
     static std::atomic<bool> done[64];
     constexpr size_t smem = Ring<T, THREADS, NCH, 4, STAGES>::kBytes;
-    const cudaError_t e = allow(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL>, smem, done);
+    const cudaError_t e = allow(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL, ZEROTH>, smem, done);
     if (e != cudaSuccess) return e;
-    return fhk::launch(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL>, dim3(sp.ctas), dim3(THREADS), smem, st, p, sp,
+    return fhk::launch(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL, ZEROTH>, dim3(sp.ctas), dim3(THREADS), smem, st, p, sp,
                        static_cast<float*>(p.scratch));
 }
 template <typename T, int THREADS, int LPR, int NCH, int STAGES>
 cudaError_t run_grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
-    if (sp.whole) return run_grad_as<T, THREADS, LPR, NCH, STAGES, true, kAny>(p, sp, st);
-    if (p.c == 8 * LPR * NCH) return run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kFull>(p, sp, st);
-    return p.c % 8 ? run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kAny>(p, sp, st)
-                   : run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kWholeChunks>(p, sp, st);
+    if (sp.whole) return run_grad_as<T, THREADS, LPR, NCH, STAGES, true, kAny, true>(p, sp, st);
+    const int fill = p.c == 8 * LPR * NCH ? kFull : p.c % 8 ? kAny : kWholeChunks;
+    if (sp.zeroth)
+        return fill == kFull  ? run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kFull, true>(p, sp, st)
+               : fill == kAny ? run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kAny, true>(p, sp, st)
+                              : run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kWholeChunks, true>(p, sp, st);
+    return fill == kFull  ? run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kFull, false>(p, sp, st)
+           : fill == kAny ? run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kAny, false>(p, sp, st)
+                          : run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kWholeChunks, false>(p, sp, st);
 }
 
 template <typename T>
@@ -715,7 +724,9 @@ cudaError_t grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_
     const int c8 = (p.c + 7) / 8;
     cudaError_t e;
     if (c8 <= 8) e = run_grad<T, 256, 8, 1, 3>(p, sp, st);
+    else if (c8 <= 16) e = run_grad<T, 256, 16, 1, 3>(p, sp, st);
     else if (c8 <= 32) e = run_grad<T, 256, 32, 1, 3>(p, sp, st);
+    else if (c8 <= 64) e = run_grad<T, 64, 64, 1, 3>(p, sp, st);
     else if (c8 <= 128) e = run_grad<T, 128, 128, 1, 3>(p, sp, st);
     else if (c8 <= 256) e = run_grad<T, 256, 256, 1, 3>(p, sp, st);
     else if (c8 <= 512) e = run_grad<T, 512, 512, 1, 3>(p, sp, st);
@@ -796,6 +807,7 @@ extern "C" int fhk_residual_norm_grad(const FhResidualNormGradParams* p, void* s
     }
     if (!p->scratch || !aligned16(p->scratch) || p->scratch_bytes < fhk_residual_norm_grad_scratch_bytes(p))
         return (int)cudaErrorInvalidValue;
-    const Split sp = split_of(p->m, p->c, p->gates, p->gate != nullptr);
+    Split sp = split_of(p->m, p->c, p->gates, p->gate != nullptr);
+    sp.zeroth = sp.whole || p->b_post || p->db_post || p->db_pre;
     return (int)(p->dtype == FH_F16 ? grad<__half>(*p, sp, st) : grad<__nv_bfloat16>(*p, sp, st));
 }
