@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kMaxC = 8192;
 // threads per SM that the registers are cut for
-constexpr int kForwardThreads = 640, kGradThreads = 512;
+constexpr int kForwardThreads = 512, kGradThreads = 512;
 
 // The sum over the LPR threads that share a row, in a fixed order, returned to all of them. LPR <= 32: within a warp;
 // above: over the CTA (LPR == its threads), red holding one float per warp (every thread adds them up, by 16-byte reads).
@@ -230,30 +230,39 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
     };
 #pragma unroll
     for (int q = 0; q < STAGES - 1; q++) fetch(q);
-    // a channel's factors, kept from row to row: w_post * scale * gate (while the gate's row stays the same; with b_post the
-    // three are applied one after another instead), w_pre
-    const bool folded = has_f && !p.b_post;
-    Chunk post_w[NCH], pre_w[NCH];
+    // a channel's factors, kept from row to row: w_post * scale * gate and b_post * scale * gate (while the gate's row stays
+    // the same), w_pre and (where a thread has one chunk) b_pre
+    constexpr bool HOIST = NCH == 1;
+    Chunk post_w[NCH], post_b[NCH], pre_w[NCH], pre_b[HOIST ? NCH : 1];
     auto fold = [&](const T* gate) {
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
             const int c = 8 * (l + k * LPR);
+            Chunk s;
 #pragma unroll
-            for (int j = 0; j < 4; j++) post_w[k].v[j] = make_float2(1.0f, 1.0f);
-            if (!valid[k]) continue;
-            mul_vec<T>(post_w[k], p.w_post, c, valid[k]);
-            mul_vec<T>(post_w[k], p.scale, c, valid[k]);
-            mul_vec<T>(post_w[k], gate, c, valid[k], gvec);
+            for (int j = 0; j < 4; j++) s.v[j] = make_float2(1.0f, 1.0f);
+            post_b[k].zero();
+            if (valid[k]) {
+                mul_vec<T>(s, p.scale, c, valid[k]);
+                mul_vec<T>(s, gate, c, valid[k], gvec);
+                add_vec<T>(post_b[k], p.b_post, c, valid[k]);
+                mul(post_b[k], s);
+                mul_vec<T>(s, p.w_post, c, valid[k]);
+            }
+            post_w[k] = s;
         }
     };
 #pragma unroll
     for (int k = 0; k < NCH; k++) {
 #pragma unroll
         for (int j = 0; j < 4; j++) pre_w[k].v[j] = make_float2(1.0f, 1.0f);
-        if (valid[k]) mul_vec<T>(pre_w[k], p.w_pre, 8 * (l + k * LPR), valid[k]);
+        if (HOIST) pre_b[HOIST ? k : 0].zero();
+        if (!valid[k]) continue;
+        mul_vec<T>(pre_w[k], p.w_pre, 8 * (l + k * LPR), valid[k]);
+        if (HOIST) add_vec<T>(pre_b[HOIST ? k : 0], p.b_pre, 8 * (l + k * LPR), valid[k]);
     }
     int gate_row = -1;
-    if (folded && !p.gate) fold(nullptr);
+    if (has_f && !p.gate) fold(nullptr);
     int stage = 0;
     // every thread of a CTA runs the same number of iterations: the sums are CTA-wide barriers or whole-warp shuffles.
     // A row's sums use the buffers of its parity: between a buffer's uses lies a barrier of the row between them.
@@ -276,21 +285,13 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
             if (gate) {
                 const int at = (unsigned)min((int)row, m - 1) / rows_per_gate;
                 gate += at * p.gate_pitch;
-                if (folded && at != gate_row) fold(gate), gate_row = at;
+                if (at != gate_row) fold(gate), gate_row = at;
             }
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
-                const int c = 8 * (l + k * LPR);
                 if (!vr[k]) continue;
-                if (folded) {
-                    add_product(xv[k], fv[k], post_w[k]);
-                } else {
-                    mul_vec<T>(fv[k], p.w_post, c, vr[k]);
-                    add_vec<T>(fv[k], p.b_post, c, vr[k]);
-                    mul_vec<T>(fv[k], p.scale, c, vr[k]);
-                    mul_vec<T>(fv[k], gate, c, vr[k], gvec);
-                    add(xv[k], fv[k]);
-                }
+                add_product(xv[k], fv[k], post_w[k]);
+                if (p.b_post) add(xv[k], post_b[k]);
                 store_chunk(y + 8 * k * LPR, vr[k], xv[k]);
             }
             y += step * p.y_pitch;
@@ -299,10 +300,10 @@ __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual
             normalise<LPR, NCH>(p.pre, xv, vr, inv_c, p.eps, sums + 128);
 #pragma unroll
             for (int k = 0; k < NCH; k++) {
-                const int c = 8 * (l + k * LPR);
                 if (!vr[k]) continue;
                 mul(xv[k], pre_w[k]);
-                add_vec<T>(xv[k], p.b_pre, c, vr[k]);
+                if constexpr (HOIST) add(xv[k], pre_b[k]);
+                else add_vec<T>(xv[k], p.b_pre, 8 * (l + k * LPR), vr[k]);
                 store_chunk(h + 8 * k * LPR, vr[k], xv[k]);
             }
             h += step * p.h_pitch;
