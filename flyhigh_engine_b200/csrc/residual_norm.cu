@@ -195,6 +195,24 @@ struct Ring {
     __device__ __forceinline__ Chunk read(int stage, int tensor, int k) const { return unpack<T>(*slot(stage, tensor, k)); }
 };
 
+// Chunks that a thread keeps for itself in shared memory, as 32-bit values
+template <int THREADS>
+struct Kept {
+    float4* buf;
+    static constexpr size_t kChunkBytes = (size_t)THREADS * 32;  // one chunk of every thread
+    __device__ __forceinline__ Chunk get(int i) const {
+        const float4 a = buf[2 * i * THREADS + threadIdx.x], b = buf[(2 * i + 1) * THREADS + threadIdx.x];
+        Chunk x;
+        x.v[0] = make_float2(a.x, a.y), x.v[1] = make_float2(a.z, a.w);
+        x.v[2] = make_float2(b.x, b.y), x.v[3] = make_float2(b.z, b.w);
+        return x;
+    }
+    __device__ __forceinline__ void put(int i, const Chunk& x) const {
+        buf[2 * i * THREADS + threadIdx.x] = make_float4(x.v[0].x, x.v[0].y, x.v[1].x, x.v[1].y);
+        buf[(2 * i + 1) * THREADS + threadIdx.x] = make_float4(x.v[2].x, x.v[2].y, x.v[3].x, x.v[3].y);
+    }
+};
+
 // THREADS / LPR rows at a time per CTA
 template <typename T, int THREADS, int LPR, int NCH, int STAGES, int FILL>
 __global__ void __launch_bounds__(THREADS, kForwardThreads / THREADS) k_residual_norm(const FhResidualNormParams p, unsigned rows_per_gate) {
@@ -349,11 +367,15 @@ template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int
 __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_norm_grad(const FhResidualNormGradParams p, const Split sp,
                                                                  float* part) {
     constexpr int RPC = THREADS / LPR;
-    __shared__ __align__(16) float red[2 * 6 * 64];
+    __shared__ __align__(16) float red[2 * 6 * 64];  // whole 128-byte lines: the ring behind it is read by whole lines (2 % of the time)
     float* sums = red;  // a row's sums use the buffers of its parity, as in the forward kernel
     __shared__ float fold[RPC > 1 ? THREADS * NCH * 8 : 1];
     extern __shared__ uint4 ring_mem[];
     const Ring<T, THREADS, NCH, 4, STAGES> ring{ring_mem};
+    // With two chunks a thread, what its registers cannot hold beside the rows: a channel's post factor at [k], sum d and
+    // sum dh at [NCH + k] and [2 NCH + k]. In registers they spilled: 4096 x 8192 with biases 257 us, 230 so
+    constexpr bool SHARED = NCH > 1;
+    const Kept<THREADS> kept{reinterpret_cast<float4*>(ring_mem + Ring<T, THREADS, NCH, 4, STAGES>::kBytes / 16)};
     const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const float inv_c = 1.0f / (float)p.c;
     int valid[NCH];
@@ -362,11 +384,30 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
     const T* f = static_cast<const T*>(p.f);
     const bool gvec = gate_vec(p);
     pdl_trigger();  // what follows sums this kernel's parts, once all of it has ended
-    Chunk a1[NCH], a0[ZEROTH ? NCH : 1], b1[NCH], b0[ZEROTH ? NCH : 1], g1[WHOLE ? NCH : 1], g0[WHOLE ? NCH : 1];
+    constexpr int Z = ZEROTH && !SHARED ? NCH : 1;
+    Chunk a1[NCH], a0[Z], b1[NCH], b0[Z], g1[WHOLE ? NCH : 1], g0[WHOLE ? NCH : 1];
+    auto set = [&](Chunk (&sum)[Z], int at, int k, const Chunk& x) {
+        if constexpr (SHARED) kept.put(at + k, x);
+        else sum[k] = x;
+    };
+    auto add_to = [&](Chunk (&sum)[Z], int at, int k, const Chunk& x) {
+        if constexpr (SHARED) {
+            Chunk t = kept.get(at + k);
+            add(t, x);
+            kept.put(at + k, t);
+        } else {
+            add(sum[k], x);
+        }
+    };
+    auto get = [&](const Chunk (&sum)[Z], int at, int k) {
+        if constexpr (SHARED) return kept.get(at + k);
+        else return sum[k];
+    };
+    constexpr int kA0 = NCH, kB0 = 2 * NCH;  // where sum d and sum dh are kept
 #pragma unroll
     for (int k = 0; k < NCH; k++) {
         a1[k].zero(), b1[k].zero();
-        if (ZEROTH) a0[k].zero(), b0[k].zero();
+        if (ZEROTH) set(a0, kA0, k, a1[k]), set(b0, kB0, k, b1[k]);
         if (WHOLE) g1[k].zero(), g0[k].zero();
     }
     // v summed over the CTA's row groups (in order), returned to all of them
@@ -423,20 +464,21 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
         for (int q = 0; q < STAGES - 1; q++) fetch(q);
         int stage = 0;
-        // what a channel's values are multiplied by in every row of the run: scale * gate * w_post, and w_pre. Kept in
-        // registers where a thread has one chunk of a row; with two they are formed again for each row.
-        constexpr bool HOIST = NCH == 1;
-        Chunk post_w[HOIST ? NCH : 1], pre_w[HOIST ? NCH : 1];
+        // what a channel's values are multiplied by in every row of the run: scale * gate * w_post, and w_pre (which two
+        // chunks a thread read again for each row)
+        Chunk post_w[NCH], pre_w[NCH];
 #pragma unroll
-        for (int k = 0; k < (HOIST ? NCH : 0); k++) {
+        for (int k = 0; k < NCH; k++) {
             const int c = 8 * (l + k * LPR);
 #pragma unroll
             for (int j = 0; j < 4; j++) post_w[k].v[j] = pre_w[k].v[j] = make_float2(1.0f, 1.0f);
-            if (!valid[k]) continue;
-            mul_vec<T>(post_w[k], p.scale, c, valid[k]);
-            if (p.gate) mul_vec<T>(post_w[k], p.gate, (long long)grp * p.gate_pitch + c, valid[k], gvec);
-            mul_vec<T>(post_w[k], p.w_post, c, valid[k]);
-            mul_vec<T>(pre_w[k], p.w_pre, c, valid[k]);
+            if (valid[k]) {
+                mul_vec<T>(post_w[k], p.scale, c, valid[k]);
+                if (p.gate) mul_vec<T>(post_w[k], p.gate, (long long)grp * p.gate_pitch + c, valid[k], gvec);
+                mul_vec<T>(post_w[k], p.w_post, c, valid[k]);
+                if (!SHARED) mul_vec<T>(pre_w[k], p.w_pre, c, valid[k]);
+            }
+            if (SHARED) kept.put(k, post_w[k]);
         }
         for (long long row = lo + sub; row - sub < hi; row += RPC) {
             Chunk d[NCH], dh[NCH], yv[NCH], fv[NCH];
@@ -466,8 +508,8 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
                 for (int k = 0; k < NCH; k++) {
                     add_product(b1[k], dh[k], yv[k]);
-                    if (ZEROTH) add(b0[k], dh[k]);
-                    if constexpr (HOIST) mul(dh[k], pre_w[k]);
+                    if (ZEROTH) add_to(b0, kB0, k, dh[k]);
+                    if constexpr (!SHARED) mul(dh[k], pre_w[k]);
                     else if (vr[k]) mul_vec<T>(dh[k], p.w_pre, 8 * (l + k * LPR), vr[k]);
                 }
                 normalise_grad<LPR, NCH>(p.pre, dh, yv, r.x, inv_c, sums + 128);
@@ -488,15 +530,9 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
                 for (int k = 0; k < NCH; k++) {
                     add_product(a1[k], d[k], fv[k]);
-                    if (ZEROTH) add(a0[k], d[k]);
-                    if constexpr (HOIST) {
-                        mul(d[k], post_w[k]);
-                    } else if (vr[k]) {
-                        const int c = 8 * (l + k * LPR);
-                        mul_vec<T>(d[k], p.scale, c, vr[k]);
-                        if (p.gate) mul_vec<T>(d[k], p.gate, (long long)grp * p.gate_pitch + c, vr[k], gvec);
-                        mul_vec<T>(d[k], p.w_post, c, vr[k]);
-                    }
+                    if (ZEROTH) add_to(a0, kA0, k, d[k]);
+                    if constexpr (SHARED) mul(d[k], kept.get(k));
+                    else mul(d[k], post_w[k]);
                 }
                 if (p.df) {
                     if (p.post != FH_NORM_NONE) normalise_grad<LPR, NCH>(p.post, d, fv, r.y, inv_c, sums + 256);
@@ -513,11 +549,12 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 #pragma unroll
             for (int k = 0; k < (WHOLE ? NCH : 1); k++) {
                 const int c = 8 * (l + k * LPR);
+                Chunk zeroth = get(a0, kA0, k);
                 over_rows(a1[k]);
-                over_rows(a0[k]);
+                over_rows(zeroth);
                 if (valid[k] && sub == 0) {
                     if (p.dgate) {
-                        Chunk q = a1[k], w0 = a0[k];
+                        Chunk q = a1[k], w0 = zeroth;
                         mul_vec<T>(q, p.w_post, c, valid[k]);
                         if (p.b_post) {
                             mul_vec<T>(w0, p.b_post, c, valid[k]);
@@ -528,13 +565,14 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
                                     (p.dgate_pitch & 7) == 0 && ((uintptr_t)p.dgate & 15) == 0);
                     }
                     mul_vec<T>(a1[k], p.gate, grow + c, valid[k], gvec);
-                    mul_vec<T>(a0[k], p.gate, grow + c, valid[k], gvec);
+                    mul_vec<T>(zeroth, p.gate, grow + c, valid[k], gvec);
                 }
                 if (sub == 0) {  // every row group of the CTA holds the run's whole sum: the first keeps it
                     add(g1[k], a1[k]);
-                    add(g0[k], a0[k]);
+                    add(g0[k], zeroth);
                 }
-                a1[k].zero(), a0[k].zero();
+                a1[k].zero();
+                set(a0, kA0, k, a1[k]);
             }
         }
     }
@@ -542,25 +580,26 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
 
     // the CTA's sums
     float* out = part + (long long)blockIdx.x * 4 * p.c;
-    auto put = [&](int q, Chunk (&x)[NCH], bool summed) {
+    auto put = [&](int q, auto value, bool summed) {
 #pragma unroll
         for (int k = 0; k < NCH; k++) {
-            if (!summed) over_rows(x[k]);
+            Chunk x = value(k);
+            if (!summed) over_rows(x);
             const int c = 8 * (l + k * LPR);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (sub == 0 && j < valid[k]) out[(long long)q * p.c + c + j] = x[k].get(j);
+                if (sub == 0 && j < valid[k]) out[(long long)q * p.c + c + j] = x.get(j);
         }
     };
     if constexpr (WHOLE) {
-        put(0, g1, true);
-        put(1, g0, true);
+        put(0, [&](int k) { return g1[k]; }, true);
+        put(1, [&](int k) { return g0[k]; }, true);
     } else {
-        put(0, a1, false);
-        if constexpr (ZEROTH) put(1, a0, false);
+        put(0, [&](int k) { return a1[k]; }, false);
+        if constexpr (ZEROTH) put(1, [&](int k) { return get(a0, kA0, k); }, false);
     }
-    put(2, b1, false);
-    if constexpr (ZEROTH) put(3, b0, false);
+    put(2, [&](int k) { return b1[k]; }, false);
+    if constexpr (ZEROTH) put(3, [&](int k) { return get(b0, kB0, k); }, false);
 }
 
 // 16 columns per CTA, 64 threads per column over the CTAs' sums; blockIdx.y: 0 the post side, 1 the pre side. Up to 64 gate
@@ -701,7 +740,8 @@ Split split_of(long long m, int c, int gates, bool gate) {
 template <typename T, int THREADS, int LPR, int NCH, int STAGES, bool WHOLE, int FILL, bool ZEROTH>
 cudaError_t run_grad_as(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
     static std::atomic<bool> done[64];
-    constexpr size_t smem = Ring<T, THREADS, NCH, 4, STAGES>::kBytes;
+    constexpr size_t smem = Ring<T, THREADS, NCH, 4, STAGES>::kBytes +
+                            (NCH > 1 ? NCH * (ZEROTH ? 3 : 1) * Kept<THREADS>::kChunkBytes : 0);
     const cudaError_t e = allow(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL, ZEROTH>, smem, done);
     if (e != cudaSuccess) return e;
     return fhk::launch(k_residual_norm_grad<T, THREADS, LPR, NCH, STAGES, WHOLE, FILL, ZEROTH>, dim3(sp.ctas), dim3(THREADS), smem, st, p, sp,
