@@ -94,8 +94,10 @@ def reference(t, y, gate, p, pre, post):
     return r
 
 
-def check(m, c, dtype, pre, post, gates=0, affine=True, scale=True, seed=0):
+def check(m, c, dtype, pre, post, gates=0, affine=True, scale=True, seed=0, biases=True):
     t, gate, p = case(m, c, dtype, pre, post, gates, affine, scale, seed)
+    if not biases:
+        p = {k: v for k, v in p.items() if not k.startswith("b_")}
     layer = ResidualNorm(c, dtype, pre=pre, post=post, eps=EPS, **p)
     y, h = layer(t["x"], t["f"], gate)
     got = {"y": y}
@@ -130,6 +132,20 @@ def test_rows_and_gates(m, gates):
     check(m, 200, BF16, "rms", "layer", gates=gates)
     if m <= 4000:
         check(m, 1200, F16, "rms", "none", gates=gates)
+
+
+@pytest.mark.parametrize("c", [60, 64, 120, 128, 250, 256, 500, 512, 1000, 1024, 2000, 2048, 4090, 4096, 5000, 8192])
+def test_without_biases(c):
+    """Several rows a CTA; without biases the gradient forms no sums of d and dh."""
+    check(1501 if c <= 2048 else 333, c, BF16, "rms", "rms", gates=0, biases=False)
+    check(300, c, F16, "layer", "none", gates=3, biases=False, scale=False)
+
+
+@pytest.mark.parametrize("c", [40, 100, 128, 300, 512, 1000, 2056, 5000])
+def test_many_gate_rows(c):
+    """CTAs that finish whole runs of rows with one gate row, more than one run each."""
+    check(2600, c, F16, "layer", "rms", gates=1300)
+    check(1300, c, BF16, "rms", "none", gates=1300, biases=False)
 
 
 def test_wide_many_rows():
