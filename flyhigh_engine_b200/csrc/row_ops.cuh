@@ -76,20 +76,6 @@ __device__ __forceinline__ void store_chunk(T* p, int valid, const Chunk& c, boo
             if (i < valid) p[i] = Elem<T>::from(c.get(i));
     }
 }
-// the same as 8 floats
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
-    const Chunk c = load_chunk(p, valid);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = c.get(i);
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[8]) {
-    Chunk c;
-#pragma unroll
-    for (int i = 0; i < 8; i++) c.set(i, v[i]);
-    store_chunk(p, valid, c);
-}
 
 constexpr long long kMaxRows = (1ll << 31) - 256;
 

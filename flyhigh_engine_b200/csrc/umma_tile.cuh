@@ -106,9 +106,6 @@ __device__ __forceinline__ void stores_read() {
 }
 __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
-    asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory");
-}
 
 // ---- tensor memory and matrix instructions ----
 template <int CTAS>
