@@ -810,8 +810,9 @@ struct Shape {
 // bytes per cycle and SM); the tail of an item is hidden by the next item's products, its last one's is not; items go
 // round the CTAs, so that more of them than CTAs cost half a longest item at the end; split sums are written and read at
 // about 1,600 bytes per cycle and cost another launch of about 8,500 cycles. All jobs' items are cut to a like length: the
-// longest K over a few numbers of cuts. Over eight shapes from 300 x 256 -> 1024 to 60,000 x 200 -> 704 the choice took 0 to
-// 6 % longer than the best of all kinds and cuts, forward and gradient, where that took 11 to 208 us.
+// longest K over a few numbers of cuts. Over eight shapes from 300 x 256 -> 1024 to 60,000 x 200 -> 704, forward and gradient
+// (11 to 243 us), the choice took 0 to 8 % longer than the best of all kinds and cuts, in one case 21 % (the gradient of
+// 3941 x 288 -> 320: 33.2 us where 128 x 64 tiles with four cuts take 27.4).
 template <int TAIL>
 Shape shape_of(const Product* p, int n) {
     if (TAIL == GLU_AGAIN) {  // 128 x 64 by one CTA
