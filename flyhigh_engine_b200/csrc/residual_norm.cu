@@ -705,16 +705,19 @@ cudaError_t run_forward(const FhResidualNormParams& p, cudaStream_t st) {
                    : run_forward_as<T, THREADS, LPR, NCH, STAGES, kWholeChunks>(p, st);
 }
 
+// Threads a row, chunks a thread and rows in the ring, by the channels alone. A row ahead or two is enough, and more reads in
+// flight beside the writes are slower: 16384 x 4096 90 us with 2 rows in the ring, 98 with 3, 99 with 4. Two tiers want a
+// third row all the same (16384 x 1536 35.7 us, 40.6 with 2; 4096 x 8192 45.4 and 48.6).
 template <typename T>
 cudaError_t forward(const FhResidualNormParams& p, cudaStream_t st) {
     const int c8 = (p.c + 7) / 8;
-    if (c8 <= 8) return run_forward<T, 256, 8, 1, 4>(p, st);
-    if (c8 <= 16) return run_forward<T, 256, 16, 1, 4>(p, st);
-    if (c8 <= 32) return run_forward<T, 256, 32, 1, 4>(p, st);
-    if (c8 <= 64) return run_forward<T, 256, 32, 2, 3>(p, st);
-    if (c8 <= 128) return run_forward<T, 128, 128, 1, 4>(p, st);
+    if (c8 <= 8) return run_forward<T, 256, 8, 1, 3>(p, st);
+    if (c8 <= 16) return run_forward<T, 256, 16, 1, 3>(p, st);
+    if (c8 <= 32) return run_forward<T, 256, 32, 1, 3>(p, st);
+    if (c8 <= 64) return run_forward<T, 256, 32, 2, 2>(p, st);
+    if (c8 <= 128) return run_forward<T, 128, 128, 1, 3>(p, st);
     if (c8 <= 256) return run_forward<T, 128, 128, 2, 3>(p, st);
-    if (c8 <= 512) return run_forward<T, 256, 256, 2, 3>(p, st);
+    if (c8 <= 512) return run_forward<T, 256, 256, 2, 2>(p, st);
     return run_forward<T, 512, 512, 2, 3>(p, st);
 }
 
@@ -760,14 +763,17 @@ cudaError_t run_grad(const FhResidualNormGradParams& p, const Split& sp, cudaStr
                           : run_grad_as<T, THREADS, LPR, NCH, STAGES, false, kWholeChunks, false>(p, sp, st);
 }
 
+// One chunk a thread up to 4096 channels, beside its four column sums. A third row in the ring costs 4 % up to 256
+// channels (60,000 x 200 with biases 52.6 us, 54.8 with it) and gains 2 % above 512 (16384 x 2048 with its forward 139.5 us,
+// 136.6 with it).
 template <typename T>
 cudaError_t grad(const FhResidualNormGradParams& p, const Split& sp, cudaStream_t st) {
     const int c8 = (p.c + 7) / 8;
     cudaError_t e;
-    if (c8 <= 8) e = run_grad<T, 256, 8, 1, 3>(p, sp, st);
-    else if (c8 <= 16) e = run_grad<T, 256, 16, 1, 3>(p, sp, st);
-    else if (c8 <= 32) e = run_grad<T, 256, 32, 1, 3>(p, sp, st);
-    else if (c8 <= 64) e = run_grad<T, 64, 64, 1, 3>(p, sp, st);
+    if (c8 <= 8) e = run_grad<T, 256, 8, 1, 2>(p, sp, st);
+    else if (c8 <= 16) e = run_grad<T, 256, 16, 1, 2>(p, sp, st);
+    else if (c8 <= 32) e = run_grad<T, 256, 32, 1, 2>(p, sp, st);
+    else if (c8 <= 64) e = run_grad<T, 64, 64, 1, 2>(p, sp, st);
     else if (c8 <= 128) e = run_grad<T, 128, 128, 1, 3>(p, sp, st);
     else if (c8 <= 256) e = run_grad<T, 256, 256, 1, 3>(p, sp, st);
     else if (c8 <= 512) e = run_grad<T, 512, 512, 1, 3>(p, sp, st);
