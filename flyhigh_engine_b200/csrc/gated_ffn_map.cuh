@@ -11,6 +11,9 @@
 // The biases of the projections enter as one more K step: a tile of ones' first column times a tile that holds the chunk's
 // 128 biases in its first column, exact in the f32 accumulators, so that the activations' warps do not touch them (adding
 // them there cost 8 of 39 us at 129,600 rows of 64 -> 256 -> 64).
+//
+// At that size the kernel takes 31 us, where the products alone would take 8: half goes into the activations' special
+// functions, the rest into the chain from accumulator to activation to operand. 6480 rows of 48 -> 192 -> 48, in 51 CTAs: 10 us.
 #pragma once
 #include <algorithm>
 #include <atomic>

@@ -4,7 +4,9 @@
 //
 // Forward: one pass. LPR threads hold a row in registers (8 channels per chunk, NCH chunks per thread), so the mean,
 // the variance (of the centred values, a second sum over registers) and the result need the row read once; x and f are
-// read and y and h written once, which is the operator's floor: it is bound by HBM.
+// read and y and h written once, which is the operator's floor. Long rows of many are bound by HBM (16384 x 4096, RMS norms:
+// 90 us, 6.0 TB/s); short ones by instructions, 26 a value, and by the launch (130,000 x 64: 11 us, 6 TB/s; a layer norm with
+// biases 13.5); a single row takes 4 us.
 //
 // Gradient: with d = dy + norm_pre'(dh) and q = s * gate * d,
 //   norm'(dv) = r * (dn - n * mean(dn * n) [- mean(dn) for a layer norm]),  dn = dv * w
@@ -12,7 +14,9 @@
 // Every parameter gradient of the post side is formed from two column sums per gate row k, A1 = sum d * n_f and
 // A0 = sum d: with Q = w A1 + b A0 (the column sum of d * p), dgate[k] = s Q[k], ds = sum_k gate[k] Q[k],
 // dw_post = s sum_k gate[k] A1[k], db_post = s sum_k gate[k] A0[k]. So a thread keeps four sums per channel (two per
-// side) for its columns over all rows of its CTA; a second kernel adds the CTAs' sums in a fixed order.
+// side) for its columns over all rows of its CTA; a second kernel adds the CTAs' sums in a fixed order. The gradient is bound
+// by instructions: 49 a value in 55 % of the issue slots, with 16 warps per SM because rows and sums fill the registers
+// (16384 x 2048, RMS norms: 92 us with the sums, 4.4 TB/s; layer norms with biases 116).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -28,7 +32,8 @@ using namespace rows;
 namespace {
 
 constexpr int kMaxC = 8192;
-// threads per SM that the registers are cut for
+// threads per SM that the registers are cut for: 128 each. Forward with 768 threads of 80 was 1 to 9 % faster at 513 to 1000
+// channels and 5 to 10 % slower up to 200 and at 1024; with 1024 threads of 64 up to 40 % slower.
 constexpr int kForwardThreads = 512, kGradThreads = 512;
 
 // The sum over the LPR threads that share a row, in a fixed order, returned to all of them. LPR <= 32: within a warp;
