@@ -412,9 +412,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                             if (!ok) break;
                             tile_get32(tiles + 2 * h * kTile, lane, g);
                             tile_get32(tiles + (2 * h + 1) * kTile, lane, u);
-                            __syncwarp();
-                            fetch(cs + 32 + 16 * h, h);
-                            __syncwarp();
                             switch (w.act) {
                                 case FH_ACT_SILU: glu_grad16<FH_ACT_SILU>(v, g, u, v); break;
                                 case FH_ACT_GELU: glu_grad16<FH_ACT_GELU>(v, g, u, v); break;
@@ -424,6 +421,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                             }
                             tile_put<T>(dst, lane, h, g);
                             tile_put<T>(dst + kTile, lane, h, u);
+                            // The copy that takes the tiles' place next is ordered behind this warp's reads by nothing but
+                            // these: every lane's values have arrived (dg and du, stored above, are formed from all of them),
+                            // and the fence keeps reads before it from copies after it. Issued right after the loads, behind a
+                            // __syncwarp alone, the copy overtook them where memory was busy: g of the next group in some lanes.
+                            fence_async();
+                            __syncwarp();
+                            fetch(cs + 32 + 16 * h, h);
+                            __syncwarp();
                         } else {
                             pairs(r0 + 16 * h, v);
                             if (part) {
