@@ -39,12 +39,15 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// 1 / (1 + exp(-z)) of a pair, with one reciprocal for both (the special functions' unit is what bounds the narrow cases):
-// 1 / a = b / (a b). The powers stop at 2^60 so that their product stays finite; beyond (z < -41) the result is 9e-19.
-__device__ __forceinline__ float2 sigmoid2(float2 z) {
+// s = 1 / (1 + exp(-z)) of a pair, with one reciprocal for both (the special functions' unit is what bounds the narrow cases):
+// 1 / a = b / (a b). The powers stop at 2^60 so that their product stays finite; beyond (z < -41) s is 0. c = 1 - s is formed as
+// exp(-z) s: a difference would leave the reciprocal's error of 6e-8 where s is 1, which a derivative multiplies by g^3.
+__device__ __forceinline__ float2 sigmoid2(float2 z, float2* c = nullptr) {
     const float2 t = mul2(z, pair(-1.44269504f));  // -log2(e) z
-    const float2 d = add2(make_float2(ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))), pair(1.0f));
-    return mul2(pair(rcp(d.x * d.y)), make_float2(d.y, d.x));
+    const float2 e = make_float2(ex2(fminf(t.x, 60.0f)), ex2(fminf(t.y, 60.0f))), d = add2(e, pair(1.0f));
+    const float2 s = mul2(pair(rcp(d.x * d.y)), make_float2(d.y, d.x));
+    if (c) *c = mul2(e, s);
+    return make_float2(t.x > 60.0f ? 0.0f : s.x, t.y > 60.0f ? 0.0f : s.y);
 }
 // Phi(g) = erfc(-g / sqrt 2) / 2 and exp(-g^2 / 2), by formula 7.1.26 of Abramowitz and Stegun (erfc to 1.5e-7): with
 // z = |g| / sqrt 2 and t = 1 / (1 + p z), erfc(z) = t (a1 + t (a2 + ... + t a5)) exp(-z^2)
@@ -87,10 +90,11 @@ __device__ __forceinline__ void act_both(float2 g, float2& v, float2& dv) {
         v = mul2(g, cdf);
         dv = fma2(mul2(g, pair(0.39894228f)), e, cdf);
     } else {
-        const float2 g2 = mul2(g, g);
-        float2 z = g;
+        // g^2 of the derivative's polynomial is held finite, since 1 - s is 0 before it could matter
+        const float2 g2 = mul2(g, g), g2f = make_float2(fminf(g2.x, 1e30f), fminf(g2.y, 1e30f));
+        float2 z = g, c;
         if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(g2, pair(0.07135481f), pair(1.59576912f)));
-        const float2 s = sigmoid2(z), c = fma2(s, pair(-1.0f), pair(1.0f));  // 1 - s
+        const float2 s = sigmoid2(z, &c);  // c: 1 - s
         if (ACT == FH_ACT_SIGMOID) {
             v = s;
             dv = mul2(s, c);
@@ -98,7 +102,7 @@ __device__ __forceinline__ void act_both(float2 g, float2& v, float2& dv) {
             v = mul2(g, s);
             // s + g s (1 - s) dz / dg
             const float2 w = mul2(v, c);
-            dv = ACT == FH_ACT_SILU ? add2(s, w) : fma2(w, fma2(g2, pair(0.21406443f), pair(1.59576912f)), s);
+            dv = ACT == FH_ACT_SILU ? add2(s, w) : fma2(w, fma2(g2f, pair(0.21406443f), pair(1.59576912f)), s);
         }
     }
 }

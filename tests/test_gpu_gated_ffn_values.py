@@ -1,0 +1,81 @@
+"""Gate values over the whole range of the type, seen one by one: a single row of x that is a unit vector hands every hidden
+channel the gate that its weight holds, u = 1 and da = 1, so that y is act(g), w_up's gradient is act(g) and w_gate's is
+act'(g), each behind one rounding to the type (or two of the same value)."""
+import math
+import random
+
+import pytest
+import torch
+
+from flyhigh_engine_b200.kernels import ACTIVATIONS, GatedFFN
+from row_ops_plain import SUBNORMAL, act64, assert_within, half_step
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+MAGNITUDES = [0.0, 1e-3, 0.3, 1.0, 2.5, 4.0, 6.0, 8.0, 10.0, 14.0, 20.0, 41.0, 42.0, 60.0, 100.0, 200.0, 300.0, 1000.0, 1e4, 6e4,
+              1e5, 1e6, 1e10, 1e18, 3e19, 1e30]
+# rows, channels in, copies of the gates (each in another order, so that gates meet other neighbours): the forms for few rows, for
+# feature maps (forward), and tiles
+FORMS = {"rows": (4, 8, 2), "map": (200, 16, 2), "tiles": (200, 16, 4)}
+
+
+def exposed(form, dtype, seed=0):
+    """(x, w_gate, w_up, w_down, dy, gates) of the block described above."""
+    m, c, copies = FORMS[form]
+    gates = [s * g for g in MAGNITUDES for s in (1, -1) if g <= torch.finfo(dtype).max]
+    rng, order = random.Random(seed), []
+    for _ in range(copies):
+        rng.shuffle(gates)
+        order += gates
+    h = len(order)
+    g = torch.tensor(order, dtype=torch.float64, device="cuda").to(dtype)
+    zeros = lambda *s: torch.zeros(s, dtype=dtype, device="cuda")
+    x, wg, wu, wd, dy = zeros(m, c), zeros(h, c), zeros(h, c), zeros(h, h), zeros(m, h)
+    assert h % 8 == 0 and (h <= 128) == (form != "tiles")
+    x[m // 2, 0], dy[m // 2] = 1, 1
+    wg[:, 0], wu[:, 0] = g, 1
+    wd.fill_diagonal_(1)
+    return x, wg, wu, wd, dy, g
+
+
+def evaluation(act, g):
+    """How far act(g) and act'(g) may be off before they are rounded. The sigmoid's argument z is known to 5 2^-24 of itself
+    (its products and constants in f32), |z| < 42 where its power counts, and the power and the reciprocal to 2^-21: s and
+    1 - s to 2^-16 of themselves, and 0 in place of s below 2^-60. erfc by 7.1.26: to 1.5e-7, and never above
+    exp(-g^2 / 2); the power there to 2^-19 of itself."""
+    s, v = 1 / (1 + torch.exp(-g)), act64(act, g)[0].abs()
+    if act == "relu":
+        return torch.zeros_like(g), torch.zeros_like(g)
+    if act == "gelu":
+        e = torch.exp(-g * g / 2)
+        return g.abs() * e.clamp(max=2.0 ** -22) + 2.0 ** -40, e.clamp(max=2.0 ** -22) + g.abs() * e * 2.0 ** -19 + 2.0 ** -24
+    d = act64(act, g)[1].abs()
+    if act == "silu":
+        d = s + g.abs() * s * (1 - s)
+    elif act == "gelu_tanh":
+        k = 2 * math.sqrt(2 / math.pi)
+        s = 1 / (1 + torch.exp(-k * (g + 0.044715 * g ** 3)))
+        slope = k * (1 + 3 * 0.044715 * g * g)
+        d = s + torch.where(s * (1 - s) > 0, g.abs() * s * (1 - s) * slope, 0.0)
+    return 2.0 ** -16 * v + 2.0 ** -40, 2.0 ** -15 * d + 2.0 ** -40
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_gates_of_every_size(dtype, act, form):
+    x, wg, wu, wd, dy, g = exposed(form, dtype)
+    row, e, tiny = x.shape[0] // 2, half_step(dtype), SUBNORMAL[dtype]
+    (v, dv), (fv, fdv) = act64(act, g.double()), evaluation(act, g.double())
+    bound = lambda v, fn: e * (v.abs() + fn) + tiny + fn
+    y = GatedFFN(wg, wu, wd, act=act)(x)
+    assert_within("y", y[row], v, bound(v, fv))
+    for keep in (True, False):
+        layer = GatedFFN(wg, wu, wd, act=act, keep=keep)
+        y, saved = layer.forward(x)
+        r = layer.backward(dy, x, saved)
+        for name, got, want in (("y", y[row], (v, fv)), ("act", r["w_up"][:, 0], (v, fv)), ("act'", r["w_gate"][:, 0], (dv, fdv)),
+                                ("a", r["w_down"].diagonal(), (v, fv))):
+            assert_within(f"{name} (keep {keep})", got, want[0], bound(*want))
+        assert not torch.isnan(r["x"]).any()
