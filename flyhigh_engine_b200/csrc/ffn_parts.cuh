@@ -63,10 +63,14 @@ __device__ __forceinline__ void normal2(float2 g, float2& cdf, float2& e) {
     s = mul2(mul2(mul2(s, t), e), pair(0.5f));  // erfc(z) / 2
     cdf = make_float2(g.x < 0.0f ? s.x : 1.0f - s.x, g.y < 0.0f ? s.y : 1.0f - s.y);
 }
+// What keeps a NaN gate one where act(g) is no product with g: relu, and sigmoid2's value (the smallest of (NaN, 60) there is 60, so
+// that a NaN does not reach the pair's other value)
+__device__ __forceinline__ float2 relu2(float2 g) { return make_float2(g.x <= 0.0f ? 0.0f : g.x, g.y <= 0.0f ? 0.0f : g.y); }
+__device__ __forceinline__ float2 keep_nan(float2 g, float2 s) { return make_float2(g.x != g.x ? g.x : s.x, g.y != g.y ? g.y : s.y); }
 // act(g) of a pair. 0.5 (1 + tanh z) = sigmoid(2 z), so the tanh form of gelu is g sigmoid(2 sqrt(2 / pi) (g + 0.044715 g^3))
 template <int ACT>
 __device__ __forceinline__ float2 act_of(float2 g) {
-    if (ACT == FH_ACT_RELU) return make_float2(g.x > 0.0f ? g.x : 0.0f, g.y > 0.0f ? g.y : 0.0f);
+    if (ACT == FH_ACT_RELU) return relu2(g);
     if (ACT == FH_ACT_GELU) {
         float2 cdf, e;
         normal2(g, cdf, e);
@@ -75,14 +79,13 @@ __device__ __forceinline__ float2 act_of(float2 g) {
     float2 z = g;
     if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(mul2(g, g), pair(0.07135481f), pair(1.59576912f)));
     const float2 s = sigmoid2(z);
-    // the smallest of (NaN, 60) is 60: a NaN is put back
-    return ACT == FH_ACT_SIGMOID ? make_float2(g.x != g.x ? g.x : s.x, g.y != g.y ? g.y : s.y) : mul2(g, s);
+    return ACT == FH_ACT_SIGMOID ? keep_nan(g, s) : mul2(g, s);
 }
-// act(g) and its derivative
+// act(g) and its derivative (relu's is 1 where g > 0, so 0 at a NaN)
 template <int ACT>
 __device__ __forceinline__ void act_both(float2 g, float2& v, float2& dv) {
     if (ACT == FH_ACT_RELU) {
-        v = make_float2(g.x > 0.0f ? g.x : 0.0f, g.y > 0.0f ? g.y : 0.0f);
+        v = relu2(g);
         dv = make_float2(g.x > 0.0f ? 1.0f : 0.0f, g.y > 0.0f ? 1.0f : 0.0f);
     } else if (ACT == FH_ACT_GELU) {
         float2 cdf, e;
@@ -96,8 +99,8 @@ __device__ __forceinline__ void act_both(float2 g, float2& v, float2& dv) {
         if (ACT == FH_ACT_GELU_TANH) z = mul2(g, fma2(g2, pair(0.07135481f), pair(1.59576912f)));
         const float2 s = sigmoid2(z, &c);  // c: 1 - s
         if (ACT == FH_ACT_SIGMOID) {
-            v = s;
-            dv = mul2(s, c);
+            v = keep_nan(g, s);
+            dv = mul2(v, c);
         } else {
             v = mul2(g, s);
             // s + g s (1 - s) dz / dg

@@ -1,6 +1,7 @@
 """Gate values over the whole range of the type, seen one by one: a single row of x that is a unit vector hands every hidden
 channel the gate that its weight holds, u = 1 and da = 1, so that y is act(g), w_up's gradient is act(g) and w_gate's is
 act'(g), each behind one rounding to the type (or two of the same value)."""
+import itertools
 import math
 import random
 
@@ -79,3 +80,36 @@ def test_gates_of_every_size(dtype, act, form):
                                 ("a", r["w_down"].diagonal(), (v, fv))):
             assert_within(f"{name} (keep {keep})", got, want[0], bound(*want))
         assert not torch.isnan(r["x"]).any()
+
+
+@pytest.mark.parametrize("by", ["weight", "bias"])
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+def test_a_gate_that_is_not_a_number_is_not_lost(act, form, by):
+    """A NaN in one hidden channel's gate weight or gate bias alone: act(g) is NaN in every row, and so are the outputs and
+    the gradients that it enters, and no others (its neighbour in a pair among them). relu's derivative there is 0, as
+    that of g > 0 ? g : 0; the other activations' is NaN."""
+    x, wg, wu, wd, dy, _ = exposed(form, BF16)
+    h, row = wg.shape[0], x.shape[0] // 2
+    wg = (torch.randn(wg.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) / 2).to(BF16)
+    bias = torch.zeros(h, dtype=BF16, device="cuda")
+
+    def step(wg, bias, keep):
+        layer = GatedFFN(wg, wu, wd, bias, act=act, keep=keep)
+        y, saved = layer.forward(x)
+        return {"y": y, "inference": layer(x), **layer.backward(dy, x, saved)}
+
+    for keep, j in itertools.product((True, False), (0, 33, h - 1)):
+        clean = step(wg, bias, keep)
+        wg2, bias2 = wg.clone(), bias.clone()
+        (wg2 if by == "weight" else bias2)[j] = float("nan")
+        got = step(wg2, bias2, keep)
+        others = torch.arange(h, device="cuda") != j
+        for k in ("y", "inference"):
+            assert torch.isnan(got[k]).all(), (k, keep, j)
+        for k in ("w_up", "w_gate", "b_gate"):
+            if k == "w_up" or act != "relu":
+                assert torch.isnan(got[k][j]).all(), (k, keep, j)
+            assert torch.equal(got[k][others], clean[k][others]), (k, keep, j)
+        assert torch.isnan(got["w_down"][:, j]).all() and torch.equal(got["w_down"][:, others], clean["w_down"][:, others])
+        assert torch.isnan(got["x"][row]).all()
