@@ -1066,8 +1066,9 @@ Product down_of(const FhGatedFfnParams& p) {
     return q;
 }
 
-// whether a forward call runs as one kernel (gated_ffn_map.cuh): few channels, and nothing of the hidden values is kept
-bool on_map(const FhGatedFfnParams& p) { return !p.g && p.cin <= kMapChannels && p.cout <= kMapChannels; }
+// whether a forward call runs as one kernel (gated_ffn_map.cuh): few channels, and nothing of the hidden values is kept (a alone
+// is kept too: without g and u it cannot serve the gradient, but the caller reads it)
+bool on_map(const FhGatedFfnParams& p) { return !p.a && !p.g && p.cin <= kMapChannels && p.cout <= kMapChannels; }
 
 template <typename T>
 cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {

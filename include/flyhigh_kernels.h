@@ -155,7 +155,7 @@ typedef struct FhGatedFfnParams {
     const void* b_up;      /* [hidden] or NULL */
     const void* b_down;    /* [cout] or NULL */
     void* y;               /* [m][cout] */
-    void* a;               /* [m][hidden], pitch h_pitch: kept for the gradient (with g and u), or NULL: the scratch's */
+    void* a;               /* [m][hidden], pitch h_pitch: written where it is not NULL. The gradient takes it with g and u */
     float* g;              /* [m][hidden] f32, pitch h_pitch: kept for the gradient, or NULL (then u is NULL too) */
     float* u;
     long long x_pitch, wg_pitch, wu_pitch, wd_pitch, y_pitch, h_pitch;

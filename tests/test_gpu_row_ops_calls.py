@@ -1,0 +1,39 @@
+"""Calls of the row operators that their documentation allows beside the ordinary ones."""
+import ctypes
+
+import pytest
+import torch
+
+import flyhigh_engine_b200 as fh
+from flyhigh_engine_b200 import kernels as K
+from row_ops_plain import act64, assert_within, ffn, half_step
+from test_gpu_gated_ffn import block
+
+pytestmark = pytest.mark.gpu
+F16 = torch.float16
+
+
+@pytest.mark.parametrize("shape", [(6, 48, 192, 48), (200, 48, 192, 48), (20300, 64, 200, 64), (200, 136, 260, 72)], ids=str)
+def test_the_activated_product_alone(shape):
+    """fhk_gated_ffn with `a` but neither g nor u: a is written, in every form."""
+    m, c, f, o = shape
+    x, w, b, _ = block(m, c, f, o, F16)
+    y, a = (torch.full((m, n), 7.0, dtype=F16, device="cuda") for n in (o, (f + 7) // 8 * 8))
+    p = K.GatedFfnParams(x=x.data_ptr(), y=y.data_ptr(), a=a.data_ptr(), x_pitch=x.stride(0), y_pitch=o, h_pitch=a.shape[1], m=m, cin=c,
+                         hidden=f, cout=o, act=K.ACTIVATIONS["silu"], dtype=0,
+                         **{n: t.data_ptr() for n, t in zip(("w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down"), (*w, *b))},
+                         **{n: t.stride(0) for n, t in zip(("wg_pitch", "wu_pitch", "wd_pitch"), w)})
+    n = fh.lib().fhk_gated_ffn_scratch_bytes(ctypes.byref(p))
+    scratch = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+    p.scratch, p.scratch_bytes = scratch.data_ptr(), n
+    assert fh.lib().fhk_gated_ffn(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert_within("y", y, *ffn(x, *w, *b, act="silu")["y"])
+    (wg, wu), (bg, bu), x = (t.double() for t in w[:2]), (t.double() for t in b[:2]), x.double()
+    g, u = x @ wg.t() + bg, x @ wu.t() + bu
+    want = act64("silu", g)[0] * u
+    # g and u are sums of c + 1 terms in 32 bits, |silu'| <= 1.1, silu itself to 2^-16 of itself (its argument's rounding)
+    sums = lambda v, wt: 1.1 * (c + 1) * 2.0 ** -23 * (v.abs() + x.abs() @ wt.abs().t())
+    off = sums(g, wg) * u.abs() + act64("silu", g)[0].abs() * sums(u, wu) + 2.0 ** -16 * want.abs()
+    assert_within("a", a[:, :f], want, off + half_step(F16) * (want.abs() + off) + 2.0 ** -25)
+    assert (a[:, f:] == 7).all()
