@@ -213,6 +213,12 @@ def _vector(name: str, t, n: int, dtype, device) -> Optional[int]:
     return t.data_ptr()
 
 
+def _places(tensors) -> list:
+    """Where a layer's parameters lie. A layer keeps its calls' parameter blocks with their pointers, and binds them anew
+    where this has changed (a parameter's .data was replaced, a module was moved)."""
+    return [None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype) for t in tensors]
+
+
 class _Call:
     """One entry point on the current stream of the tensors' device, and its scratch: the bytes by sizes are asked for
     once per layer (`sizes`, a dict of its own), the memory is torch's, for this call alone."""
@@ -277,11 +283,13 @@ class GatedFFN:
     y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down.
 
     w_gate, w_up: [hidden][cin], w_down: [cout][hidden], biases [hidden], [hidden], [cout] or None: CUDA tensors of one
-    type (float16 or bfloat16), used where they lie (no copy: an optimiser may update them in place). act: silu, gelu
-    (erf), gelu_tanh, relu or sigmoid. x: (..., cin); every tensor's rows begin on 16-byte boundaries (empty_rows).
-    keep: whether a training forward call keeps the hidden values for its gradient (10 bytes each), or the gradient forms
-    them again; None: the faster, which is to form them again up to 448 channels in and out (bf16 step, keeping / forming
-    again: 60,000 x 256 -> 1024 470 / 400 us, 16,000 x 384 -> 1536 268 / 256, 16,000 x 512 -> 2048 326 / 340).
+    type (float16 or bfloat16), used where they lie at each call (no copy: an optimiser may update them in place, or their
+    .data be replaced by a tensor of the same shape, type and device; a captured graph keeps the place of its capture).
+    act: silu, gelu (erf), gelu_tanh, relu or sigmoid. x: (..., cin); every tensor's rows begin on 16-byte boundaries
+    (empty_rows). keep: whether a training forward call keeps the hidden values for its gradient (10 bytes each), or the
+    gradient forms them again, from the weights as they are when it is called; None: the faster, which is to form them
+    again up to 448 channels in and out (bf16 step, keeping / forming again: 60,000 x 256 -> 1024 470 / 400 us, 16,000 x
+    384 -> 1536 268 / 256, 16,000 x 512 -> 2048 326 / 340).
     No autograd: forward / backward are called by the training step."""
 
     def __init__(self, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", keep: Optional[bool] = None):
@@ -294,25 +302,37 @@ class GatedFFN:
         self.cout = w_down.shape[0]
         self.weights = (w_gate, w_up, w_down)
         self.biases = (b_gate, b_up, b_down)
-        code = _dtype_code(self.dtype)
+        self._bind()
+        self._sizes, self._grad_sizes = {}, {}
+        self.keep = max(self.cin, self.cout) > 448 if keep is None else bool(keep)
+
+    def _bind(self) -> None:
+        """The calls' parameter blocks with all that does not change from call to call."""
+        code, where = _dtype_code(self.dtype), _places(self.weights + self.biases)
+        (w_gate, w_up, w_down), (b_gate, b_up, b_down) = self.weights, self.biases
         wg, wgp, mg = _rows("w_gate", w_gate, self.cin, self.dtype, self.device)
         wu, wup, mu = _rows("w_up", w_up, self.cin, self.dtype, self.device)
-        wd, wdp, _ = _rows("w_down", w_down, self.hidden, self.dtype, self.device)
-        if mg != mu or w_up.dim() != 2 or min(self.hidden, self.cin, self.cout) < 1:
+        wd, wdp, md = _rows("w_down", w_down, self.hidden, self.dtype, self.device)
+        if (mg, mu, md) != (self.hidden, self.hidden, self.cout) or w_up.dim() != 2 or min(self.hidden, self.cin, self.cout) < 1:
             raise FlyHighError(f"w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and w_down {tuple(w_down.shape)} do not match")
         bias = [_vector(n, b, k, self.dtype, self.device) for n, b, k in
                 (("b_gate", b_gate, self.hidden), ("b_up", b_up, self.hidden), ("b_down", b_down, self.cout))]
         common = dict(w_gate=wg, w_up=wu, w_down=wd, wg_pitch=wgp, wu_pitch=wup, wd_pitch=wdp, cin=self.cin,
-                      hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[act], dtype=code, h_pitch=_up8(self.hidden))
-        # the calls' parameter blocks with all that does not change from call to call
+                      hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[self.act], dtype=code, h_pitch=_up8(self.hidden))
         self._forward_params = GatedFfnParams(**common, b_gate=bias[0], b_up=bias[1], b_down=bias[2])
         self._grad_params = GatedFfnGradParams(**common, b_gate=bias[0], b_up=bias[1])
-        self._sizes, self._grad_sizes = {}, {}
-        self.keep = max(self.cin, self.cout) > 448 if keep is None else bool(keep)
+        self._bound = where
+
+    def _block(self, which: str):
+        """A copy of a parameter block, bound to where the weights are now."""
+        if _places(self.weights + self.biases) != self._bound:
+            self._bind()
+        p = getattr(self, which)
+        return type(p).from_buffer_copy(p)
 
     def _forward(self, x, out, keep: bool):
         import torch
-        p = GatedFfnParams.from_buffer_copy(self._forward_params)
+        p = self._block("_forward_params")
         p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
         if out is None:
             out = _rows_like(x) if self.cout == self.cin else empty_rows((*x.shape[:-1], self.cout), self.dtype, self.device)
@@ -348,7 +368,7 @@ class GatedFFN:
             if not set(want) <= set(names):
                 raise FlyHighError(f"gradients of {sorted(set(want) - set(names))} are not among {names}")
             names = [n for n in names if n in set(want)]
-        p = GatedFfnGradParams.from_buffer_copy(self._grad_params)
+        p = self._block("_grad_params")
         p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
         p.dy, p.dy_pitch, mdy = _rows("dy", dy, self.cout, self.dtype, self.device)
         a = saved._a
@@ -405,21 +425,31 @@ class ResidualNorm:
             raise FlyHighError("a weight or bias was given for a norm that is none")
         self.channels, self.dtype, self.pre, self.post, self.eps = channels, dtype, pre, post, float(eps)
         self.params = {"w_pre": w_pre, "b_pre": b_pre, "w_post": w_post, "b_post": b_post, "scale": scale}
-        code = _dtype_code(dtype)
+        _dtype_code(dtype)
         given = [t for t in self.params.values() if t is not None]
-        ptrs = {}
-        if given:
-            if not given[0].is_cuda:
-                raise FlyHighError("the norms' vectors are CUDA tensors")
-            ptrs = {n: _vector(n, t, channels, dtype, given[0].device) for n, t in self.params.items() if t is not None}
+        if given and not given[0].is_cuda:
+            raise FlyHighError("the norms' vectors are CUDA tensors")
         self.device = given[0].device if given else None
-        common = dict(c=channels, pre=NORMS[pre], post=NORMS[post], eps=self.eps, dtype=code)
-        # the calls' parameter blocks with all that does not change from call to call
+        self._bind()
+        self._names = [n for n, t in self.params.items() if t is not None]
+        self._sizes = {}
+
+    def _bind(self) -> None:
+        """The calls' parameter blocks with all that does not change from call to call."""
+        where = _places(self.params.values())
+        ptrs = {n: _vector(n, t, self.channels, self.dtype, self.device) for n, t in self.params.items() if t is not None}
+        common = dict(c=self.channels, pre=NORMS[self.pre], post=NORMS[self.post], eps=self.eps, dtype=_dtype_code(self.dtype))
         self._forward_params = ResidualNormParams(**common, **ptrs)
         ptrs.pop("b_pre", None)
         self._grad_params = ResidualNormGradParams(**common, **ptrs)
-        self._names = [n for n, t in self.params.items() if t is not None]
-        self._sizes = {}
+        self._bound = where
+
+    def _block(self, which: str):
+        """A copy of a parameter block, bound to where the vectors are now."""
+        if _places(self.params.values()) != self._bound:
+            self._bind()
+        p = getattr(self, which)
+        return type(p).from_buffer_copy(p)
 
     def _device(self, t):
         if not t.is_cuda or (self.device is not None and t.device != self.device):
@@ -441,7 +471,7 @@ class ResidualNorm:
     def __call__(self, x, f=None, gate=None):
         """(y, h); h is None where pre is "none", and y is x itself where f is None."""
         dev, c, dt = self._device(x), self.channels, self.dtype
-        p = ResidualNormParams.from_buffer_copy(self._forward_params)
+        p = self._block("_forward_params")
         p.x, p.x_pitch, m = _rows("x", x, c, dt, dev)
         p.m = m
         y, h = x, None
@@ -469,7 +499,7 @@ class ResidualNorm:
         if first is None or (dh is not None and self.pre == "none"):
             raise FlyHighError("dy or dh is needed, and dh only with a norm before the next block")
         dev, c, dt = self._device(first), self.channels, self.dtype
-        p = ResidualNormGradParams.from_buffer_copy(self._grad_params)
+        p = self._block("_grad_params")
         ptr, pitch, m = _rows("dy" if dy is not None else "dh", first, c, dt, dev)
         p.m = m
         if dy is not None:

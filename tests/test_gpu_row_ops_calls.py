@@ -6,8 +6,10 @@ import torch
 
 import flyhigh_engine_b200 as fh
 from flyhigh_engine_b200 import kernels as K
+from flyhigh_engine_b200.kernels import GatedFFN, ResidualNorm
 from row_ops_plain import act64, assert_within, ffn, half_step
 from test_gpu_gated_ffn import block
+from test_gpu_residual_norm import case
 
 pytestmark = pytest.mark.gpu
 F16 = torch.float16
@@ -37,3 +39,56 @@ def test_the_activated_product_alone(shape):
     off = sums(g, wg) * u.abs() + act64("silu", g)[0].abs() * sums(u, wu) + 2.0 ** -16 * want.abs()
     assert_within("a", a[:, :f], want, off + half_step(F16) * (want.abs() + off) + 2.0 ** -25)
     assert (a[:, f:] == 7).all()
+
+
+@pytest.mark.parametrize("keep", [True, False])
+@pytest.mark.parametrize("m", [5, 200])
+def test_replaced_weights_are_used(m, keep):
+    """A parameter whose .data is replaced lies elsewhere: calls use it there. What a layer cannot use it refuses, until it is
+    put right."""
+    x, w, b, dy = block(m, 48, 96, 40, F16)
+    _, w2, b2, _ = block(m, 48, 96, 40, F16, seed=1)
+    layer, other = GatedFFN(*w, *b, keep=keep), GatedFFN(*w2, *b2, keep=keep)
+
+    def step(layer):
+        y, saved = layer.forward(x)
+        return {"y": y, "inference": layer(x), **layer.backward(dy, x, saved)}
+
+    step(layer)
+    old = [t.data for t in (*w, *b)]  # alive all along
+    for t, new in zip((*w, *b), (*w2, *b2)):
+        t.data = new
+    got, want = step(layer), step(other)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    for i, bad in ((0, old[0][:, :40]), (0, old[0][:88]), (2, old[2].float()), (2, old[2].cpu()), (4, old[4][:90])):
+        t = (*w, *b)[i]
+        good, t.data = t.data, bad
+        with pytest.raises(fh.FlyHighError):
+            layer(x)
+        with pytest.raises(fh.FlyHighError):
+            layer.forward(x)
+        t.data = good
+        assert torch.equal(layer(x), want["inference"])
+
+
+def test_replaced_vectors_of_a_norm_are_used():
+    t, gate, p = case(40, 96, F16, "layer", "rms", gates=2)
+    _, _, p2 = case(40, 96, F16, "layer", "rms", gates=2, seed=1)
+    layer, other = (ResidualNorm(96, F16, pre="layer", post="rms", **v) for v in (p, p2))
+
+    def step(layer):
+        y, h = layer(t["x"], t["f"], gate)
+        return {"y": y, "h": h, **layer.backward(t["dy"], t["dh"], y, t["f"], gate)}
+
+    step(layer)
+    old = {k: v.data for k, v in p.items()}  # alive all along
+    for k, v in p.items():
+        v.data = p2[k]
+    got, want = step(layer), step(other)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    for bad in (old["scale"][:88], old["scale"].float(), old["scale"].cpu(), old["scale"][1:]):
+        good, p["scale"].data = p["scale"].data, bad
+        with pytest.raises(fh.FlyHighError, match="scale"):
+            layer(t["x"], t["f"], gate)
+        p["scale"].data = good
+    assert torch.equal(layer(t["x"], t["f"], gate)[0], want["y"])
