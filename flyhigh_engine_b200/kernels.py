@@ -184,7 +184,7 @@ def _rows(name: str, t, channels: int, dtype, device):
                 continue
             if m == 1:
                 pitch = st
-            elif st != pitch * m:
+            elif st != pitch * m and 0 not in shape[:-1]:
                 raise FlyHighError(f"{name}: its leading dimensions are not rows of one pitch (strides {stride})")
             m *= n
     ptr = t.data_ptr()

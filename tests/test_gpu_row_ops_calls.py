@@ -92,3 +92,20 @@ def test_replaced_vectors_of_a_norm_are_used():
             layer(t["x"], t["f"], gate)
         p["scale"].data = good
     assert torch.equal(layer(t["x"], t["f"], gate)[0], want["y"])
+
+
+@pytest.mark.parametrize("lead", [(3, 0), (0, 3), (2, 0, 5)], ids=str)
+def test_maps_without_pixels(lead):
+    """No rows in any dimension: outputs of that shape, and parameters' gradients of 0."""
+    x, w, b, _ = block(1, 48, 96, 40, F16)
+    empty = lambda c: K.empty_rows((*lead, c), F16)
+    layer = GatedFFN(*w, *b)
+    y, saved = layer.forward(empty(48))
+    assert y.shape == (*lead, 40) and layer(empty(48)).shape == y.shape
+    g = layer.backward(empty(40), empty(48), saved)
+    assert g["x"].shape == (*lead, 48) and all((v == 0).all() for v in g.values())
+    _, gate, p = case(6, 48, F16, "rms", "rms", gates=2)
+    norm = ResidualNorm(48, F16, pre="rms", post="rms", **p)
+    y, h = norm(empty(48), empty(48), gate)
+    assert y.shape == h.shape == (*lead, 48)
+    assert all((v == 0).all() for v in norm.backward(empty(48), empty(48), y, empty(48), gate).values())
