@@ -6,6 +6,7 @@ the caller's CUDA stream."""
 from __future__ import annotations
 
 import ctypes
+import warnings
 from ctypes import Structure, c_float, c_int, c_longlong, c_size_t, c_void_p
 from typing import Optional
 
@@ -219,6 +220,18 @@ def _places(tensors) -> list:
     return [None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype) for t in tensors]
 
 
+def _outside_autograd(layer: str, tensors, stacklevel: int) -> None:
+    """Says so when autograd is on and would be expected to record a call that it cannot see."""
+    import torch
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                warnings.warn(f"{layer} is not recorded by autograd, though one of its tensors requires a gradient: its outputs "
+                              "are cut off from it. Call backward of the layer, and the layer under torch.no_grad()",
+                              stacklevel=stacklevel)
+                return
+
+
 class _Call:
     """One entry point on the current stream of the tensors' device, and its scratch: the bytes by sizes are asked for
     once per layer (`sizes`, a dict of its own), the memory is torch's, for this call alone."""
@@ -290,7 +303,8 @@ class GatedFFN:
     gradient forms them again, from the weights as they are when it is called; None: the faster, which is to form them
     again up to 448 channels in and out (bf16 step, keeping / forming again: 60,000 x 256 -> 1024 470 / 400 us, 16,000 x
     384 -> 1536 268 / 256, 16,000 x 512 -> 2048 326 / 340).
-    No autograd: forward / backward are called by the training step."""
+    No autograd: forward / backward are called by the training step, under torch.no_grad() where a tensor requires a
+    gradient (else a warning says that nothing is recorded)."""
 
     def __init__(self, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", keep: Optional[bool] = None):
         if act not in ACTIVATIONS:
@@ -332,6 +346,7 @@ class GatedFFN:
 
     def _forward(self, x, out, keep: bool):
         import torch
+        _outside_autograd("GatedFFN", (x, *self.weights, *self.biases), 4)
         p = self._block("_forward_params")
         p.x, p.x_pitch, m = _rows("x", x, self.cin, self.dtype, self.device)
         if out is None:
@@ -409,7 +424,7 @@ class ResidualNorm:
     pre, post: "rms", "layer" or "none"; w_pre, b_pre, w_post, b_post, scale: vectors of `channels` or None (a norm
     without them is only normalised). x, f: (..., channels); gate: (gates, channels) of any alignment, each of its rows
     for an equal run of rows (one per image of a batch, say), or None. f None: y is x (the norm before a first block). No
-    autograd."""
+    autograd, as for GatedFFN."""
 
     def __init__(self, channels: int, dtype, pre: str = "rms", post: str = "none", w_pre=None, b_pre=None, w_post=None,
                  b_post=None, scale=None, eps: float = 1e-6):
@@ -470,6 +485,7 @@ class ResidualNorm:
 
     def __call__(self, x, f=None, gate=None):
         """(y, h); h is None where pre is "none", and y is x itself where f is None."""
+        _outside_autograd("ResidualNorm", (x, f, gate, *self.params.values()), 3)
         dev, c, dt = self._device(x), self.channels, self.dtype
         p = self._block("_forward_params")
         p.x, p.x_pitch, m = _rows("x", x, c, dt, dev)

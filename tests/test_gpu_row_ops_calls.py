@@ -1,5 +1,6 @@
 """Calls of the row operators that their documentation allows beside the ordinary ones."""
 import ctypes
+import warnings
 
 import pytest
 import torch
@@ -109,3 +110,28 @@ def test_maps_without_pixels(lead):
     y, h = norm(empty(48), empty(48), gate)
     assert y.shape == h.shape == (*lead, 48)
     assert all((v == 0).all() for v in norm.backward(empty(48), empty(48), y, empty(48), gate).values())
+
+
+def test_a_call_that_autograd_cannot_see_says_so():
+    x, w, b, _ = block(20, 48, 96, 48, F16)
+    _, gate, p = case(20, 48, F16, "rms", "rms", gates=2)
+    ffn_, norm = GatedFFN(*w, *b), ResidualNorm(48, F16, pre="rms", post="rms", **p)
+    calls = [lambda: ffn_(x), lambda: ffn_.forward(x), lambda: norm(x, x, gate)]
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        quiet = [c() for c in calls]
+    for t in (x, w[1], b[2], gate, p["w_post"]):
+        t.requires_grad_(True)
+        concerned = 0
+        for call in calls:
+            with warnings.catch_warnings(record=True) as seen:
+                warnings.simplefilter("always")
+                call()
+            concerned += len(seen)
+            assert all("not recorded by autograd" in str(v.message) and v.filename == __file__ for v in seen)
+            with warnings.catch_warnings(), torch.no_grad():
+                warnings.simplefilter("error")
+                call()
+        assert concerned == (3 if t is x else 2 if t is w[1] or t is b[2] else 1)
+        t.requires_grad_(False)
+    assert torch.equal(ffn_(x), quiet[0])
