@@ -72,6 +72,7 @@ struct Work {
     void* out[2];      // the same outputs
     int jobs, items, bn, stages, act, keep;
     int sums;  // some job's rows are summed: A times a tile of ones, one matrix instruction of 16 columns beside each
+    int extra;  // bytes that a stage's barrier expects beyond its copies (0, or a test's)
     long long limit;
 };
 
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product(const __grid_constant__
                 const CUtensorMap* ma = &j.a[term];
                 const CUtensorMap* mb = &j.b[TAIL == GLU && CTAS == 2 ? rank : term];
                 if (leader) {
-                    if (rank == 0) bar_expect(full + 8 * s, CTAS * (TAIL == GLU_AGAIN && !term ? stage_bytes - kAgain * 128 : stage_bytes));
+                    if (rank == 0) bar_expect(full + 8 * s, CTAS * (TAIL == GLU_AGAIN && !term ? stage_bytes - kAgain * 128 : stage_bytes) + w.extra);
                     if (mn_a) {
                         tensor_load<CTAS>(da, ma, row, kk, bar);
                         tensor_load<CTAS>(da + 8192, ma, row + 64, kk, bar);
@@ -908,11 +909,12 @@ cudaError_t launch_work(const Work& w, cudaStream_t st) {
 }
 
 // the products of one launch; part: scratch_floats, whose sums are added to `sums`
-template <typename T, int TAIL>
-cudaError_t products(const Shape& s, const Product* p, int n, int act, int dtype, long long limit, float* part, Sums* sums,
-                     cudaStream_t st) {
+template <typename T, int TAIL, typename P>
+cudaError_t products(const Shape& s, const Product* p, int n, const P& call, float* part, Sums* sums, cudaStream_t st) {
+    const int dtype = call.dtype;
     Work w;
-    w.jobs = n, w.items = 0, w.bn = s.bn, w.act = act, w.keep = 0, w.sums = 0, w.limit = limit > 0 ? limit : 2000000000ll;
+    w.jobs = n, w.items = 0, w.bn = s.bn, w.act = call.act, w.keep = 0, w.sums = 0, w.extra = call.test_extra_tx;
+    w.limit = call.wait_cycles > 0 ? call.wait_cycles : 2000000000ll;
     const int nb = TAIL == GLU_AGAIN ? 2 * kAgain : s.bn / s.ctas;
     bool ones = false;
     for (int i = 0; i < n; i++) ones = ones || p[i].sums;
@@ -1036,7 +1038,8 @@ template <typename P>
 bool good_sizes(const P* p) {
     return p->m >= 0 && p->m <= kMaxRows && p->cin >= 1 && p->cin <= kMaxChannels && p->hidden >= 1 &&
            p->hidden <= kMaxChannels && p->cout >= 1 && p->cout <= kMaxChannels && p->act >= FH_ACT_SILU &&
-           p->act <= FH_ACT_SIGMOID && (p->dtype == FH_F16 || p->dtype == FH_BF16) && p->wait_cycles >= 0;
+           p->act <= FH_ACT_SIGMOID && (p->dtype == FH_F16 || p->dtype == FH_BF16) && p->wait_cycles >= 0 &&
+           p->test_extra_tx >= 0 && p->test_extra_tx <= 65536 && p->test_extra_tx % 16 == 0;
 }
 template <typename P>
 bool good_weights(const P* p) {
@@ -1080,9 +1083,9 @@ cudaError_t forward(const FhGatedFfnParams& p, cudaStream_t st) {
         return few_rows<T, false>(down, p.act, st);
     }
     if (on_map(p)) return block_on_map<T>(p, st);
-    FH_TRY((products<T, GLU>(shape_of<GLU>(&glu, 1), &glu, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    FH_TRY((products<T, GLU>(shape_of<GLU>(&glu, 1), &glu, 1, p, nullptr, nullptr, st)));
     fhk::PdlScope pdl(true);  // what follows waits on a kernel of this file
-    FH_TRY((products<T, PLAIN>(shape_of<PLAIN>(&down, 1), &down, 1, p.act, p.dtype, p.wait_cycles,
+    FH_TRY((products<T, PLAIN>(shape_of<PLAIN>(&down, 1), &down, 1, p,
                                 reinterpret_cast<float*>(static_cast<char*>(p.scratch) + own_a_bytes(p)), &sums, st)));
     return finish<T>(sums, st);
 }
@@ -1178,12 +1181,12 @@ cudaError_t gradient(const FhGatedFfnGradParams& p, const GradPlan& g, cudaStrea
     // whether dg or du is read (or a, formed with them)
     const bool hidden = p.dx || p.dw_gate || p.dw_up || p.db_gate || p.db_up || (g.again && p.dw_down);
     Sums sums{};
-    if (hidden && g.again) FH_TRY((products<T, GLU_AGAIN>(shape_of<GLU_AGAIN>(&g.da, 1), &g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
-    if (hidden && !g.again) FH_TRY((products<T, GLU_GRAD>(shape_of<GLU_GRAD>(&g.da, 1), &g.da, 1, p.act, p.dtype, p.wait_cycles, nullptr, nullptr, st)));
+    if (hidden && g.again) FH_TRY((products<T, GLU_AGAIN>(shape_of<GLU_AGAIN>(&g.da, 1), &g.da, 1, p, nullptr, nullptr, st)));
+    if (hidden && !g.again) FH_TRY((products<T, GLU_GRAD>(shape_of<GLU_GRAD>(&g.da, 1), &g.da, 1, p, nullptr, nullptr, st)));
     bool mine = hidden;  // whether the stream's last kernel is one of this file's, which the next may wait for itself
     if (g.outs) {
         fhk::PdlScope pdl(mine);
-        FH_TRY((products<T, PLAIN>(g.shape, g.out, g.outs, p.act, p.dtype, p.wait_cycles,
+        FH_TRY((products<T, PLAIN>(g.shape, g.out, g.outs, p,
                                    reinterpret_cast<float*>(static_cast<char*>(p.scratch) + g.all_hidden_bytes), &sums, st)));
         mine = true;
     }

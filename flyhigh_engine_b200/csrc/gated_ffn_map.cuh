@@ -39,6 +39,7 @@ struct alignas(64) MapWork {
     int chunks, slots, resident;
     int groups;      // 128-row tiles of a CTA, 1 or 2
     int tiles, act;
+    int extra;       // bytes that x's barrier expects beyond its copies (0, or a test's)
     const void *b_gate, *b_up, *b_down;
     void* out;
     long long pitch, limit;
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(kMapThreads, 1) k_block(const __grid_constant_
             if (!wait(xempty + 8 * b, n / xbufs + 1)) break;
             if (leader) {
                 const int live = groups == 2 && tile_of(n, 1) < w.tiles ? 2 : 1;
-                bar_expect(xfull + 8 * b, live * xtile);
+                bar_expect(xfull + 8 * b, live * xtile + w.extra);
                 for (int g = 0; g < live; g++)
                     for (int k = 0; k < kb; k++)
                         tensor_load<1>(xs + (b * 2 + g) * xtile + k * 16384, &w.x, k * BK, tile_of(n, g) * 128, xfull + 8 * b);
@@ -329,7 +330,7 @@ cudaError_t block_on_map(const FhGatedFfnParams& p, cudaStream_t st) {
         prepared[dev].store(true, std::memory_order_release);
     }
     MapWork w;
-    w.m = (int)p.m, w.hidden = p.hidden, w.cout = p.cout, w.act = p.act;
+    w.m = (int)p.m, w.hidden = p.hidden, w.cout = p.cout, w.act = p.act, w.extra = p.test_extra_tx;
     w.kb = (p.cin + 63) / 64, w.ksteps = (p.cin + 15) / 16, w.np = (p.cout + 31) / 32 * 32;
     w.chunks = (p.hidden + kMapChunk - 1) / kMapChunk;
     w.slots = std::min(kMapSlots, kMapW / (w.kb * 16384 + w.np * 128));

@@ -113,7 +113,7 @@ class GatedFfnParams(Structure):  # FhGatedFfnParams
     _fields_ = [(n, c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down", "y", "a", "g", "u")] + \
         [(n, c_longlong) for n in ("x_pitch", "wg_pitch", "wu_pitch", "wd_pitch", "y_pitch", "h_pitch", "m")] + \
         [(n, c_int) for n in ("cin", "hidden", "cout", "act", "dtype")] + \
-        [("scratch", c_void_p), ("scratch_bytes", c_size_t), ("wait_cycles", c_longlong)]
+        [("scratch", c_void_p), ("scratch_bytes", c_size_t), ("wait_cycles", c_longlong), ("test_extra_tx", c_int)]
 
 
 class GatedFfnGradParams(Structure):  # FhGatedFfnGradParams
@@ -122,7 +122,7 @@ class GatedFfnGradParams(Structure):  # FhGatedFfnGradParams
         [(n, c_longlong) for n in ("x_pitch", "wg_pitch", "wu_pitch", "wd_pitch", "h_pitch", "dy_pitch", "dx_pitch",
                                    "dwg_pitch", "dwu_pitch", "dwd_pitch", "m")] + \
         [(n, c_int) for n in ("cin", "hidden", "cout", "act", "dtype")] + \
-        [("scratch", c_void_p), ("scratch_bytes", c_size_t), ("wait_cycles", c_longlong)]
+        [("scratch", c_void_p), ("scratch_bytes", c_size_t), ("wait_cycles", c_longlong), ("test_extra_tx", c_int)]
 
 
 class ResidualNormParams(Structure):  # FhResidualNormParams
@@ -303,17 +303,22 @@ class GatedFFN:
     gradient forms them again, from the weights as they are when it is called; None: the faster, which is to form them
     again up to 448 channels in and out (bf16 step, keeping / forming again: 60,000 x 256 -> 1024 470 / 400 us, 16,000 x
     384 -> 1536 268 / 256, 16,000 x 512 -> 2048 326 / 340).
+    wait_cycles: the bound of each wait inside the kernels, in SM clock cycles (0: about a second); a wait that runs out ends
+    its call with unusable outputs, which `check` reports.
     No autograd: forward / backward are called by the training step, under torch.no_grad() where a tensor requires a
     gradient (else a warning says that nothing is recorded)."""
 
-    def __init__(self, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", keep: Optional[bool] = None):
+    def __init__(self, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, act: str = "silu", keep: Optional[bool] = None,
+                 wait_cycles: int = 0):
+        if not 0 <= wait_cycles < 2 ** 63:
+            raise FlyHighError(f"wait_cycles {wait_cycles} is not a number of cycles")
         if act not in ACTIVATIONS:
             raise FlyHighError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
         if w_gate.dim() != 2 or w_down.dim() != 2 or not w_gate.is_cuda:
             raise FlyHighError("the weights are CUDA matrices")
         self.dtype, self.device, self.act = w_gate.dtype, w_gate.device, act
         self.hidden, self.cin = w_gate.shape
-        self.cout = w_down.shape[0]
+        self.cout, self.wait_cycles = w_down.shape[0], int(wait_cycles)
         self.weights = (w_gate, w_up, w_down)
         self.biases = (b_gate, b_up, b_down)
         self._bind()
@@ -332,7 +337,8 @@ class GatedFFN:
         bias = [_vector(n, b, k, self.dtype, self.device) for n, b, k in
                 (("b_gate", b_gate, self.hidden), ("b_up", b_up, self.hidden), ("b_down", b_down, self.cout))]
         common = dict(w_gate=wg, w_up=wu, w_down=wd, wg_pitch=wgp, wu_pitch=wup, wd_pitch=wdp, cin=self.cin,
-                      hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[self.act], dtype=code, h_pitch=_up8(self.hidden))
+                      hidden=self.hidden, cout=self.cout, act=ACTIVATIONS[self.act], dtype=code, h_pitch=_up8(self.hidden),
+                      wait_cycles=self.wait_cycles)
         self._forward_params = GatedFfnParams(**common, b_gate=bias[0], b_up=bias[1], b_down=bias[2])
         self._grad_params = GatedFfnGradParams(**common, b_gate=bias[0], b_up=bias[1])
         self._bound = where
@@ -364,6 +370,16 @@ class GatedFFN:
         p.a, p.g, p.u = a.data_ptr(), gu.data_ptr(), gu.data_ptr() + 4 * m * hp
         _gated_ffn(p, self.device, self._sizes, (m, True))
         return out, GatedFFNSaved(m, self.hidden, a, gu)
+
+    def check(self) -> None:
+        """Waits for the layer's device and raises if a wait inside the kernels of any gated feed-forward block there ran
+        out since the last check: the outputs of the calls since then are not to be used. Not during a stream capture."""
+        import torch
+        with torch.cuda.device(self.device):
+            torch.cuda.synchronize()
+            n = lib().fhk_gated_ffn_wait_timeouts(1)
+        if n:
+            raise FlyHighError(f"gated_ffn: {n} waits inside its kernels ran out" if n > 0 else "gated_ffn: its count of waits cannot be read")
 
     def __call__(self, x, out=None):
         """y for x (inference: nothing is kept)."""

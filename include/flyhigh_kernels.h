@@ -166,6 +166,7 @@ typedef struct FhGatedFfnParams {
     void* scratch;         /* fhk_gated_ffn_scratch_bytes; NULL where that is 0 */
     size_t scratch_bytes;
     long long wait_cycles; /* bound of each wait inside the kernels, SM clock cycles; 0 = 2e9 (about a second) */
+    int test_extra_tx;     /* 0. Tests only: bytes a barrier expects beyond its copies (a multiple of 16), so its waits run out */
 } FhGatedFfnParams;
 int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream);
 /* Of the sizes, and of whether a and g are NULL. Up to 128 channels in and out the hidden values of a call that keeps nothing
@@ -173,8 +174,8 @@ int fhk_gated_ffn(const FhGatedFfnParams* p, void* stream);
 size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p);
 
 /* The block's gradient for dy, from x, the weights and what the forward call kept (g, u, a), or with all three NULL from x,
- * the weights and the biases alone: g, u and a are formed again (with few channels this costs less than to keep and read
- * them; it always costs less memory).
+ * the weights and the biases alone, as they are at this call: g, u and a are formed again (with few channels this costs less
+ * than to keep and read them; it always costs less memory).
  * da = dy w_down; dg = da * u * act'(g), du = da * act(g), both rounded to the element type;
  * dx = dg w_gate + du w_up; dw_gate = dg^T x; dw_up = du^T x; dw_down = dy^T a; db_* the column sums of dg, du, dy.
  * Each output may be NULL (not wanted). Every output is written, not added to. With m = 0 the weights' and biases'
@@ -196,11 +197,14 @@ typedef struct FhGatedFfnGradParams {
     void* scratch;
     size_t scratch_bytes;
     long long wait_cycles;
+    int test_extra_tx;
 } FhGatedFfnGradParams;
 int fhk_gated_ffn_grad(const FhGatedFfnGradParams* p, void* stream);
 size_t fhk_gated_ffn_grad_scratch_bytes(const FhGatedFfnGradParams* p);
-/* Waits inside the block's kernels that ran out (the call's outputs are then not to be used) since the last reset, on
- * the current device; reset != 0 zeroes the count. Returns -1 when the count cannot be read. */
+/* Waits inside the block's kernels that ran out (the call's outputs are then not to be used; the call itself returned 0, since
+ * this is known only once its kernels have run) since the last reset, on the current device; reset != 0 zeroes the count.
+ * Synchronise the calls' streams first: reading the count waits for none of them. Not during a stream capture. Returns -1
+ * when the count cannot be read. */
 long long fhk_gated_ffn_wait_timeouts(int reset);
 
 /* norm kinds */
