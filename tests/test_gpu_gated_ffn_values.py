@@ -82,6 +82,37 @@ def test_gates_of_every_size(dtype, act, form):
         assert not torch.isnan(r["x"]).any()
 
 
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+def test_hidden_values_between_the_types_steps(dtype, act, form):
+    """g and u that 16 bits do not hold (sums of a weight and a small one, exact in 32): act(g) u, act'(g) u and act(g) are
+    still one rounding away, so neither g nor u is rounded on the way, kept or formed again."""
+    x, wg, wu, wd, dy, _ = exposed(form, dtype)
+    h, row, e, tiny = wg.shape[0], x.shape[0] // 2, half_step(dtype), SUBNORMAL[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    rnd = lambda: torch.randn(h, generator=gen, device="cuda")
+    x[row, 1] = 1
+    for w, v in ((wg, 2 * rnd()), (wu, rnd())):
+        w[:, 0], w[:, 1] = v.to(dtype), (v * rnd().clamp(-1, 1) * e).to(dtype)
+    g, u = (w[:, 0].double() + w[:, 1].double() for w in (wg, wu))
+    (v, dv), (fv, fdv) = act64(act, g), evaluation(act, g)
+    # the evaluation's bound, and the products' roundings in 32 bits
+    want = {"a": (v * u, fv * u.abs()), "act": (v, fv), "act'": (dv * u, fdv * u.abs())}
+    bound = lambda v, fn: (e + 2.0 ** -22) * (v.abs() + fn) + tiny + fn
+    for keep in (True, False):
+        layer = GatedFFN(wg, wu, wd, act=act, keep=keep)
+        y, saved = layer.forward(x)
+        r = layer.backward(dy, x, saved)
+        for name, got in (("a", y[row]), ("act", r["w_up"][:, 0]), ("act'", r["w_gate"][:, 1]), ("a", r["w_down"].diagonal())):
+            assert_within(f"{name} (keep {keep})", got, want[name][0], bound(*want[name]))
+    # the bound would tell: with g and u rounded to the type, some of these values are beyond it
+    if act not in ("relu", "sigmoid"):
+        g16, u16 = (t.to(dtype).double() for t in (g, u))
+        rounded = act64(act, g16)[1] * u16
+        assert ((rounded.to(dtype).double() - want["act'"][0]).abs() > bound(*want["act'"])).any()
+
+
 @pytest.mark.parametrize("by", ["weight", "bias"])
 @pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("act", list(ACTIVATIONS))
