@@ -214,10 +214,22 @@ def _vector(name: str, t, n: int, dtype, device) -> Optional[int]:
     return t.data_ptr()
 
 
-def _places(tensors) -> list:
+class _Places:
     """Where a layer's parameters lie. A layer keeps its calls' parameter blocks with their pointers, and binds them anew
-    where this has changed (a parameter's .data was replaced, a module was moved)."""
-    return [None if t is None else (t.data_ptr(), t.shape, t.stride(), t.dtype) for t in tensors]
+    where this has changed (a parameter's .data was replaced, a module was moved). Asked at every call, so it looks at what
+    a replacement of the same shape and type may change: the addresses, and the pitches of matrices (0.8 us; all of
+    shape, strides and type took 3)."""
+
+    def __init__(self, tensors):
+        given = [t for t in tensors if t is not None]
+        self.ptr, self.stride = [t.data_ptr for t in given], [t.stride for t in given if t.dim() > 1]
+        self.was = self.now()
+
+    def now(self):
+        return [f() for f in self.ptr], [f() for f in self.stride]
+
+    def changed(self) -> bool:
+        return self.now() != self.was
 
 
 def _outside_autograd(layer: str, tensors, stacklevel: int) -> None:
@@ -301,8 +313,8 @@ class GatedFFN:
     act: silu, gelu (erf), gelu_tanh, relu or sigmoid. x: (..., cin); every tensor's rows begin on 16-byte boundaries
     (empty_rows). keep: whether a training forward call keeps the hidden values for its gradient (10 bytes each), or the
     gradient forms them again, from the weights as they are when it is called; None: the faster, which is to form them
-    again up to 448 channels in and out (bf16 step, keeping / forming again: 60,000 x 256 -> 1024 470 / 400 us, 16,000 x
-    384 -> 1536 268 / 256, 16,000 x 512 -> 2048 326 / 340).
+    again up to 448 channels in and out (bf16 step, keeping / forming again: 60,000 x 256 -> 1024 472 / 416 us, 16,000 x
+    384 -> 1536 271 / 261, 16,000 x 512 -> 2048 335 / 348).
     wait_cycles: the bound of each wait inside the kernels, in SM clock cycles (0: about a second); a wait that runs out ends
     its call with unusable outputs, which `check` reports.
     No autograd: forward / backward are called by the training step, under torch.no_grad() where a tensor requires a
@@ -327,7 +339,7 @@ class GatedFFN:
 
     def _bind(self) -> None:
         """The calls' parameter blocks with all that does not change from call to call."""
-        code, where = _dtype_code(self.dtype), _places(self.weights + self.biases)
+        code, places = _dtype_code(self.dtype), _Places(self.weights + self.biases)
         (w_gate, w_up, w_down), (b_gate, b_up, b_down) = self.weights, self.biases
         wg, wgp, mg = _rows("w_gate", w_gate, self.cin, self.dtype, self.device)
         wu, wup, mu = _rows("w_up", w_up, self.cin, self.dtype, self.device)
@@ -341,11 +353,11 @@ class GatedFFN:
                       wait_cycles=self.wait_cycles)
         self._forward_params = GatedFfnParams(**common, b_gate=bias[0], b_up=bias[1], b_down=bias[2])
         self._grad_params = GatedFfnGradParams(**common, b_gate=bias[0], b_up=bias[1])
-        self._bound = where
+        self._places = places
 
     def _block(self, which: str):
         """A copy of a parameter block, bound to where the weights are now."""
-        if _places(self.weights + self.biases) != self._bound:
+        if self._places.changed():
             self._bind()
         p = getattr(self, which)
         return type(p).from_buffer_copy(p)
@@ -467,17 +479,17 @@ class ResidualNorm:
 
     def _bind(self) -> None:
         """The calls' parameter blocks with all that does not change from call to call."""
-        where = _places(self.params.values())
+        places = _Places(self.params.values())
         ptrs = {n: _vector(n, t, self.channels, self.dtype, self.device) for n, t in self.params.items() if t is not None}
         common = dict(c=self.channels, pre=NORMS[self.pre], post=NORMS[self.post], eps=self.eps, dtype=_dtype_code(self.dtype))
         self._forward_params = ResidualNormParams(**common, **ptrs)
         ptrs.pop("b_pre", None)
         self._grad_params = ResidualNormGradParams(**common, **ptrs)
-        self._bound = where
+        self._places = places
 
     def _block(self, which: str):
         """A copy of a parameter block, bound to where the vectors are now."""
-        if _places(self.params.values()) != self._bound:
+        if self._places.changed():
             self._bind()
         p = getattr(self, which)
         return type(p).from_buffer_copy(p)
