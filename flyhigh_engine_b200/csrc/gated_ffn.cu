@@ -12,9 +12,12 @@
 // parts. Each waits for the one before on the device (programmatic dependent launch). Few rows (k_rows) and feature maps
 // of few channels (gated_ffn_map.cuh) have forms of their own.
 //
-// At 8192 rows of 2048 -> 8192 -> 2048 in bf16 the first launch takes 338 us with the tensor pipe active 93 % of the time
-// (1,626 TFLOP/s), the second 205 us (71 %: 256 tiles in four turns of 74 CTA pairs); of a training step's gradient da takes
-// 265 us (54 %, at 3.9 TB/s of g, u and their gradients) and the four products after it 985 us (83 %).
+// At 8192 rows of 2048 -> 8192 -> 2048 in bf16 the first launch takes 336 us with the tensor pipe active 93 % of the time
+// (1,636 TFLOP/s), the second 203 us (72 %: 256 tiles in four turns of 74 CTA pairs); of a training step's gradient da takes
+// 267 us (54 %, at 3.8 TB/s of g, u and their gradients) and the four products after it 975 us (84 %).
+//
+// What is rounded to 16 bits is what the next product takes as its operand: a, dg and du (a product of 32-bit operands would be of
+// tf32, at half the rate and twice the bytes). Everything else, g and u among it, stays in 32.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -1069,8 +1072,11 @@ Product down_of(const FhGatedFfnParams& p) {
     return q;
 }
 
-// whether a forward call runs as one kernel (gated_ffn_map.cuh): few channels, and nothing of the hidden values is kept (a alone
-// is kept too: without g and u it cannot serve the gradient, but the caller reads it)
+// Whether a forward call runs as one kernel (gated_ffn_map.cuh): few channels, and nothing of the hidden values is kept (a alone
+// is kept too: without g and u it cannot serve the gradient, but the caller reads it). It needs no scratch, and is the faster
+// where tiles fill the SMs or hidden channels are few (f16, us, this form / tiles: 129,600 x 64 -> 256 32 / 49, 19,000 x 128 ->
+// 16,384 434 / 468, 6480 x 48 -> 192 8.7 / 11.6); few tiles of many hidden channels go through few SMs one chunk after another
+// and are slower by far (1000 x 128 -> 512 16 / 10, 8000 x 128 -> 4096 88 / 58, 64 x 128 -> 16,384 408 / 19).
 bool on_map(const FhGatedFfnParams& p) { return !p.a && !p.g && p.cin <= kMapChannels && p.cout <= kMapChannels; }
 
 template <typename T>

@@ -378,7 +378,8 @@ __global__ void __launch_bounds__(THREADS, kGradThreads / THREADS) k_residual_no
     extern __shared__ uint4 ring_mem[];
     const Ring<T, THREADS, NCH, 4, STAGES> ring{ring_mem};
     // With two chunks a thread, what its registers cannot hold beside the rows: a channel's post factor at [k], sum d and
-    // sum dh at [NCH + k] and [2 NCH + k]. In registers they spilled: 4096 x 8192 with biases 257 us, 230 so
+    // sum dh at [NCH + k] and [2 NCH + k]. In registers more of the row's values spilled: 4096 x 8192 with biases 257 us, 230
+    // so. 64 to 144 bytes a thread still do (404 with whole runs, where those of one chunk spill 16 to 32)
     constexpr bool SHARED = NCH > 1;
     const Kept<THREADS> kept{reinterpret_cast<float4*>(ring_mem + Ring<T, THREADS, NCH, 4, STAGES>::kBytes / 16)};
     const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR;
@@ -726,6 +727,8 @@ cudaError_t forward(const FhResidualNormParams& p, cudaStream_t st) {
     return run_forward<T, 512, 512, 2, 3>(p, st);
 }
 
+// Slices and runs are whole numbers, so gate rows just past a divisor of the CTAs leave up to half of them without work (above 2048
+// channels 75 and 149 gate rows, at 1025 to 2048 or up to 256 channels 150 and 297).
 Split split_of(long long m, int c, int gates, bool gate) {
     Split s{};
     s.groups = gate ? gates : 1;

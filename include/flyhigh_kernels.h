@@ -129,10 +129,11 @@ size_t fhk_gmhs_noalloc_max_floats(void);
  * `channels` values with a row pitch in elements: an NHWC view of contiguous pixels is one, its pitch the pixel pitch
  * cs. Element type FH_F16 or FH_BF16, the same for every tensor of a call (weights, biases and gradients too). Every
  * tensor begins on a 16-byte boundary and pitches are multiples of 8 elements; vectors are contiguous. Elements
- * between a row's channels and its pitch have no influence and are never written. All products, sums, statistics and activations are held in
- * f32. A call runs on the current device and on the given stream, allocates nothing, and leaves nothing behind:
- * scratch is the caller's (16-byte aligned, contents of no meaning before or after), and calls that may overlap need
- * scratch of their own. Results do not depend on timing: every sum has a fixed order. Invalid arguments are refused with
+ * between a row's channels and its pitch have no influence and are never written. All products, sums, statistics and
+ * activations are held in f32. A call runs on the current device and on the given stream, allocates nothing, and leaves
+ * nothing behind: scratch is the caller's (16-byte aligned, contents of no meaning before or after), and calls that may
+ * overlap need scratch of their own. No output overlaps an input or another output, but fhk_residual_norm's y may be its
+ * x. Results do not depend on timing: every sum has a fixed order. Invalid arguments are refused with
  * cudaErrorInvalidValue before anything is launched. */
 #define FH_F16 0
 #define FH_BF16 1
@@ -145,7 +146,8 @@ size_t fhk_gmhs_noalloc_max_floats(void);
 #define FH_ACT_SIGMOID 4   /* the plain gated linear unit */
 
 /* Gated feed-forward block: g = x w_gate^T + b_gate, u = x w_up^T + b_up, a = act(g) * u, y = a w_down^T + b_down.
- * a is rounded to the element type before the down projection. */
+ * a is rounded to the element type before the down projection (f16: infinite beyond 65504). A sigmoid
+ * below 2^-60 is 0. */
 typedef struct FhGatedFfnParams {
     const void* x;         /* [m][cin] */
     const void* w_gate;    /* [hidden][cin] */
@@ -176,7 +178,7 @@ size_t fhk_gated_ffn_scratch_bytes(const FhGatedFfnParams* p);
 /* The block's gradient for dy, from x, the weights and what the forward call kept (g, u, a), or with all three NULL from x,
  * the weights and the biases alone, as they are at this call: g, u and a are formed again (with few channels this costs less
  * than to keep and read them; it always costs less memory).
- * da = dy w_down; dg = da * u * act'(g), du = da * act(g), both rounded to the element type;
+ * da = dy w_down; dg = da * u * act'(g), du = da * act(g), both rounded to the element type (relu' is 0 at a NaN);
  * dx = dg w_gate + du w_up; dw_gate = dg^T x; dw_up = du^T x; dw_down = dy^T a; db_* the column sums of dg, du, dy.
  * Each output may be NULL (not wanted). Every output is written, not added to. With m = 0 the weights' and biases'
  * gradients are set to zero. */
